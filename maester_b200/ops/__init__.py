@@ -13,3 +13,5 @@ from maester_b200.ops.functional import (  # noqa: F401
     rope_table,
     use_native,
 )
+from maester_b200.ops.fp8 import Fp8Blocks, linear_fp8, matmul_fp8, quantize_fp8  # noqa: F401
+from maester_b200.ops.logprobs import TokenLogprobs, linear_logprobs, token_logprobs  # noqa: F401

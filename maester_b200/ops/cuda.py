@@ -6,6 +6,7 @@ bounded wait expires.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -701,3 +702,99 @@ def moe_slot_dot(buf: torch.Tensor, slot_row: torch.Tensor, g: torch.Tensor, k: 
     _ck(_lib.lib().mb_moe_slot_dot(buf.data_ptr(), slot_row.data_ptr(), g.data_ptr(), k, T, dim, buf.shape[0],
                                    out.data_ptr(), _stream()), "moe_slot_dot")
     return out
+
+
+# ------------------------------------------------------------------ token log-probabilities
+_LOGITS_TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_TOP = 64
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (its current stream takes the launches)."""
+    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor | None, scale: float, entropy: bool, top: int, stats: bool):
+    """Rows of ``logits`` [R, V] -> (logprobs | None, entropy | None, top_logprobs | None, top_tokens | None, stats | None)."""
+    R, V = logits.shape
+    f32 = dict(device=logits.device, dtype=torch.float32)
+    lp = torch.empty(R, **f32) if tokens is not None else None
+    ent = torch.empty(R, **f32) if entropy else None
+    top_lp = torch.empty(R, top, **f32) if top else None
+    top_id = torch.empty(R, top, device=logits.device, dtype=torch.int64) if top else None
+    st = torch.empty(R, 4, **f32) if stats else None
+    with on_device(logits):
+        _ck(_lib.lib().mb_logprobs_fwd(logits.data_ptr(), _ptr(tokens), _LOGITS_TYPE[logits.dtype], R, V, logits.stride(0),
+                                       float(scale), _ptr(lp), _ptr(ent), top, _ptr(top_lp), _ptr(top_id), _ptr(st),
+                                       _stream()), "logprobs_fwd")
+    return lp, ent, top_lp, top_id, st
+
+
+def logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor | None, scale: float, stats: torch.Tensor,
+                 g_lp: torch.Tensor | None, g_ent: torch.Tensor | None, top_id: torch.Tensor | None,
+                 g_top: torch.Tensor | None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of the logits; ``out`` (optional, row-major) may be bf16 beside fp32 logits."""
+    R, V = logits.shape
+    if out is None:
+        out = torch.empty(R, V, device=logits.device, dtype=logits.dtype)
+    top = 0 if g_top is None else g_top.shape[1]
+    with on_device(logits):
+        _ck(_lib.lib().mb_logprobs_bwd(logits.data_ptr(), _ptr(tokens), _LOGITS_TYPE[logits.dtype], R, V, logits.stride(0),
+                                       float(scale), stats.data_ptr(), _ptr(g_lp), _ptr(g_ent), top,
+                                       _ptr(top_id) if top else None, _ptr(g_top), out.data_ptr(), _LOGITS_TYPE[out.dtype],
+                                       out.stride(0), _stream()), "logprobs_bwd")
+    return out
+
+
+# ------------------------------------------------------------------ e4m3 with power-of-two block scales
+FP8_ROWS, FP8_COLS, FP8_SQUARE = 1, 2, 4
+FP8_OUT = {torch.bfloat16: 0, torch.float32: 1}
+FP8_OUT_F32_ACC = 2
+
+
+def _fp8_buffers(rows: int, cols: int, device):
+    nb = (cols + 127) // 128
+    codes = torch.empty(rows, nb * 128, device=device, dtype=torch.float8_e4m3fn)
+    return codes, torch.empty((rows + 127) // 128, (nb + 3) // 4, 32, 4, 4, device=device, dtype=torch.uint8)
+
+
+def fp8_quantize(x: torch.Tensor, rows: bool = True, cols: bool = False, square: bool = False):
+    """((codes, scales) of ``x`` | None, (codes, scales) of ``x.T`` | None) from one pass over ``x`` [R, C]."""
+    R, C = x.shape
+    q, sq = _fp8_buffers(R, C, x.device) if rows else (None, None)
+    qt, sqt = _fp8_buffers(C, R, x.device) if cols else (None, None)
+    mode = FP8_ROWS * rows + FP8_COLS * cols + FP8_SQUARE * square
+    with on_device(x):
+        _ck(_lib.lib().mb_fp8_quantize(x.data_ptr(), _LOGITS_TYPE[x.dtype], R, C, x.stride(0), mode, _ptr(q), _ptr(sq),
+                                       _ptr(qt), _ptr(sqt), _stream()), "fp8_quantize")
+    return ((q, sq) if rows else None), ((qt, sqt) if cols else None)
+
+
+def fp8_gemm(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, out: torch.Tensor,
+             accumulate: bool = False) -> torch.Tensor:
+    """``out (+)= A @ B.T`` of codes [M, Kp] and [N, Kp] with packed exponents; ``out`` row-major bf16 or fp32."""
+    M, N = a.shape[0], b.shape[0]
+    assert a.shape[1] == b.shape[1] and a.shape[1] % 128 == 0 and out.shape == (M, N) and out.stride(1) == 1
+    assert not accumulate or out.dtype == torch.float32
+    with on_device(out):
+        _ck(_lib.lib().mb_fp8_gemm(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), out.data_ptr(), M, N,
+                                   a.shape[1] // 128, a.stride(0), b.stride(0), out.stride(0),
+                                   FP8_OUT_F32_ACC if accumulate else FP8_OUT[out.dtype], _stream()), "fp8_gemm")
+    return out
+
+
+# ------------------------------------------------------------------ AdamW over many tensors
+ADAMW_ROW = 48   # bytes of one row of the tensor table: p, g, copy, n, off (8 bytes each), 8 bytes for the launcher
+
+
+def adamw_multi(table, bf16: bool, bits: int, m: torch.Tensor, m_exp: torch.Tensor | None, r: torch.Tensor,
+                r_exp: torch.Tensor | None, hyper: tuple) -> None:
+    """``table``: int64 numpy array [n, 6] of (parameter, gradient, copy, elements, state offset, 0)."""
+    assert table.flags.c_contiguous and table.itemsize * table.shape[1] == ADAMW_ROW
+    h = (ctypes.c_float * 8)(*hyper)
+    with on_device(m):
+        _ck(_lib.lib().mb_adamw_multi(table.ctypes.data, table.shape[0], int(bf16), bits, m.data_ptr(), _ptr(m_exp),
+                                      r.data_ptr(), _ptr(r_exp), h, _stream()), "adamw_multi")

@@ -182,3 +182,120 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, eps: float = 1e-7) -> torch.T
     if transposed:
         x = x.mT
     return x
+
+
+# --------------------------------------------------------------------------- token log-probabilities
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, scale: float = 1.0, entropy: bool = False,
+                   top: int = 0):
+    """``(logprobs, entropy, top_logprobs, top_tokens)`` of the rows of ``logits`` [R, V] (see ``ops.token_logprobs``)."""
+    V = logits.shape[-1]
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    scored = torch.ones(x.shape[0], dtype=torch.bool, device=x.device) if tokens is None else tokens != IGNORE_INDEX
+    if tokens is not None and bool((scored & ((tokens < 0) | (tokens >= V))).any()):
+        raise ValueError(f"token ids have to be in [0, {V}) or {IGNORE_INDEX}")
+    logp = torch.log_softmax(x * scale, dim=-1)
+    lp = ent = top_lp = top_id = None
+    if tokens is not None:
+        at = torch.where(scored, tokens, torch.zeros_like(tokens))
+        lp = torch.where(scored, logp.gather(1, at[:, None])[:, 0], torch.zeros_like(logp[:, 0]))
+    if entropy:
+        p = logp.exp()
+        plogp = torch.where(p == 0, torch.zeros_like(p), p * torch.where(p == 0, torch.zeros_like(logp), logp))
+        ent = torch.where(scored, -plogp.sum(-1), torch.zeros_like(plogp[:, 0]))
+    if top:
+        # a stable descending sort keeps the lowest index of equal values first; NaN sorts above +inf
+        top_id = torch.sort(x.detach() + 0.0, dim=-1, descending=True, stable=True).indices[:, :top]
+        top_lp = torch.where(scored[:, None], logp.gather(1, top_id), torch.full_like(logp[:, :top], -math.inf))
+        top_id = torch.where(scored[:, None], top_id, torch.full_like(top_id, -1))
+    return lp, ent, top_lp, top_id
+
+
+# --------------------------------------------------------------------------- e4m3 with power-of-two block scales
+E4M3_MAX = 448.0
+E4M3_TINY = 2.0 ** -9    # smallest positive code
+FP8_BLOCK = 128          # values of a contraction that share a scale
+FP8_MIN_EXP, FP8_MAX_EXP = -117, 120
+
+
+def pow2(k: torch.Tensor) -> torch.Tensor:
+    """``2^k`` in fp32 for whole ``k`` in [-126, 127] (exact: the exponent field itself)."""
+    return ((k.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def fp8_block_exponents(amax: torch.Tensor, k_min: int) -> torch.Tensor:
+    """Smallest whole ``k`` in [k_min, 120] with ``amax <= 448 * 2^k``."""
+    mant, e = torch.frexp(amax)                       # amax = mant * 2^e with 0.5 <= mant < 1, and 448 = 0.875 * 2^9
+    k = torch.where(mant <= 0.875, e - 9, e - 8)
+    return torch.where(amax > 0, k, torch.full_like(k, k_min)).clamp(k_min, FP8_MAX_EXP)
+
+
+def _finite_abs(x: torch.Tensor) -> torch.Tensor:
+    """|x|, and 0 where x is not finite: infinities and NaN become the NaN code and leave their block's scale alone."""
+    a = x.abs()
+    return torch.where(a <= torch.finfo(torch.float32).max, a, torch.zeros_like(a))
+
+
+def fp8_quantize(x: torch.Tensor, square: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """e4m3 codes [R, C rounded up to 128] and biased exponents uint8 [R, C blocks] of a matrix: one scale for every 128
+    values of a row, or (``square``) for every 128 x 128 tile."""
+    rows, cols = x.shape
+    nb = -(-cols // FP8_BLOCK)
+    f = F.pad(x.float(), (0, nb * FP8_BLOCK - cols)).view(rows, nb, FP8_BLOCK)
+    amax = _finite_abs(f).amax(dim=2)
+    if square:
+        rb = -(-rows // FP8_BLOCK)
+        amax = F.pad(amax, (0, 0, 0, rb * FP8_BLOCK - rows)).view(rb, FP8_BLOCK, nb).amax(dim=1, keepdim=True)
+        amax = amax.expand(rb, FP8_BLOCK, nb).reshape(-1, nb)[:rows]
+    k = fp8_block_exponents(amax, FP8_MIN_EXP)
+    codes = (f * pow2(-k)[:, :, None]).to(torch.float8_e4m3fn).view(rows, nb * FP8_BLOCK)
+    return codes, (k + 127).to(torch.uint8)
+
+
+def fp8_pack_exponents(exps: torch.Tensor) -> torch.Tensor:
+    """[R, blocks] exponent bytes in the order of the block-scaled matrix unit: [R/128, blocks/4, 32, 4, 4] with row
+    ``32 i + j`` of 128 at [j, i] and zeros past the end."""
+    rows, nb = exps.shape
+    rt, kt = -(-rows // 128), -(-nb // 4)
+    full = F.pad(exps, (0, kt * 4 - nb, 0, rt * 128 - rows))
+    return full.view(rt, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).contiguous()
+
+
+def fp8_unpack_exponents(scales: torch.Tensor, rows: int, blocks: int) -> torch.Tensor:
+    rt, kt = scales.shape[:2]
+    return scales.permute(0, 3, 2, 1, 4).reshape(rt * 128, kt * 4)[:rows, :blocks]
+
+
+def fp8_dequantize(codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
+    """fp32 values of codes [R, 128 blocks] with exponents [R, blocks]."""
+    rows, nb = exps.shape
+    return (codes.float().view(rows, nb, FP8_BLOCK) * pow2(exps.to(torch.int32) - 127)[:, :, None]).view(rows, -1)
+
+
+# --------------------------------------------------------------------------- AdamW with 8-bit or 32-bit moments
+STATE_BLOCK = 256        # values of an optimizer state that share a scale
+STATE_MIN_EXP, ROOT_MIN_EXP = -117, -54   # (the square of the smallest root code is still a normal number)
+
+
+def state_encode(x: torch.Tensor, root: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and biased block exponents of a flat state whose length is a multiple of 256; ``root``: a value that is not
+    zero does not become zero."""
+    b = x.view(-1, STATE_BLOCK)
+    k = fp8_block_exponents(_finite_abs(b).amax(dim=1), ROOT_MIN_EXP if root else STATE_MIN_EXP)
+    y = b * pow2(-k)[:, None]
+    if root:
+        y = torch.where(y > 0, y.clamp_min(E4M3_TINY), y)
+    return y.to(torch.float8_e4m3fn).view(-1), (k + 127).to(torch.uint8)
+
+
+def state_decode(codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
+    return (codes.float().view(-1, STATE_BLOCK) * pow2(exps.to(torch.int32) - 127)[:, None]).view(-1)
+
+
+def adamw_multi_step(p: torch.Tensor, g: torch.Tensor, m: torch.Tensor, v: torch.Tensor, *, b1: float, b2: float,
+                     decay: float, step_size: float, inv_root: float, eps: float):
+    """One AdamW step on flat fp32 values, every operation rounded on its own; returns new (p, m, sqrt(v), v).
+    ``decay`` = 1 - lr wd, ``step_size`` = lr / (1 - b1^t), ``inv_root`` = 1 / sqrt(1 - b2^t)."""
+    m = m * b1 + g * (1 - b1)
+    v = v * b2 + g * g * (1 - b2)
+    root = v.sqrt()
+    return p * decay - m / (root * inv_root + eps) * step_size, m, root, v

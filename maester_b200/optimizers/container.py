@@ -89,7 +89,8 @@ class OptimizersContainer(Optimizer, Stateful):
                 for u in sharded.units:
                     u.eager_done = False
             sharded.lowp_fresh = sharded.device.type == "cuda" and all(
-                isinstance(o, FusedAdamW) and o._flat is not None for o in self.optimizers)
+                (isinstance(o, FusedAdamW) and o._flat is not None) or getattr(o, "writes_lowp", False)
+                for o in self.optimizers)
             # every parameter's gradient was consumed and cleared by a kernel that owns it: zero_grad() may skip
             if sharded.grad_cleared_by_optimizer is not None:
                 sharded.grad_cleared_by_optimizer = all(getattr(o, "cleared_grad", False) for o in self.optimizers)
@@ -119,7 +120,9 @@ class OptimizersContainer(Optimizer, Stateful):
         for g in opt.param_groups:
             for p in g["params"]:
                 fqn = self._names.get(id(p), str(id(p)))
-                for k, v in opt.state.get(p, {}).items():
+                # an optimizer that holds its states in another form says what a checkpoint has of a parameter
+                held = opt.param_state(p) if hasattr(opt, "param_state") else opt.state.get(p, {})
+                for k, v in held.items():
                     out[f"state.{fqn}.{k}"] = v
         groups = []
         for g in opt.param_groups:
@@ -137,6 +140,9 @@ class OptimizersContainer(Optimizer, Stateful):
             fqn, _, k = key[len("state."):].rpartition(".")
             p = by_name.get(fqn)
             if p is None:
+                continue
+            if hasattr(opt, "load_param_state"):
+                opt.load_param_state(p, {k: val})
                 continue
             st = opt.state.setdefault(p, {})
             if torch.is_tensor(st.get(k)) and torch.is_tensor(val) and st[k].shape == val.shape:
