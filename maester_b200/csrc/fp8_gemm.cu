@@ -1,52 +1,306 @@
 // C[M,N] = sum over blocks b of 2^(ea[m,b] + eb[n,b]) * sum over the 128 values of block b of A[m,:] B[n,:]
 // for e4m3 codes with block exponents as fp8_blocks.cu writes them.
+//
+// The tensor core applies the scales itself: tcgen05.mma.kind::mxf8f6f4.block_scale multiplies every group of 32 values of the
+// contraction by 2^(ea + eb) on its way into the fp32 accumulator, so the main loop is that of a plain product at the 8-bit
+// rate and no partial sum passes through registers.  A scale covers 128 values here: the four instructions (K = 32) of a
+// 128-deep k-block select the same exponent byte, and one 32-bit word of tensor memory serves four k-blocks.
+//
+// CTA pairs (cta_group::2): a 256 x 256 tile per pair of SMs, each CTA stages its 128 rows of A and its half of B, 128 bytes
+// deep, in a 6-stage ring (32 KiB a stage).  The exponents of four k-blocks (512 bytes for 128 rows, in the order of the
+// matrix unit) come with the first of them and are copied into tensor memory by tcgen05.cp; both CTAs hold those of all
+// 256 rows of B.
+//
+// Tensor memory: two 256-column accumulators and the exponents do not fit 512 columns, so the accumulators share 32: the
+// second starts at column 224, the exponents (two sets, used in turn) are at 480.  The epilogue drains the shared columns
+// first and releases them at once; the other columns are double-buffered as usual.
+//
+// Warp 0: TMA; warp 1: MMA issue (even CTA); warps 2-5: epilogue.  All waits are bounded; both CTAs always reach the cluster
+// barriers.
+#include "gemm_common.cuh"
 #include "host_common.cuh"
-#include "sm100.cuh"
-#include <cuda_fp8.h>
+#include "sm100_pair.cuh"
 
 namespace {
+using namespace mb;
 
 enum { OUT_BF16 = 0, OUT_F32 = 1, OUT_F32_ACC = 2 };
 
-__device__ __forceinline__ float decode(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+constexpr int BM = 128, BN = 256, BNH = 128, BK = 128;   // rows per CTA, tile columns, rows of B per CTA, bytes of K
+constexpr int STAGES = 6;
+constexpr int A_BYTES = BM * BK, B_BYTES = BNH * BK;
+constexpr int SFA_BYTES = 512, SFB_BYTES = 1024;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int SF_BYTES = SFA_BYTES + SFB_BYTES;
+constexpr int SF_STRIDE = 2048;
+constexpr int THREADS = 192;
+constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SF_STRIDE) + 1024 + 256;
+constexpr int GROUP_M = 8;
+constexpr uint32_t ACC1 = 224, SF_COL = 480, SF_SET = 16, SFB_COL = 4;
+
+struct Params {
+  void* C;
+  int M, N, kblocks;
+  long long ldc;
+  int out;
+  int vec;       // 16-byte stores are aligned
+  int* status;
+};
+
+__device__ __forceinline__ void umma2_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
 }
-__device__ __forceinline__ float scale_of(const uint8_t* s, int kt, int row, int blk) {
-  const int byte = s[(static_cast<long long>(row >> 7) * kt + (blk >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (blk & 3)];
-  return byte ? __uint_as_float(static_cast<uint32_t>(byte) << 23) : 0.f;
+// 512 bytes of exponents (32 lanes x 16 bytes) into 4 columns of both CTAs, repeated for the four lane groups
+__device__ __forceinline__ void sf_copy2(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// unswizzled operand of 8-row groups of 16 bytes
+__device__ __forceinline__ uint64_t sf_desc(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>(128 >> 4) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar) & PEER_MASK), "r"(x), "r"(y), "r"(z)
+      : "memory");
 }
 
-__global__ void __launch_bounds__(256) fp8_gemm_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ sa,
-                                                       const uint8_t* __restrict__ b, const uint8_t* __restrict__ sb, void* c,
-                                                       int M, int N, int kblocks, long long lda, long long ldb, long long ldc,
-                                                       int out) {
-  __shared__ float ta[64][33], tb[64][33];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, kt = (kblocks + 3) / 4;
-  float acc[4][4] = {};
-  for (int kb = 0; kb < kblocks; ++kb)
-    for (int k0 = kb * 128; k0 < kb * 128 + 128; k0 += 32) {
-      for (int i = tid; i < 64 * 32; i += 256) {
-        const int r = i >> 5, k = i & 31;
-        ta[r][k] = m0 + r < M ? decode(a[(m0 + r) * lda + k0 + k]) * scale_of(sa, kt, m0 + r, kb) : 0.f;
-        tb[r][k] = n0 + r < N ? decode(b[(n0 + r) * ldb + k0 + k]) * scale_of(sb, kt, n0 + r, kb) : 0.f;
+// e4m3 x e4m3, power-of-two scales, fp32 accumulation; both operands K-major
+constexpr uint32_t idesc_mxf8(int m, int n) {
+  return (1u << 23) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)[32], int row, int col0) {
+  if (row >= p.M || col0 >= p.N) return;
+  MB_CHECK_OR(p.status, row >= 0 && col0 >= 0 && static_cast<long long>(min(col0 + 32, p.N)) <= p.ldc, return);
+  const bool whole = p.vec && col0 + 32 <= p.N;
+  const long long at = static_cast<long long>(row) * p.ldc + col0;
+  if (p.out == OUT_BF16) {
+    __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.C) + at;
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint4 o;
+        o.x = pack_bf16(__uint_as_float(r[j * 8 + 0]), __uint_as_float(r[j * 8 + 1]));
+        o.y = pack_bf16(__uint_as_float(r[j * 8 + 2]), __uint_as_float(r[j * 8 + 3]));
+        o.z = pack_bf16(__uint_as_float(r[j * 8 + 4]), __uint_as_float(r[j * 8 + 5]));
+        o.w = pack_bf16(__uint_as_float(r[j * 8 + 6]), __uint_as_float(r[j * 8 + 7]));
+        reinterpret_cast<uint4*>(c)[j] = o;
       }
-      __syncthreads();
-      for (int k = 0; k < 32; ++k)
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 32; ++i)
+        if (col0 + i < p.N) c[i] = __float2bfloat16(__uint_as_float(r[i]));
+    }
+  } else {
+    float* c = static_cast<float*>(p.C) + at;
+    const bool acc = p.out == OUT_F32_ACC;
+    if (whole) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] += ta[ty * 4 + i][k] * tb[tx * 4 + j][k];
-      __syncthreads();
+      for (int j = 0; j < 8; ++j) {
+        float4 o = make_float4(__uint_as_float(r[j * 4]), __uint_as_float(r[j * 4 + 1]), __uint_as_float(r[j * 4 + 2]),
+                               __uint_as_float(r[j * 4 + 3]));
+        if (acc) {
+          const float4 old = reinterpret_cast<const float4*>(c)[j];
+          o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
+        }
+        reinterpret_cast<float4*>(c)[j] = o;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (col0 + i < p.N) c[i] = (acc ? c[i] : 0.f) + __uint_as_float(r[i]);
     }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m >= M || n >= N) continue;
-      if (out == OUT_BF16) static_cast<__nv_bfloat16*>(c)[m * ldc + n] = __float2bfloat16(acc[i][j]);
-      else if (out == OUT_F32) static_cast<float*>(c)[m * ldc + n] = acc[i][j];
-      else static_cast<float*>(c)[m * ldc + n] += acc[i][j];
+  }
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sf = smem + STAGES * STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sf + STAGES * SF_STRIDE);
+  uint64_t* full = bars;                        // [STAGES] used in the even CTA
+  uint64_t* empty = bars + STAGES;              // [STAGES] one per CTA
+  uint64_t* acc_full = bars + 2 * STAGES;       // [2]      one per CTA
+  uint64_t* acc_empty = bars + 2 * STAGES + 2;  // [2]      used in the even CTA
+  uint64_t* shared_free = bars + 2 * STAGES + 4;  // shared accumulator columns drained (even CTA), one phase per tile
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const int tm = (p.M + 2 * BM - 1) / (2 * BM), tn = (p.N + BN - 1) / BN;
+  const int num_tiles = tm * tn;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    prefetch_tmap(&tmap_sa);
+    prefetch_tmap(&tmap_sb);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 2);
+      mbar_init(&empty[s], 1);
     }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 256);
+    }
+    mbar_init(shared_free, 256);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc2(tmem_slot, 512);
+    tmem_relinquish2();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += npairs) {
+        int mt, nt;
+        mbg::tile_coords(t, tm, tn, GROUP_M, mt, nt);
+        const int m0 = mt * 2 * BM + static_cast<int>(cta) * BM;
+        const int n0 = nt * BN + static_cast<int>(cta) * BNH;
+        for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1)) {
+            atomicCAS(p.status, 0, ERR_WAIT_EMPTY);
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + s * STAGE_BYTES;
+          const bool first = (kb & 3) == 0;
+          mbar_expect_tx_leader(&full[s], STAGE_BYTES + (first ? SF_BYTES : 0));
+          tma_load_2d_pair(sa, &tmap_a, &full[s], kb * BK, m0);
+          tma_load_2d_pair(sa + A_BYTES, &tmap_b, &full[s], kb * BK, n0);
+          if (first) {
+            uint8_t* ss = sf + s * SF_STRIDE;
+            tma_load_3d_pair(ss, &tmap_sa, &full[s], 0, kb >> 2, m0 / 128);
+            tma_load_3d_pair(ss + SFA_BYTES, &tmap_sb, &full[s], 0, kb >> 2, nt * (BN / 128));
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && cta == 0) {
+      constexpr uint32_t idesc = idesc_mxf8(2 * BM, BN);
+      uint32_t it = 0, tcount = 0, group = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += npairs, ++tcount) {
+        const uint32_t acc = tcount & 1;
+        if (!mbar_wait(&acc_empty[acc], ((tcount >> 1) & 1) ^ 1) || (tcount && !mbar_wait(shared_free, (tcount - 1) & 1))) {
+          atomicCAS(p.status, 0, ERR_WAIT_ACC_EMPTY);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + (acc ? ACC1 : 0u);
+        uint32_t sfc = 0;
+        for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&full[s], (it / STAGES) & 1)) {
+            atomicCAS(p.status, 0, ERR_WAIT_FULL);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if ((kb & 3) == 0) {
+            sfc = tmem + SF_COL + (group & 1) * SF_SET;
+            ++group;
+            const uint32_t ss = smem_u32(sf + s * SF_STRIDE);
+            sf_copy2(sfc, sf_desc(ss));
+            sf_copy2(sfc + SFB_COL, sf_desc(ss + SFA_BYTES));
+            sf_copy2(sfc + SFB_COL + 4, sf_desc(ss + SFA_BYTES + 512));
+          }
+          const uint32_t id = idesc | (static_cast<uint32_t>(kb & 3) << 29) | (static_cast<uint32_t>(kb & 3) << 4);
+          const uint32_t sa = smem_u32(smem + s * STAGE_BYTES);
+          const uint64_t da = make_smem_desc(sa, 16, 1024), db = make_smem_desc(sa + A_BYTES, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma2_mxf8(d, smem_desc_advance(da, k * 32), smem_desc_advance(db, k * 32), id, sfc, sfc + SFB_COL,
+                       (kb | k) ? 1u : 0u);
+          umma2_commit_both(&empty[s]);
+        }
+        if (ok) umma2_commit_both(&acc_full[acc]);
+      }
+    }
+  } else {
+    const int q = warp & 3;
+    uint32_t tcount = 0;
+    for (int t = pair; t < num_tiles; t += npairs, ++tcount) {
+      int mt, nt;
+      mbg::tile_coords(t, tm, tn, GROUP_M, mt, nt);
+      const uint32_t acc = tcount & 1;
+      if (!mbar_wait(&acc_full[acc], (tcount >> 1) & 1)) {
+        atomicCAS(p.status, 0, ERR_WAIT_ACC_FULL);
+        break;
+      }
+      tc_fence_after();
+      const int row = mt * 2 * BM + static_cast<int>(cta) * BM + q * 32 + lane;
+      const uint32_t taddr = tmem + (acc ? ACC1 : 0u) + (static_cast<uint32_t>(q * 32) << 16);
+#pragma unroll 1
+      for (int i = 0; i < BN / 32; ++i) {
+        const int c = acc ? i : (i + BN / 32 - 1) % (BN / 32);   // the shared columns first: 7 of the first, 0 of the second
+        uint32_t r[32];
+        tmem_ld_32x32(taddr + c * 32, r);
+        tmem_ld_wait();
+        if (i == 0) {
+          tc_fence_before();
+          mbar_arrive_leader(shared_free);
+        }
+        store_chunk(p, r, row, nt * BN + c * 32);
+      }
+      tc_fence_before();
+      mbar_arrive_leader(&acc_empty[acc]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc2(tmem, 512);
+  }
+}
+
+int make_codes_tmap(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t ld, uint32_t box_rows) {
+  mbh::EncodeTiledFn fn = mbh::encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld};
+  cuuint32_t box[2] = {128, box_rows}, es[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? 0 : -2;
+}
+// exponents: [row tiles][4-block groups][512 bytes]
+int make_scales_tmap(CUtensorMap* m, const void* base, uint64_t row_tiles, uint64_t groups, uint32_t box_tiles) {
+  mbh::EncodeTiledFn fn = mbh::encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[3] = {128, groups, row_tiles}, strides[2] = {512, groups * 512};
+  cuuint32_t box[3] = {128, 1, box_tiles}, es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
 }
 
 }  // namespace
@@ -55,12 +309,47 @@ __global__ void __launch_bounds__(256) fp8_gemm_kernel(const uint8_t* __restrict
 extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb, void* c, int M, int N, int kblocks,
                            long long lda, long long ldb, long long ldc, int out, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  if (kblocks <= 0 || out < 0 || out > 2) return -3;
-  if ((lda & 15) || (ldb & 15) || (reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(b) & 15)) return -3;
-  const dim3 grid((N + 63) / 64, (M + 63) / 64);
-  if (grid.y > 65535) return -3;
-  fp8_gemm_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(sa),
-                                            static_cast<const uint8_t*>(b), static_cast<const uint8_t*>(sb), c, M, N, kblocks,
-                                            lda, ldb, ldc, out);
+  if (kblocks <= 0 || kblocks > (1 << 23) || out < 0 || out > 2) return -3;
+  if ((lda & 15) || (ldb & 15) || (reinterpret_cast<uintptr_t>(a) & 15) || (reinterpret_cast<uintptr_t>(b) & 15) ||
+      (reinterpret_cast<uintptr_t>(sa) & 15) || (reinterpret_cast<uintptr_t>(sb) & 15))
+    return -3;
+  Params p;
+  p.C = c;
+  p.M = M;
+  p.N = N;
+  p.kblocks = kblocks;
+  p.ldc = ldc;
+  p.out = out;
+  p.vec = !(reinterpret_cast<uintptr_t>(c) & 15) && !((ldc * (out == OUT_BF16 ? 2 : 4)) & 15);
+  p.status = mbh::status().dev;
+  if (!p.status) return -4;
+  const long long tiles = static_cast<long long>((M + 255) / 256) * ((N + BN - 1) / BN);
+  if (tiles > 0x7fffffffll / 2) return -3;
+  CUtensorMap ta, tb, tsa, tsb;
+  const uint64_t cols = static_cast<uint64_t>(kblocks) * 128, groups = (kblocks + 3) / 4;
+  int e = make_codes_tmap(&ta, a, cols, M, lda, BM);
+  if (!e) e = make_codes_tmap(&tb, b, cols, N, ldb, BNH);
+  if (!e) e = make_scales_tmap(&tsa, sa, (M + 127) / 128, groups, 1);
+  if (!e) e = make_scales_tmap(&tsb, sb, (N + 127) / 128, groups, 2);
+  if (e) return e;
+  MB_SET_MAX_SMEM_ONCE(fp8_gemm_kernel, SMEM_BYTES);
+  const int max_pairs = mbh::sm_count() / 2;
+  const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * pairs, 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, fp8_gemm_kernel, ta, tb, tsa, tsb, p) != cudaSuccess) {
+    const int e2 = mbh::check_launch("fp8_gemm");
+    return e2 ? e2 : -100;
+  }
   return mbh::check_launch("fp8_gemm");
 }
