@@ -4,8 +4,11 @@
 // a power of two is exact, so every value is rounded once.  Codes: [rows, columns rounded up to 128], the columns past the
 // end are zero.  Exponent bytes come in the order in which the block-scaled tensor-core product takes them: for 128 rows and
 // 4 blocks of the contraction 512 consecutive bytes, row r and block b at 16 (r mod 32) + 4 (r div 32) + b.
+//
 // A thread block owns a 128 x 128 tile of x: it reads it once and writes the codes of x (blocks along a row, or the whole
-// tile as one block), of its transpose (blocks along a column), or of both.
+// tile as one block), of its transpose (blocks along a column), or of both.  A thread holds 8 x 8 values: maxima along rows
+// meet within 16 lanes, maxima along columns through shared memory, and the transposed codes go through a swizzled 16 KiB
+// tile so that both outputs leave as whole 128-byte lines.
 #include "host_common.cuh"
 #include "sm100.cuh"
 #include <cuda_fp8.h>
@@ -15,80 +18,287 @@ namespace {
 constexpr int B = 128;
 enum { ROWS = 1, COLS = 2, SQUARE = 4 };
 
-__device__ __forceinline__ float ld_f(const float* p) { return *p; }
-__device__ __forceinline__ float ld_f(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+constexpr int THREADS = 256;
+constexpr uint32_t INF16 = 0x7f80u, INF32 = 0x7f800000u;
+
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
+// smallest k in [-117, 120] with amax <= 448 * 2^k = 1.75 * 2^(k + 8)
 __device__ __forceinline__ int block_exponent(uint32_t amax_bits) {
   const int e = static_cast<int>(amax_bits >> 23) - 127;
   const int k = (amax_bits & 0x7fffffu) <= 0x600000u ? e - 8 : e - 7;
   return min(max(k, -117), 120);
 }
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
+// e4m3 codes of two values (lo in the low byte); NaN gives the NaN code
+__device__ __forceinline__ uint32_t encode2(float lo, float hi) {
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3));
 }
-__device__ __forceinline__ uint8_t encode(float y) {
-  if (!(fabsf(y) <= 3.4028234e38f)) return 0x7f;
-  return static_cast<uint8_t>(__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3));
+__device__ __forceinline__ float no_inf(float v) { return fabsf(v) <= 3.4028234e38f ? v : __uint_as_float(0x7fffffffu); }
+
+// 8 x 8 values of one thread; maxima are the ordered bits of |x| (16 bits for bf16)
+template <typename T>
+struct Patch;
+
+template <>
+struct Patch<__nv_bfloat16> {
+  uint4 v[8];
+  __device__ __forceinline__ void load_row(int i, const __nv_bfloat16* p, int n, bool vec) {
+    if (vec && n >= 8) {
+      v[i] = __ldg(reinterpret_cast<const uint4*>(p));
+    } else {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) w[j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[j]) << (16 * (j & 1));
+      v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __device__ __forceinline__ void zero_row(int i) { v[i] = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ uint32_t word(int i, int w) const { return w == 0 ? v[i].x : w == 1 ? v[i].y : w == 2 ? v[i].z : v[i].w; }
+  __device__ __forceinline__ float at(int i, int j) const {
+    const uint32_t w = word(i, j >> 1);
+    return __uint_as_float((j & 1) ? (w & 0xffff0000u) : (w << 16));
+  }
+  template <bool SAFE>
+  __device__ __forceinline__ uint32_t mag(int i, int w) const {   // |x| of two neighbours as 16-bit halves
+    uint32_t a = word(i, w) & 0x7fff7fffu;
+    if (!SAFE) {   // something in this tile is not finite: it counts as zero
+      if ((a & 0xffffu) >= INF16) a &= 0xffff0000u;
+      if ((a >> 16) >= INF16) a &= 0x0000ffffu;
+    }
+    return a;
+  }
+  __device__ __forceinline__ bool finite() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) m = __vmaxu2(m, word(i, w) & 0x7fff7fffu);
+    return (m & 0xffffu) < INF16 && (m >> 16) < INF16;
+  }
+  // maxima of the rows over this half-warp's 128 columns: fp32 bits
+  template <bool SAFE>
+  __device__ __forceinline__ void row_max(uint32_t (&am)[8]) const {
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a = __vmaxu2(__vmaxu2(mag<SAFE>(i, 0), mag<SAFE>(i, 1)), __vmaxu2(mag<SAFE>(i, 2), mag<SAFE>(i, 3)));
+      uint32_t b = __vmaxu2(__vmaxu2(mag<SAFE>(i + 4, 0), mag<SAFE>(i + 4, 1)), __vmaxu2(mag<SAFE>(i + 4, 2), mag<SAFE>(i + 4, 3)));
+      p[i] = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));   // row i low, row i + 4 high
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = __vmaxu2(p[i], __shfl_xor_sync(~0u, p[i], o));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      am[i] = p[i] << 16;
+      am[i + 4] = p[i] & 0xffff0000u;
+    }
+  }
+  // maxima of the 8 columns over the whole tile: fp32 bits.  s: 8 warps x 128 x 16 bits
+  template <bool SAFE>
+  __device__ __forceinline__ void col_max(uint32_t (&am)[8], uint32_t* s, int warp, int lane) const {
+    uint32_t p[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      p[w] = mag<SAFE>(0, w);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) p[w] = __vmaxu2(p[w], mag<SAFE>(i, w));
+      p[w] = __vmaxu2(p[w], __shfl_xor_sync(~0u, p[w], 16));
+    }
+    uint4* s4 = reinterpret_cast<uint4*>(s);
+    if (lane < 16) s4[warp * 16 + lane] = make_uint4(p[0], p[1], p[2], p[3]);
+    __syncthreads();
+    uint4 m = s4[lane & 15];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) {
+      const uint4 o = s4[k * 16 + (lane & 15)];
+      m.x = __vmaxu2(m.x, o.x); m.y = __vmaxu2(m.y, o.y); m.z = __vmaxu2(m.z, o.z); m.w = __vmaxu2(m.w, o.w);
+    }
+    am[0] = m.x << 16; am[1] = m.x & 0xffff0000u; am[2] = m.y << 16; am[3] = m.y & 0xffff0000u;
+    am[4] = m.z << 16; am[5] = m.z & 0xffff0000u; am[6] = m.w << 16; am[7] = m.w & 0xffff0000u;
+  }
+};
+
+template <>
+struct Patch<float> {
+  float v[8][8];
+  __device__ __forceinline__ void load_row(int i, const float* p, int n, bool vec) {
+    if (vec && n >= 8) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
+      v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = j < n ? p[j] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void zero_row(int i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+  }
+  __device__ __forceinline__ float at(int i, int j) const { return v[i][j]; }
+  template <bool SAFE>
+  __device__ __forceinline__ uint32_t mag(int i, int j) const {
+    const uint32_t a = __float_as_uint(v[i][j]) & 0x7fffffffu;
+    return SAFE || a < INF32 ? a : 0u;
+  }
+  __device__ __forceinline__ bool finite() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
+    return m < INF32;
+  }
+  template <bool SAFE>
+  __device__ __forceinline__ void row_max(uint32_t (&am)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      am[i] = mag<SAFE>(i, 0);
+#pragma unroll
+      for (int j = 1; j < 8; ++j) am[i] = max(am[i], mag<SAFE>(i, j));
+#pragma unroll
+      for (int o = 8; o; o >>= 1) am[i] = max(am[i], __shfl_xor_sync(~0u, am[i], o));
+    }
+  }
+  // s: 8 warps x 128 x 32 bits
+  template <bool SAFE>
+  __device__ __forceinline__ void col_max(uint32_t (&am)[8], uint32_t* s, int warp, int lane) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      am[j] = mag<SAFE>(0, j);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) am[j] = max(am[j], mag<SAFE>(i, j));
+      am[j] = max(am[j], __shfl_xor_sync(~0u, am[j], 16));
+      if (lane < 16) s[warp * 128 + lane * 8 + j] = am[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      for (int k = 0; k < 8; ++k) am[j] = max(am[j], s[k * 128 + (lane & 15) * 8 + j]);
+  }
+};
+
+// where the exponent byte of row r (of this 128-row tile) and block b (of this group of 4) lies among 512
+__device__ __forceinline__ int scale_at(int r, int b) { return (r & 31) * 16 + (r >> 5) * 4 + b; }
+
+template <typename T, int MODE, bool SAFE>
+__device__ __forceinline__ void quantize_tile(const Patch<T>& x, uint32_t* maxima, uint8_t* tile, int rows, int cols, int rt,
+                                              int ct, int rtiles, int ctiles, uint8_t* q, uint8_t* sq, uint8_t* qt, uint8_t* sqt) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c8 = tid & 15, r8 = tid >> 4;
+  const int r0 = rt * B + r8 * 8, c0 = ct * B + c8 * 8;
+  uint32_t am[8];
+  if (MODE & SQUARE) {
+    x.template row_max<SAFE>(am);
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = max(a, am[i]);
+    a = max(a, __shfl_xor_sync(~0u, a, 16));
+    if (lane == 0) maxima[warp] = a;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a = max(a, maxima[k]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) am[i] = a;
+  }
+  if (MODE & ROWS) {
+    if (!(MODE & SQUARE)) x.template row_max<SAFE>(am);
+    const long long pitch = static_cast<long long>(ctiles) * B;
+    const int kt = (ctiles + 3) / 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = block_exponent(am[i]);
+      if (c8 == i)
+        sq[(static_cast<long long>(rt) * kt + (ct >> 2)) * 512 + scale_at(r8 * 8 + i, ct & 3)] =
+            r0 + i < rows ? static_cast<uint8_t>(k + 127) : 0;
+      const float s = pow2(-k);
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = __fmul_rn(x.at(i, 2 * j), s), b = __fmul_rn(x.at(i, 2 * j + 1), s);
+        w[j] = SAFE ? encode2(a, b) : encode2(no_inf(a), no_inf(b));
+      }
+      if (r0 + i < rows)
+        *reinterpret_cast<uint2*>(q + (r0 + i) * pitch + c0) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    }
+  }
+  if (MODE & COLS) {
+    if (!(MODE & SQUARE)) x.template col_max<SAFE>(am, maxima, warp, lane);
+    const long long pitch = static_cast<long long>(rtiles) * B;
+    const int kt = (rtiles + 3) / 4;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = block_exponent(am[j]);
+      if (r8 == j)
+        sqt[(static_cast<long long>(ct) * kt + (rt >> 2)) * 512 + scale_at(c8 * 8 + j, rt & 3)] =
+            c0 + j < cols ? static_cast<uint8_t>(k + 127) : 0;
+      const float s = pow2(-k);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = __fmul_rn(x.at(2 * i, j), s), b = __fmul_rn(x.at(2 * i + 1, j), s);
+        w[i] = SAFE ? encode2(a, b) : encode2(no_inf(a), no_inf(b));
+      }
+      // 8 rows of column c8 * 8 + j; the 8-byte chunk r8 of that line sits at r8 ^ c8: the 16 lanes fill all banks
+      *reinterpret_cast<uint2*>(tile + (c8 * 8 + j) * B + ((r8 ^ c8) << 3)) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int c = n * 32 + (tid >> 3), part = tid & 7, x8 = c >> 3;
+      uint4 o = *reinterpret_cast<const uint4*>(tile + c * B + ((part ^ (x8 >> 1)) << 4));
+      if (x8 & 1) o = make_uint4(o.z, o.w, o.x, o.y);
+      if (ct * B + c < cols) *reinterpret_cast<uint4*>(qt + (static_cast<long long>(ct) * B + c) * pitch + rt * B + part * 16) = o;
+    }
+  }
+}
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(THREADS) fp8_quantize_kernel(const T* __restrict__ x, int rows, int cols, long long ld, int vec,
+                                                               uint8_t* q, uint8_t* sq, uint8_t* qt, uint8_t* sqt) {
+  __shared__ __align__(16) uint8_t tile[(MODE & COLS) ? B * B : 16];
+  __shared__ __align__(16) uint32_t maxima[(MODE & COLS) ? 8 * 128 : 8];
+  const int rt = blockIdx.y, ct = blockIdx.x, tid = threadIdx.x;
+  const int ctiles = (cols + B - 1) / B, rtiles = (rows + B - 1) / B;
+  if (rt >= rtiles || ct >= ctiles) {  // past the matrix: only the padding of the exponent bytes
+    if (tid < B) {
+      if ((MODE & ROWS) && rt < rtiles)
+        sq[(static_cast<long long>(rt) * ((ctiles + 3) / 4) + (ct >> 2)) * 512 + scale_at(tid, ct & 3)] = 0;
+      if ((MODE & COLS) && ct < ctiles)
+        sqt[(static_cast<long long>(ct) * ((rtiles + 3) / 4) + (rt >> 2)) * 512 + scale_at(tid, rt & 3)] = 0;
+    }
+    return;
+  }
+  Patch<T> p;
+  const int r0 = rt * B + (tid >> 4) * 8, c0 = ct * B + (tid & 15) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (r0 + i < rows && c0 < cols) p.load_row(i, x + (r0 + i) * ld + c0, cols - c0, vec);
+    else p.zero_row(i);
+  }
+  if (__syncthreads_and(p.finite()))
+    quantize_tile<T, MODE, true>(p, maxima, tile, rows, cols, rt, ct, rtiles, ctiles, q, sq, qt, sqt);
+  else
+    quantize_tile<T, MODE, false>(p, maxima, tile, rows, cols, rt, ct, rtiles, ctiles, q, sq, qt, sqt);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, int rows, int cols, long long ld, int mode,
-                                                           uint8_t* q, uint8_t* sq, uint8_t* qt, uint8_t* sqt) {
-  extern __shared__ float tile[];   // [128][129]
-  __shared__ uint32_t am_row[B], am_col[B];
-  const int rt = blockIdx.y, ct = blockIdx.x, tid = threadIdx.x;
-  const int r0 = rt * B, c0 = ct * B;
-  const int ctiles = (cols + B - 1) / B, rtiles = (rows + B - 1) / B;
-  if (tid < B) am_row[tid] = am_col[tid] = 0;
-  __syncthreads();
-  for (int i = tid; i < B * B; i += 256) {
-    const int r = i >> 7, c = i & 127;
-    float v = 0.f;
-    if (r0 + r < rows && c0 + c < cols) v = ld_f(x + static_cast<long long>(r0 + r) * ld + c0 + c);
-    tile[r * 129 + c] = v;
-    const uint32_t b = finite_bits(v);
-    atomicMax(&am_row[r], b);
-    atomicMax(&am_col[c], b);
+int launch(int mode, dim3 grid, cudaStream_t stream, const void* x, int rows, int cols, long long ld, uint8_t* const* o) {
+  const int vec = !(reinterpret_cast<uintptr_t>(x) & 15) && !((ld * static_cast<int>(sizeof(T))) & 15);
+  const T* p = static_cast<const T*>(x);
+  switch (mode) {
+#define CASE(m) case m: fp8_quantize_kernel<T, m><<<grid, THREADS, 0, stream>>>(p, rows, cols, ld, vec, o[0], o[1], o[2], o[3]); break
+    CASE(ROWS);
+    CASE(COLS);
+    CASE(ROWS | COLS);
+    CASE(ROWS | SQUARE);
+    CASE(COLS | SQUARE);
+    CASE(ROWS | COLS | SQUARE);
+#undef CASE
+    default: return -3;
   }
-  __syncthreads();
-  if (mode & SQUARE) {
-    if (tid == 0) {
-      uint32_t a = 0;
-      for (int i = 0; i < B; ++i) a = max(a, am_row[i]);
-      am_row[0] = a;
-    }
-    __syncthreads();
-    const uint32_t a = am_row[0];
-    __syncthreads();
-    if (tid < B) am_row[tid] = am_col[tid] = a;
-    __syncthreads();
-  }
-  const bool in = rt < rtiles && ct < ctiles;
-  if (mode & ROWS) {
-    const long long pitch = static_cast<long long>(ctiles) * B;
-    const int kt = (ctiles + 3) / 4;
-    if (rt < rtiles && tid < B)
-      sq[(static_cast<long long>(rt) * kt + (ct >> 2)) * 512 + (tid & 31) * 16 + (tid >> 5) * 4 + (ct & 3)] =
-          (in && r0 + tid < rows) ? static_cast<uint8_t>(block_exponent(am_row[tid]) + 127) : 0;
-    if (in)
-      for (int i = tid; i < B * B; i += 256) {
-        const int r = i >> 7, c = i & 127;
-        if (r0 + r < rows) q[(r0 + r) * pitch + c0 + c] = encode(__fmul_rn(tile[r * 129 + c], pow2(-block_exponent(am_row[r]))));
-      }
-  }
-  if (mode & COLS) {
-    const long long pitch = static_cast<long long>(rtiles) * B;
-    const int kt = (rtiles + 3) / 4;
-    if (ct < ctiles && tid < B)
-      sqt[(static_cast<long long>(ct) * kt + (rt >> 2)) * 512 + (tid & 31) * 16 + (tid >> 5) * 4 + (rt & 3)] =
-          (in && c0 + tid < cols) ? static_cast<uint8_t>(block_exponent(am_col[tid]) + 127) : 0;
-    if (in)
-      for (int i = tid; i < B * B; i += 256) {
-        const int c = i >> 7, r = i & 127;
-        if (c0 + c < cols) qt[(c0 + c) * pitch + r0 + r] = encode(__fmul_rn(tile[r * 129 + c], pow2(-block_exponent(am_col[c]))));
-      }
-  }
+  return mbh::check_launch("fp8_quantize");
 }
 
 }  // namespace
@@ -104,16 +314,7 @@ extern "C" int mb_fp8_quantize(const void* x, int type, int rows, int cols, long
   // the tiles past the end only write the padding of the exponent bytes
   const int gx = (mode & ROWS) ? (ct + 3) / 4 * 4 : ct, gy = (mode & COLS) ? (rt + 3) / 4 * 4 : rt;
   if (gy > 65535) return -3;
-  const int smem = B * 129 * 4;
   uint8_t* o[4] = {static_cast<uint8_t*>(q), static_cast<uint8_t*>(sq), static_cast<uint8_t*>(qt), static_cast<uint8_t*>(sqt)};
-  if (type == 0) {
-    MB_SET_MAX_SMEM_ONCE(fp8_quantize_kernel<__nv_bfloat16>, smem);
-    fp8_quantize_kernel<<<dim3(gx, gy), 256, smem, stream>>>(static_cast<const __nv_bfloat16*>(x), rows, cols, ld, mode, o[0],
-                                                             o[1], o[2], o[3]);
-  } else {
-    MB_SET_MAX_SMEM_ONCE(fp8_quantize_kernel<float>, smem);
-    fp8_quantize_kernel<<<dim3(gx, gy), 256, smem, stream>>>(static_cast<const float*>(x), rows, cols, ld, mode, o[0], o[1],
-                                                             o[2], o[3]);
-  }
-  return mbh::check_launch("fp8_quantize");
+  return type == 0 ? launch<__nv_bfloat16>(mode, dim3(gx, gy), stream, x, rows, cols, ld, o)
+                   : launch<float>(mode, dim3(gx, gy), stream, x, rows, cols, ld, o);
 }
