@@ -28,62 +28,77 @@ __device__ __forceinline__ int block_exponent(uint32_t amax_bits) {
   const int k = (amax_bits & 0x7fffffu) <= 0x600000u ? e - 8 : e - 7;
   return min(max(k, -117), 120);
 }
-// e4m3 codes of two values (lo in the low byte); NaN gives the NaN code
-__device__ __forceinline__ uint32_t encode2(float lo, float hi) {
-  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3));
+// e4m3 codes of two values (x in the low byte); NaN gives the NaN code
+__device__ __forceinline__ uint32_t encode2(float2 v) {
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3));
 }
-__device__ __forceinline__ float no_inf(float v) { return fabsf(v) <= 3.4028234e38f ? v : __uint_as_float(0x7fffffffu); }
 
-// 8 x 8 values of one thread; maxima are the ordered bits of |x| (16 bits for bf16)
+// 8 x 8 values of one thread.  Maxima are the ordered bits of |x| (16 bits for bf16), over what is finite: a thread that
+// holds an infinity or NaN (seen from its maxima) turns infinities into NaN and takes its maxima again without them.
 template <typename T>
 struct Patch;
 
 template <>
 struct Patch<__nv_bfloat16> {
-  uint4 v[8];
+  uint32_t v[8][4];
   __device__ __forceinline__ void load_row(int i, const __nv_bfloat16* p, int n, bool vec) {
     if (vec && n >= 8) {
-      v[i] = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+      v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
     } else {
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v[i][w] = 0u;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < n) w[j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[j]) << (16 * (j & 1));
-      v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (j < n) v[i][j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(p)[j]) << (16 * (j & 1));
     }
   }
-  __device__ __forceinline__ void zero_row(int i) { v[i] = make_uint4(0u, 0u, 0u, 0u); }
-  __device__ __forceinline__ uint32_t word(int i, int w) const { return w == 0 ? v[i].x : w == 1 ? v[i].y : w == 2 ? v[i].z : v[i].w; }
-  __device__ __forceinline__ float at(int i, int j) const {
-    const uint32_t w = word(i, j >> 1);
-    return __uint_as_float((j & 1) ? (w & 0xffff0000u) : (w << 16));
+  __device__ __forceinline__ void zero_row(int i) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[i][w] = 0u;
   }
-  template <bool SAFE>
-  __device__ __forceinline__ uint32_t mag(int i, int w) const {   // |x| of two neighbours as 16-bit halves
-    uint32_t a = word(i, w) & 0x7fff7fffu;
-    if (!SAFE) {   // something in this tile is not finite: it counts as zero
-      if ((a & 0xffffu) >= INF16) a &= 0xffff0000u;
-      if ((a >> 16) >= INF16) a &= 0x0000ffffu;
+  static __device__ __forceinline__ uint32_t mag(uint32_t w) { return w & 0x7fff7fffu; }
+  static __device__ __forceinline__ bool bad(uint32_t m) { return (m & 0xffffu) >= INF16 || (m >> 16) >= INF16; }
+  static __device__ __forceinline__ uint32_t finite(uint32_t m) {
+    if ((m & 0xffffu) >= INF16) m &= 0xffff0000u;
+    if ((m >> 16) >= INF16) m &= 0x0000ffffu;
+    return m;
+  }
+  template <bool FILTER>
+  __device__ __forceinline__ void thread_rows(uint32_t (&p)[4]) const {   // row i low, row i + 4 high
+    auto f = [](uint32_t w) { return FILTER ? finite(mag(w)) : mag(w); };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = __vmaxu2(__vmaxu2(f(v[i][0]), f(v[i][1])), __vmaxu2(f(v[i][2]), f(v[i][3])));
+      const uint32_t b = __vmaxu2(__vmaxu2(f(v[i + 4][0]), f(v[i + 4][1])), __vmaxu2(f(v[i + 4][2]), f(v[i + 4][3])));
+      p[i] = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
     }
-    return a;
   }
-  __device__ __forceinline__ bool finite() const {
-    uint32_t m = 0;
+  template <bool FILTER>
+  __device__ __forceinline__ void thread_cols(uint32_t (&p)[4]) const {   // columns 2 w (low) and 2 w + 1 (high)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      p[w] = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[w] = __vmaxu2(p[w], FILTER ? finite(mag(v[i][w])) : mag(v[i][w]));
+    }
+  }
+  __device__ __forceinline__ void no_infinities() {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) m = __vmaxu2(m, word(i, w) & 0x7fff7fffu);
-    return (m & 0xffffu) < INF16 && (m >> 16) < INF16;
+      for (int w = 0; w < 4; ++w) {
+        if ((v[i][w] & 0x7fffu) == INF16) v[i][w] |= 0x1u;
+        if ((v[i][w] & 0x7fff0000u) == (INF16 << 16)) v[i][w] |= 0x10000u;
+      }
   }
   // maxima of the rows over this half-warp's 128 columns: fp32 bits
-  template <bool SAFE>
-  __device__ __forceinline__ void row_max(uint32_t (&am)[8]) const {
+  __device__ __forceinline__ void row_max(uint32_t (&am)[8]) {
     uint32_t p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t a = __vmaxu2(__vmaxu2(mag<SAFE>(i, 0), mag<SAFE>(i, 1)), __vmaxu2(mag<SAFE>(i, 2), mag<SAFE>(i, 3)));
-      uint32_t b = __vmaxu2(__vmaxu2(mag<SAFE>(i + 4, 0), mag<SAFE>(i + 4, 1)), __vmaxu2(mag<SAFE>(i + 4, 2), mag<SAFE>(i + 4, 3)));
-      p[i] = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));   // row i low, row i + 4 high
+    thread_rows<false>(p);
+    if (bad(__vmaxu2(__vmaxu2(p[0], p[1]), __vmaxu2(p[2], p[3])))) {
+      no_infinities();
+      thread_rows<true>(p);
     }
 #pragma unroll
     for (int o = 8; o; o >>= 1)
@@ -96,16 +111,15 @@ struct Patch<__nv_bfloat16> {
     }
   }
   // maxima of the 8 columns over the whole tile: fp32 bits.  s: 8 warps x 128 x 16 bits
-  template <bool SAFE>
-  __device__ __forceinline__ void col_max(uint32_t (&am)[8], uint32_t* s, int warp, int lane) const {
+  __device__ __forceinline__ void col_max(uint32_t (&am)[8], uint32_t* s, int warp, int lane) {
     uint32_t p[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      p[w] = mag<SAFE>(0, w);
-#pragma unroll
-      for (int i = 1; i < 8; ++i) p[w] = __vmaxu2(p[w], mag<SAFE>(i, w));
-      p[w] = __vmaxu2(p[w], __shfl_xor_sync(~0u, p[w], 16));
+    thread_cols<false>(p);
+    if (bad(__vmaxu2(__vmaxu2(p[0], p[1]), __vmaxu2(p[2], p[3])))) {
+      no_infinities();
+      thread_cols<true>(p);
     }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) p[w] = __vmaxu2(p[w], __shfl_xor_sync(~0u, p[w], 16));
     uint4* s4 = reinterpret_cast<uint4*>(s);
     if (lane < 16) s4[warp * 16 + lane] = make_uint4(p[0], p[1], p[2], p[3]);
     __syncthreads();
@@ -117,6 +131,33 @@ struct Patch<__nv_bfloat16> {
     }
     am[0] = m.x << 16; am[1] = m.x & 0xffff0000u; am[2] = m.y << 16; am[3] = m.y & 0xffff0000u;
     am[4] = m.z << 16; am[5] = m.z & 0xffff0000u; am[6] = m.w << 16; am[7] = m.w & 0xffff0000u;
+  }
+  // word w of row i times the powers of two s (two bf16; exact down to 2^-126, far below the smallest code): two values
+  __device__ __forceinline__ float2 scaled(int i, int w, uint32_t s) const {
+    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v[i][w]), *reinterpret_cast<__nv_bfloat162*>(&s));
+    const uint32_t b = *reinterpret_cast<const uint32_t*>(&y);
+    return make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
+  }
+  // codes of row i, all with the scale 2^-k
+  __device__ __forceinline__ uint2 row_codes(int i, int k) const {
+    const uint32_t h = static_cast<uint32_t>(127 - k) << 7, s = h | (h << 16);
+    uint32_t c[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) c[w] = encode2(scaled(i, w, s));
+    return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+  }
+  // codes of columns 2 w and 2 w + 1 down the 8 rows, with the scales 2^-k0 and 2^-k1
+  __device__ __forceinline__ void col_codes(int w, int k0, int k1, uint2& c0, uint2& c1) const {
+    const uint32_t s = (static_cast<uint32_t>(127 - k0) << 7) | (static_cast<uint32_t>(127 - k1) << 23);
+    uint32_t a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = scaled(2 * i, w, s), y = scaled(2 * i + 1, w, s);
+      a[i] = encode2(make_float2(x.x, y.x));
+      b[i] = encode2(make_float2(x.y, y.y));
+    }
+    c0 = make_uint2(a[0] | (a[1] << 16), a[2] | (a[3] << 16));
+    c1 = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
   }
 };
 
@@ -137,39 +178,27 @@ struct Patch<float> {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
   }
-  __device__ __forceinline__ float at(int i, int j) const { return v[i][j]; }
-  template <bool SAFE>
-  __device__ __forceinline__ uint32_t mag(int i, int j) const {
+  __device__ __forceinline__ uint32_t mag(int i, int j) const {   // (NaN may stand for an infinity here: neither counts)
     const uint32_t a = __float_as_uint(v[i][j]) & 0x7fffffffu;
-    return SAFE || a < INF32 ? a : 0u;
+    return a < INF32 ? a : 0u;
   }
-  __device__ __forceinline__ bool finite() const {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
-    return m < INF32;
-  }
-  template <bool SAFE>
   __device__ __forceinline__ void row_max(uint32_t (&am)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      am[i] = mag<SAFE>(i, 0);
+      am[i] = mag(i, 0);
 #pragma unroll
-      for (int j = 1; j < 8; ++j) am[i] = max(am[i], mag<SAFE>(i, j));
+      for (int j = 1; j < 8; ++j) am[i] = max(am[i], mag(i, j));
 #pragma unroll
       for (int o = 8; o; o >>= 1) am[i] = max(am[i], __shfl_xor_sync(~0u, am[i], o));
     }
   }
   // s: 8 warps x 128 x 32 bits
-  template <bool SAFE>
   __device__ __forceinline__ void col_max(uint32_t (&am)[8], uint32_t* s, int warp, int lane) const {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      am[j] = mag<SAFE>(0, j);
+      am[j] = mag(0, j);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) am[j] = max(am[j], mag<SAFE>(i, j));
+      for (int i = 1; i < 8; ++i) am[j] = max(am[j], mag(i, j));
       am[j] = max(am[j], __shfl_xor_sync(~0u, am[j], 16));
       if (lane < 16) s[warp * 128 + lane * 8 + j] = am[j];
     }
@@ -178,85 +207,37 @@ struct Patch<float> {
     for (int j = 0; j < 8; ++j)
       for (int k = 0; k < 8; ++k) am[j] = max(am[j], s[k * 128 + (lane & 15) * 8 + j]);
   }
+  // (the conversion would saturate an infinity; the NaN code stands for it)
+  static __device__ __forceinline__ float scaled(float x, float s) {
+    return fabsf(x) <= 3.4028234e38f ? __fmul_rn(x, s) : __uint_as_float(0x7fffffffu);
+  }
+  __device__ __forceinline__ uint2 row_codes(int i, int k) const {
+    const float s = pow2(-k);
+    uint32_t c[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) c[w] = encode2(make_float2(scaled(v[i][2 * w], s), scaled(v[i][2 * w + 1], s)));
+    return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+  }
+  __device__ __forceinline__ uint2 col(int j, int k) const {
+    const float s = pow2(-k);
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = encode2(make_float2(scaled(v[2 * i][j], s), scaled(v[2 * i + 1][j], s)));
+    return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+  }
+  __device__ __forceinline__ void col_codes(int w, int k0, int k1, uint2& c0, uint2& c1) const {
+    c0 = col(2 * w, k0);
+    c1 = col(2 * w + 1, k1);
+  }
 };
 
 // where the exponent byte of row r (of this 128-row tile) and block b (of this group of 4) lies among 512
 __device__ __forceinline__ int scale_at(int r, int b) { return (r & 31) * 16 + (r >> 5) * 4 + b; }
 
-template <typename T, int MODE, bool SAFE>
-__device__ __forceinline__ void quantize_tile(const Patch<T>& x, uint32_t* maxima, uint8_t* tile, int rows, int cols, int rt,
-                                              int ct, int rtiles, int ctiles, uint8_t* q, uint8_t* sq, uint8_t* qt, uint8_t* sqt) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c8 = tid & 15, r8 = tid >> 4;
-  const int r0 = rt * B + r8 * 8, c0 = ct * B + c8 * 8;
-  uint32_t am[8];
-  if (MODE & SQUARE) {
-    x.template row_max<SAFE>(am);
-    uint32_t a = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a = max(a, am[i]);
-    a = max(a, __shfl_xor_sync(~0u, a, 16));
-    if (lane == 0) maxima[warp] = a;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 8; ++k) a = max(a, maxima[k]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) am[i] = a;
-  }
-  if (MODE & ROWS) {
-    if (!(MODE & SQUARE)) x.template row_max<SAFE>(am);
-    const long long pitch = static_cast<long long>(ctiles) * B;
-    const int kt = (ctiles + 3) / 4;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = block_exponent(am[i]);
-      if (c8 == i)
-        sq[(static_cast<long long>(rt) * kt + (ct >> 2)) * 512 + scale_at(r8 * 8 + i, ct & 3)] =
-            r0 + i < rows ? static_cast<uint8_t>(k + 127) : 0;
-      const float s = pow2(-k);
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = __fmul_rn(x.at(i, 2 * j), s), b = __fmul_rn(x.at(i, 2 * j + 1), s);
-        w[j] = SAFE ? encode2(a, b) : encode2(no_inf(a), no_inf(b));
-      }
-      if (r0 + i < rows)
-        *reinterpret_cast<uint2*>(q + (r0 + i) * pitch + c0) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-    }
-  }
-  if (MODE & COLS) {
-    if (!(MODE & SQUARE)) x.template col_max<SAFE>(am, maxima, warp, lane);
-    const long long pitch = static_cast<long long>(rtiles) * B;
-    const int kt = (rtiles + 3) / 4;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = block_exponent(am[j]);
-      if (r8 == j)
-        sqt[(static_cast<long long>(ct) * kt + (rt >> 2)) * 512 + scale_at(c8 * 8 + j, rt & 3)] =
-            c0 + j < cols ? static_cast<uint8_t>(k + 127) : 0;
-      const float s = pow2(-k);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = __fmul_rn(x.at(2 * i, j), s), b = __fmul_rn(x.at(2 * i + 1, j), s);
-        w[i] = SAFE ? encode2(a, b) : encode2(no_inf(a), no_inf(b));
-      }
-      // 8 rows of column c8 * 8 + j; the 8-byte chunk r8 of that line sits at r8 ^ c8: the 16 lanes fill all banks
-      *reinterpret_cast<uint2*>(tile + (c8 * 8 + j) * B + ((r8 ^ c8) << 3)) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-    }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int c = n * 32 + (tid >> 3), part = tid & 7, x8 = c >> 3;
-      uint4 o = *reinterpret_cast<const uint4*>(tile + c * B + ((part ^ (x8 >> 1)) << 4));
-      if (x8 & 1) o = make_uint4(o.z, o.w, o.x, o.y);
-      if (ct * B + c < cols) *reinterpret_cast<uint4*>(qt + (static_cast<long long>(ct) * B + c) * pitch + rt * B + part * 16) = o;
-    }
-  }
-}
-
 template <typename T, int MODE>
-__global__ void __launch_bounds__(THREADS) fp8_quantize_kernel(const T* __restrict__ x, int rows, int cols, long long ld, int vec,
-                                                               uint8_t* q, uint8_t* sq, uint8_t* qt, uint8_t* sqt) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : MODE == (ROWS | COLS) ? 1 : 2)
+fp8_quantize_kernel(const T* __restrict__ src, int rows, int cols, long long ld, int vec, uint8_t* q, uint8_t* sq, uint8_t* qt,
+                    uint8_t* sqt) {
   __shared__ __align__(16) uint8_t tile[(MODE & COLS) ? B * B : 16];
   __shared__ __align__(16) uint32_t maxima[(MODE & COLS) ? 8 * 128 : 8];
   const int rt = blockIdx.y, ct = blockIdx.x, tid = threadIdx.x;
@@ -270,17 +251,70 @@ __global__ void __launch_bounds__(THREADS) fp8_quantize_kernel(const T* __restri
     }
     return;
   }
-  Patch<T> p;
-  const int r0 = rt * B + (tid >> 4) * 8, c0 = ct * B + (tid & 15) * 8;
+  const int lane = tid & 31, warp = tid >> 5, c8 = tid & 15, r8 = tid >> 4;
+  const int r0 = rt * B + r8 * 8, c0 = ct * B + c8 * 8;
+  Patch<T> x;
+  {
+    const T* at = src + r0 * ld + c0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (r0 + i < rows && c0 < cols) p.load_row(i, x + (r0 + i) * ld + c0, cols - c0, vec);
-    else p.zero_row(i);
+    for (int i = 0; i < 8; ++i, at += ld) {
+      if (r0 + i < rows && c0 < cols) x.load_row(i, at, cols - c0, vec);
+      else x.zero_row(i);
+    }
   }
-  if (__syncthreads_and(p.finite()))
-    quantize_tile<T, MODE, true>(p, maxima, tile, rows, cols, rt, ct, rtiles, ctiles, q, sq, qt, sqt);
-  else
-    quantize_tile<T, MODE, false>(p, maxima, tile, rows, cols, rt, ct, rtiles, ctiles, q, sq, qt, sqt);
+  uint32_t am[8];
+  if (MODE & (ROWS | SQUARE)) x.row_max(am);
+  if (MODE & SQUARE) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = max(a, am[i]);
+    a = max(a, __shfl_xor_sync(~0u, a, 16));
+    if (lane == 0) maxima[warp] = a;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a = max(a, maxima[k]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) am[i] = a;
+  }
+  if (MODE & ROWS) {
+    const long long pitch = static_cast<long long>(ctiles) * B;
+    uint8_t* to = q + r0 * pitch + c0;
+    uint8_t* st = sq + (static_cast<long long>(rt) * ((ctiles + 3) / 4) + (ct >> 2)) * 512;
+#pragma unroll
+    for (int i = 0; i < 8; ++i, to += pitch) {
+      const int k = block_exponent(am[i]);
+      if (c8 == i) st[scale_at(r8 * 8 + i, ct & 3)] = r0 + i < rows ? static_cast<uint8_t>(k + 127) : 0;
+      const uint2 c = x.row_codes(i, k);
+      if (r0 + i < rows) *reinterpret_cast<uint2*>(to) = c;
+    }
+  }
+  if (MODE & COLS) {
+    if (!(MODE & SQUARE)) x.col_max(am, maxima, warp, lane);
+    const long long pitch = static_cast<long long>(rtiles) * B;
+    uint8_t* st = sqt + (static_cast<long long>(ct) * ((rtiles + 3) / 4) + (rt >> 2)) * 512;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int k0 = block_exponent(am[2 * w]), k1 = block_exponent(am[2 * w + 1]);
+      if (r8 == w) {
+        st[scale_at(c8 * 8 + 2 * w, rt & 3)] = c0 + 2 * w < cols ? static_cast<uint8_t>(k0 + 127) : 0;
+        st[scale_at(c8 * 8 + 2 * w + 1, rt & 3)] = c0 + 2 * w + 1 < cols ? static_cast<uint8_t>(k1 + 127) : 0;
+      }
+      uint2 a, b;
+      x.col_codes(w, k0, k1, a, b);
+      // 8 rows of a column: the 8-byte chunk r8 of that line sits at r8 ^ c8, so that the 16 lanes fill all banks
+      uint8_t* line = tile + (c8 * 8 + 2 * w) * B + ((r8 ^ c8) << 3);
+      *reinterpret_cast<uint2*>(line) = a;
+      *reinterpret_cast<uint2*>(line + B) = b;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int c = n * 32 + (tid >> 3), part = tid & 7, x8 = c >> 3;
+      uint4 o = *reinterpret_cast<const uint4*>(tile + c * B + ((part ^ (x8 >> 1)) << 4));
+      if (x8 & 1) o = make_uint4(o.z, o.w, o.x, o.y);
+      if (ct * B + c < cols) *reinterpret_cast<uint4*>(qt + (static_cast<long long>(ct) * B + c) * pitch + rt * B + part * 16) = o;
+    }
+  }
 }
 
 template <typename T>
