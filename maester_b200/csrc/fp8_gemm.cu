@@ -156,9 +156,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 256);
+      mbar_init(&acc_empty[a], 8);   // one arrival for each epilogue warp of both CTAs
     }
-    mbar_init(shared_free, 256);
+    mbar_init(shared_free, 8);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -265,12 +265,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         tmem_ld_wait();
         if (i == 0) {
           tc_fence_before();
-          mbar_arrive_leader(shared_free);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_leader(shared_free);
         }
         store_chunk(p, r, row, nt * BN + c * 32);
       }
       tc_fence_before();
-      mbar_arrive_leader(&acc_empty[acc]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_leader(&acc_empty[acc]);
     }
   }
 
