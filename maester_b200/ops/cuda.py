@@ -738,8 +738,10 @@ def logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor | None, scale: float
                  g_top: torch.Tensor | None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of the logits; ``out`` (optional, row-major) may be bf16 beside fp32 logits."""
     R, V = logits.shape
-    if out is None:
-        out = torch.empty(R, V, device=logits.device, dtype=logits.dtype)
+    if out is None:   # rows that lie as the logits' rows do: both are then aligned alike
+        pitch = logits.stride(0) if V <= logits.stride(0) < 2 * V else V
+        out = torch.empty(R, pitch, device=logits.device, dtype=logits.dtype)
+        out = out if pitch == V else out[:, :V]
     top = 0 if g_top is None else g_top.shape[1]
     with on_device(logits):
         _ck(_lib.lib().mb_logprobs_bwd(logits.data_ptr(), _ptr(tokens), _LOGITS_TYPE[logits.dtype], R, V, logits.stride(0),
