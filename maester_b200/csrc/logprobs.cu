@@ -9,10 +9,11 @@
 // Forward: one pass over the logits.  A row belongs to one block of 256 threads, or to a cluster of 2, 4 or 8 of them when
 // rows are few (their partial results meet in the first block's shared memory).  Every thread keeps its own running (max, sum,
 // weighted sum); it takes the maximum of 32 values first, so the sums are rescaled once for 32.
-// The alternatives come out of the same pass: a threshold below which no value can be among the best `top` starts as the
-// top-th largest of the 256 threads' first maxima, and what reaches it (some `top` values of every 8192 at first) goes into a
-// short list of its warp.  A full list is cut down to its best `top`, which raises the threshold for the whole block.  Keys are
-// (ordered value, inverted index), all different: equal values come out by the lowest index, whatever the order of the work.
+// The alternatives need the threads' maxima only: at least `top` values reach the top-th largest of the 256, and hardly more
+// do, so the second look goes to the values of some `top` threads (a 256th of the row each, mostly still in L2).  What
+// reaches that threshold goes into short lists, one a warp; a full list is cut down to its best `top`, which raises the
+// threshold for the whole block.  Entries are (ordered value, inverted index), all different: equal values come out by the
+// lowest index, whatever the order of the work.
 #include "host_common.cuh"
 #include "sm100.cuh"
 #include <cuda_fp16.h>
@@ -50,7 +51,16 @@ struct Vec;
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
+  static constexpr bool PACKED = true;
+  static constexpr float LOWEST = -3.3895314e38f;
   uint32_t w[4];
+  static __device__ __forceinline__ uint32_t both(float v) { return mb::pack_bf16(v, v); }
+  // neighbours 2 i and 2 i + 1, nothing below `low` (NaN stays)
+  __device__ __forceinline__ float2 pair(int i, uint32_t low) const {
+    const __nv_bfloat162 v = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), *reinterpret_cast<const __nv_bfloat162*>(&low));
+    const uint32_t b = *reinterpret_cast<const uint32_t*>(&v);
+    return make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u));
+  }
   __device__ __forceinline__ float at(int i) const { return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16)); }
   // largest value; NaN if there is one
   __device__ __forceinline__ float top() const {
@@ -62,7 +72,16 @@ struct Vec<__nv_bfloat16> {
 template <>
 struct Vec<__half> {
   static constexpr int N = 8;
+  static constexpr bool PACKED = true;
+  static constexpr float LOWEST = -65504.f;
   uint32_t w[4];
+  static __device__ __forceinline__ uint32_t both(float v) {
+    const __half2 h = __float2half2_rn(v);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ __forceinline__ float2 pair(int i, uint32_t low) const {
+    return __half22float2(__hmax2_nan(*reinterpret_cast<const __half2*>(&w[i]), *reinterpret_cast<const __half2*>(&low)));
+  }
   __device__ __forceinline__ float at(int i) const {
     const __half2 v = *reinterpret_cast<const __half2*>(&w[i >> 1]);
     return to_f((i & 1) ? v.y : v.x);
@@ -81,7 +100,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
+  static constexpr bool PACKED = false;
+  static constexpr float LOWEST = 0.f;
   uint32_t w[4];
+  static __device__ __forceinline__ uint32_t both(float) { return 0u; }
+  __device__ __forceinline__ float2 pair(int i, uint32_t) const { return make_float2(at(2 * i), at(2 * i + 1)); }
   __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i]); }
   __device__ __forceinline__ float top() const { return max_nan(max_nan(at(0), at(1)), max_nan(at(2), at(3))); }
 };
@@ -99,11 +122,26 @@ __device__ __forceinline__ uint32_t order_of(float v) {
   const uint32_t b = __float_as_uint(v + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float value_of(uint32_t key) {
-  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
-}
 __device__ __forceinline__ u64 entry_of(float v, uint32_t idx) { return (static_cast<u64>(order_of(v)) << 32) | (0xffffffffu - idx); }
 __device__ __forceinline__ long long index_of(u64 e) { return 0xffffffffu - static_cast<uint32_t>(e); }
+
+// two fp32 operations an instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<u64&>(r))
+      : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)), "l"(reinterpret_cast<u64&>(c)));
+  return r;
+}
 
 // Running (maximum m of x, sum s of exp(scale (x - m)), sum t of (x - m) exp(scale (x - m))).
 struct Sums {
@@ -138,44 +176,63 @@ __device__ __forceinline__ void add_values(Sums& a, const Vec<T> (&v)[U], float 
     }
     a.m = cm == cm ? cm : fmaxf(a.m, 0.f);
   }
-  const float m = a.m;
-  float s = 0.f, t = 0.f;
+  // Two values an instruction.  What is so far below the maximum that its weight is 0 is lifted to a finite value first, so
+  // that -inf does not meet the weight 0 in the entropy's sum; 16-bit logits in packed form where there is room below m
+  const float m = a.m, low = m - fmaxf(far, 0.02f * fabsf(m));
+  float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
+  const float2 nm = make_float2(-m, -m), k2 = make_float2(k, k);
+  if (Vec<T>::PACKED && ENT && low >= Vec<T>::LOWEST) {
+    const uint32_t low2 = Vec<T>::both(low);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int i = 0; i < Vec<T>::N; ++i) {
-      float d = v[u].at(i) - m;
-      const float e = ex2(d * k);
-      s += e;
-      if (ENT) t = fmaf(e, fmaxf(d, -far), t);   // (-inf has weight 0 and must not meet it as 0 * inf)
-    }
+      for (int i = 0; i < Vec<T>::N / 2; ++i) {
+        const float2 d = add2(v[u].pair(i, low2), nm), z = mul2(d, k2), e = make_float2(ex2(z.x), ex2(z.y));
+        s = add2(s, e);
+        t = fma2(e, d, t);
+      }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < Vec<T>::N / 2; ++i) {
+        float2 d = add2(make_float2(v[u].at(2 * i), v[u].at(2 * i + 1)), nm);
+        const float2 z = mul2(d, k2), e = make_float2(ex2(z.x), ex2(z.y));
+        s = add2(s, e);
+        if (ENT) {
+          d.x = fmaxf(d.x, -far);
+          d.y = fmaxf(d.y, -far);
+          t = fma2(e, d, t);
+        }
+      }
   }
-  a.s += s;
-  if (ENT) a.t += t;
+  a.s += s.x + s.y;
+  if (ENT) a.t += t.x + t.y;
 }
 
 // ---- lists of candidates
 struct Lists {
   u64 entry[WARPS][CAP];
-  u64 merged[WARPS * CAP];       // survivors of this block; in the first block of a cluster, the blocks' best
-  alignas(16) uint32_t first[THREADS];   // maxima of the threads' first values
+  alignas(16) u64 merged[WARPS * CAP];   // survivors of this block
   u64 threshold;                 // an entry below it is not among the best
-  uint32_t first_min;
+  uint32_t maxima[THREADS];      // of the threads' values (as ordered whole numbers, 0: none)
+  uint16_t queue[THREADS];       // threads that reach the threshold
+  int queued;
   int count[WARPS];
   int survivors;
 };
 
-// Cut a warp's full list down to its best `top`, best first; their last entry becomes the threshold.
-__device__ __noinline__ void cut_list(Lists& l, int warp, int lane, int top) {
+// Cut a warp's list of n entries (n >= top) down to its best `top`, best first; their last one becomes the threshold.
+__device__ __noinline__ void cut_list(Lists& l, int warp, int lane, int n, int top) {
   u64 mine[CAP / 32];
   int rank[CAP / 32];
 #pragma unroll
   for (int i = 0; i < CAP / 32; ++i) {
-    mine[i] = l.entry[warp][i * 32 + lane];
+    mine[i] = i * 32 + lane < n ? l.entry[warp][i * 32 + lane] : 0;
     rank[i] = 0;
   }
 #pragma unroll 4
-  for (int j = 0; j < CAP; ++j) {
+  for (int j = 0; j < n; ++j) {
     const u64 e = l.entry[warp][j];
 #pragma unroll
     for (int i = 0; i < CAP / 32; ++i) rank[i] += e > mine[i];
@@ -183,45 +240,58 @@ __device__ __noinline__ void cut_list(Lists& l, int warp, int lane, int top) {
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < CAP / 32; ++i) {
-    if (rank[i] < top) l.entry[warp][rank[i]] = mine[i];
-    if (rank[i] == top - 1) atomicMax(&l.threshold, mine[i]);
+    if (mine[i] && rank[i] < top) l.entry[warp][rank[i]] = mine[i];
+    if (mine[i] && rank[i] == top - 1) atomicMax(&l.threshold, mine[i]);
   }
-  if (lane == 0) l.count[warp] = top;
   __syncwarp();
 }
 
-// Values above the threshold go into the warp's list; value i of vector u has index idx0[u] + i, `valid` says which exist.
-// All lanes of the warp call this together.  When the list is full it is cut down and the values that found no room are
-// offered again, against the raised threshold.
-template <typename T, int U>
-__device__ __noinline__ void offer(Lists& l, const Vec<T> (&v)[U], const uint32_t (&idx0)[U], uint32_t valid, int warp, int lane,
-                                   int top) {
-  constexpr int N = Vec<T>::N;
-  uint32_t stored = 0;
-  for (;;) {
-    const u64 thr = *const_cast<volatile u64*>(&l.threshold);
-    uint32_t left = 0;
+// Largest key that at least `top` of the 256 maxima reach (0: fewer have a value).  One warp.
+__device__ __forceinline__ uint32_t top_of_maxima(const uint32_t* maxima, int lane, int top) {
+  uint32_t key[THREADS / 32], t = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+  for (int i = 0; i < THREADS / 32; ++i) key[i] = maxima[i * 32 + lane];
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = t | (1u << bit);
+    int n = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t bit = 1u << (u * N + i);
-        if (!(valid & bit) || (stored & bit)) continue;
-        const u64 e = entry_of(v[u].at(i), idx0[u] + i);
-        if (e <= thr) continue;
-        const int at = atomicAdd(&l.count[warp], 1);
-        if (at < CAP) {
-          l.entry[warp][at] = e;
-          stored |= bit;
-        } else {
-          left |= bit;
-        }
-      }
-    __syncwarp();
-    if (*const_cast<volatile int*>(&l.count[warp]) < CAP) return;   // (a list that is just full is cut as well)
-    cut_list(l, warp, lane, top);
-    if (!__any_sync(~0u, left)) return;
+    for (int i = 0; i < THREADS / 32; ++i) n += __popc(__ballot_sync(~0u, key[i] >= c));
+    if (n >= top) t = c;
   }
+  return t;
+}
+
+// Values above the threshold go into the warp's list (n entries, returned).  Every lane brings a vector whose first value has
+// index j0 (valid: there is one).  The whole warp calls this together and looks at one vector at a time, a value per lane.
+template <typename T>
+__device__ __forceinline__ int offer(Lists& l, const Vec<T>& v, bool valid, uint32_t j0, int n, int warp, int lane, int top) {
+  constexpr int N = Vec<T>::N;
+  u64 thr = *const_cast<volatile u64*>(&l.threshold);
+  // the best entry that the vector can hold: its maximum at its first index
+  const u64 most = valid ? entry_of(v.top(), j0) : 0;
+  for (uint32_t h = __ballot_sync(~0u, most > thr); h; h &= h - 1) {
+    const int from = __ffs(h) - 1;
+    if (__shfl_sync(~0u, most, from) <= thr) continue;    // (a cut has raised the threshold)
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __shfl_sync(~0u, v.w[i], from);
+    const uint32_t first = __shfl_sync(~0u, j0, from);
+    const int i = lane & (N - 1), word = N == 8 ? i >> 1 : i;
+    Vec<T> mine;
+    mine.w[0] = word == 0 ? w[0] : word == 1 ? w[1] : word == 2 ? w[2] : w[3];
+    const u64 e = entry_of(N == 8 && (i & 1) ? mine.at(1) : mine.at(0), first + i);
+    const bool keep = lane < N && e > thr;
+    const uint32_t kept = __ballot_sync(~0u, keep);
+    if (keep) l.entry[warp][n + __popc(kept & ((1u << lane) - 1u))] = e;
+    n += __popc(kept);
+    if (n > CAP - N) {
+      __syncwarp();
+      cut_list(l, warp, lane, n, top);
+      n = top;
+      thr = *const_cast<volatile u64*>(&l.threshold);
+    }
+  }
+  return n;
 }
 
 // Best `top` entries of the block, best first, into out (missing ones 0).  All threads call this; a barrier is inside.
@@ -238,10 +308,16 @@ __device__ __forceinline__ void block_best(Lists& l, u64* out, int top, int tid)
   if (tid < top) out[tid] = 0;
   __syncthreads();
   const int n = l.survivors;
+  if (tid == 0 && (n & 1)) l.merged[n] = 0;     // (an odd n is below the array's size)
+  __syncthreads();
   for (int i = tid; i < n; i += THREADS) {
     const u64 e = l.merged[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += l.merged[j] > e;
+#pragma unroll 4
+    for (int j = 0; j < n; j += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&l.merged[j]);
+      rank += (o.x > e) + (o.y > e);
+    }
     if (rank < top) out[rank] = e;
   }
   __syncthreads();
@@ -302,26 +378,18 @@ logprobs_fwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
   const T* xv = xr + head;
   Sums a{-INFINITY, 0.f, 0.f};
   if (TOP) {
-    if (tid < WARPS) l.count[tid] = 0;
-    if (tid == 0) {
-      l.survivors = 0;
-      l.threshold = 0;
-      l.first_min = 0xffffffffu;
-    }
+    if (tid == 0) l.survivors = l.queued = 0;
   }
-  // one value of a ragged end for some threads of the first block
-  Vec<T> edge[1];
-  uint32_t edge_at[1] = {0u};
+  // one value of a ragged end for some lanes of the first warp of the first block
+  float edge_v = -INFINITY;
+  uint32_t edge_at = 0;
   bool has_edge = false;
   {
-    const int tail0 = head + vectors * N, ends = head + V - tail0;
+    const int tail0 = head + vectors * N, ends = head + V - tail0;   // (at most 14)
     if (block == 0 && tid < ends) {
-      const int j = tid < head ? tid : tail0 + tid - head;
-      const float v = to_f(xr[j]);
+      edge_at = tid < head ? tid : tail0 + tid - head;
       has_edge = true;
-      edge_at[0] = j;
-      edge[0].w[0] = sizeof(T) == 4 ? __float_as_uint(v) : static_cast<uint32_t>(reinterpret_cast<const unsigned short*>(xr)[j]);
-      edge[0].w[1] = edge[0].w[2] = edge[0].w[3] = 0u;
+      const float v = edge_v = to_f(xr[edge_at]);
       if (v != -INFINITY) {
         a.m = v == v ? v : 0.f;
         const float e = ex2((v - a.m) * k);
@@ -330,22 +398,19 @@ logprobs_fwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
       }
     }
   }
-  bool first = true;
-  for (int i0 = v0; i0 < v1 || (TOP && first); i0 += THREADS * U) {
+  float most = edge_v;    // largest value of this thread; NaN if there is one
+  for (int i0 = v0; i0 < v1; i0 += THREADS * U) {
     Vec<T> v[U];
-    uint32_t idx0[U], valid = 0;
     float cm = -INFINITY;
     if (i0 + THREADS * U <= v1) {
 #pragma unroll
       for (int u = 0; u < U; ++u) v[u] = load_vec(xv + static_cast<long long>(i0 + u * THREADS + tid) * N);
-      valid = (U * N == 32) ? ~0u : (1u << (U * N)) - 1u;
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = i0 + u * THREADS + tid;
         if (at < v1) {
           v[u] = load_vec(xv + static_cast<long long>(at) * N);
-          valid |= ((1u << N) - 1u) << (u * N);
         } else {   // -inf: no weight
           const uint32_t none = sizeof(T) == 4 ? 0xff800000u : sizeof(T) == 2 && __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
           v[u].w[0] = v[u].w[1] = v[u].w[2] = v[u].w[3] = none;
@@ -353,33 +418,8 @@ logprobs_fwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      idx0[u] = static_cast<uint32_t>(head + (i0 + u * THREADS + tid) * N);
-      cm = max_nan(cm, v[u].top());
-    }
-    if (TOP && first) {
-      // the top-th largest of the threads' maxima: at least `top` values reach it
-      const float edge_v = has_edge ? edge[0].at(0) : -INFINITY;
-      l.first[tid] = valid || has_edge ? order_of(max_nan(cm, edge_v)) : 0u;
-      __syncthreads();
-      const uint32_t mine = l.first[tid];
-      int above = 0;
-#pragma unroll 4
-      for (int j = 0; j < THREADS; j += 4) {
-        const uint4 o = *reinterpret_cast<const uint4*>(&l.first[j]);
-        above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
-      }
-      if (above < top) atomicMin(&l.first_min, mine);
-      __syncthreads();
-      if (tid == 0 && l.first_min) l.threshold = (static_cast<u64>(l.first_min) << 32) - 1;
-      __syncthreads();
-      first = false;
-      if (__any_sync(~0u, has_edge)) offer<T, 1>(l, edge, edge_at, has_edge ? 1u : 0u, warp, lane, top);
-    }
-    if (TOP) {
-      const u64 thr = *const_cast<volatile u64*>(&l.threshold);
-      if (__any_sync(~0u, valid && !(cm < value_of(static_cast<uint32_t>(thr >> 32))))) offer<T, U>(l, v, idx0, valid, warp, lane, top);
-    }
+    for (int u = 0; u < U; ++u) cm = max_nan(cm, v[u].top());
+    if (TOP) most = max_nan(most, cm);
     add_values<T, U, ENT>(a, v, cm, k, far);
   }
 #pragma unroll
@@ -391,8 +431,46 @@ logprobs_fwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
     a = merge(a, b, k, far);
   }
   if (lane == 0) parts[warp] = a;
-  if (TOP) block_best(l, best, top, tid);
-  else __syncthreads();
+  if (TOP) {
+    const uint32_t key = v0 + tid < v1 || has_edge ? order_of(most) : 0u;
+    l.maxima[tid] = key;
+    __syncthreads();
+    if (warp == 0) {
+      const uint32_t t = top_of_maxima(l.maxima, lane, top);
+      if (lane == 0) l.threshold = t ? (static_cast<u64>(t) << 32) - 1 : 0;   // (every entry of that value is above it)
+    }
+    __syncthreads();
+    const u64 thr = l.threshold;
+    if (key && key > static_cast<uint32_t>(thr >> 32)) l.queue[atomicAdd(&l.queued, 1)] = static_cast<uint16_t>(tid);
+    __syncthreads();
+    int listed = 0;
+    if (warp == 0) {   // the ragged ends: at most 14 values
+      const u64 e = has_edge ? entry_of(edge_v, edge_at) : 0;
+      const uint32_t kept = __ballot_sync(~0u, e > thr);
+      if (e > thr) l.entry[0][__popc(kept & ((1u << lane) - 1u))] = e;
+      listed = __popc(kept);
+    }
+    const int turns = (v1 - v0 + THREADS - 1) / THREADS, items = l.queued * turns;   // (at most the block's vectors and 255)
+    for (int i0 = warp * 32; i0 < items; i0 += THREADS * 2) {
+      Vec<T> v[2];
+      uint32_t j0[2];
+      bool valid[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int item = i0 + u * THREADS + lane, q = item / turns;
+        const int at = item < items ? v0 + l.queue[q] + (item - q * turns) * THREADS : v1;
+        valid[u] = at < v1;
+        j0[u] = static_cast<uint32_t>(head + at * N);
+        if (valid[u]) v[u] = load_vec(xv + static_cast<long long>(at) * N);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) listed = offer<T>(l, v[u], valid[u], j0[u], listed, warp, lane, top);
+    }
+    if (lane == 0) l.count[warp] = listed;
+    block_best(l, best, top, tid);
+  } else {
+    __syncthreads();
+  }
   a = parts[0];
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) a = merge(a, parts[w], k, far);
