@@ -6,9 +6,11 @@
 // Statistics are 32-bit whatever the type of the logits.  -inf logits have probability 0 and gradient 0; a row without a
 // finite logit, or with NaN or +inf, has no distribution and comes out as NaN.
 //
-// Forward: one pass over the logits.  A row belongs to one block of 256 threads, or to a cluster of 2, 4 or 8 of them when
-// rows are few (their partial results meet in the first block's shared memory).  Every thread keeps its own running (max, sum,
-// weighted sum); it takes the maximum of 32 values first, so the sums are rescaled once for 32.
+// Forward: one pass over the logits by resident blocks of 256 threads that take row after row; with few rows a cluster of 2, 4
+// or 8 blocks shares each (their results meet in the first block's shared memory).  Every thread copies its own next vectors
+// into its own slots of shared memory (cp.async), STAGES turns ahead and across the ends of rows, so that loads go on while a
+// row's results are put together; no thread waits for another's copy.  It keeps its own running (max, sum, weighted sum) and
+// takes the maximum of 32 values first, so the sums are rescaled once for 32.
 // The alternatives need the threads' maxima only: at least `top` values reach the top-th largest of the 256, and hardly more
 // do, so the second look goes to the values of some `top` threads (a 256th of the row each, mostly still in L2).  What
 // reaches that threshold goes into short lists, one a warp; a full list is cut down to its best `top`, which raises the
@@ -26,7 +28,10 @@ constexpr int MAX_TOP = 64;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float FAR = 1000.f;      // exp(-1000) is 0 in fp32: distances are cut there so that a weight of 0 never meets infinity
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int CAP = 128;           // entries of a warp's list
+constexpr int CAP = 96;            // entries of a warp's list: more than MAX_TOP and a vector
+constexpr int TURN = 4;            // vectors of a thread's turn
+constexpr int STAGES = 2;          // turns in flight
+constexpr int RESIDENT = 4;        // blocks of an SM
 constexpr int MAX_CLUSTER = 8;
 typedef unsigned long long u64;
 
@@ -121,6 +126,9 @@ __device__ __forceinline__ uint32_t order_of(float v) {
   if (v != v) return 0xffffffffu;
   const uint32_t b = __float_as_uint(v + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 __device__ __forceinline__ u64 entry_of(float v, uint32_t idx) { return (static_cast<u64>(order_of(v)) << 32) | (0xffffffffu - idx); }
 __device__ __forceinline__ long long index_of(u64 e) { return 0xffffffffu - static_cast<uint32_t>(e); }
@@ -224,6 +232,7 @@ struct Lists {
 
 // Cut a warp's list of n entries (n >= top) down to its best `top`, best first; their last one becomes the threshold.
 __device__ __noinline__ void cut_list(Lists& l, int warp, int lane, int n, int top) {
+  static_assert(CAP % 32 == 0 && CAP >= MAX_TOP + 16, "");
   u64 mine[CAP / 32];
   int rank[CAP / 32];
 #pragma unroll
@@ -308,8 +317,12 @@ __device__ __forceinline__ void block_best(Lists& l, u64* out, int top, int tid)
   if (tid < top) out[tid] = 0;
   __syncthreads();
   const int n = l.survivors;
-  if (tid == 0 && (n & 1)) l.merged[n] = 0;     // (an odd n is below the array's size)
+  if (tid == 0) {
+    if (n & 1) l.merged[n] = 0;     // (an odd n is below the array's size)
+    l.queued = 0;
+  }
   __syncthreads();
+  if (tid == 0) l.survivors = 0;
   for (int i = tid; i < n; i += THREADS) {
     const u64 e = l.merged[i];
     int rank = 0;
@@ -336,182 +349,260 @@ __device__ __forceinline__ uint32_t in_block(const void* p, uint32_t block) {   
   return a;
 }
 
+// The part of a row that a block reads: vectors [v0, v1) counted from the first 16-byte boundary, `head` values into the row.
+template <typename T>
+struct Part {
+  const T* row;
+  int head, vectors, v0, v1;
+  __device__ __forceinline__ Part(const T* x, int V, int blocks, int block) : row(x) {
+    head = min(V, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+    vectors = (V - head) / Vec<T>::N;
+    const int per = (vectors + blocks - 1) / blocks;
+    v0 = min(vectors, block * per);
+    v1 = min(vectors, v0 + per);
+  }
+};
+
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mb::smem_u32(to)), "l"(from) : "memory");
+}
+
+struct FwdArgs {
+  const long long* tokens;
+  int rows, V;
+  long long ld;
+  float scale;
+  int blocks;                // of a row
+  float *logprob, *entropy;
+  int top;
+  float* top_lp;
+  long long* top_id;
+  float4* stats;
+  int* status;
+};
+
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(THREADS, 4)
-logprobs_fwd_kernel(const T* __restrict__ x, const long long* __restrict__ tokens, int V, long long ld, float scale, int blocks,
-                    float* __restrict__ logprob, float* __restrict__ entropy, int top, float* __restrict__ top_lp,
-                    long long* __restrict__ top_id, float4* __restrict__ stats, int* status) {
-  constexpr int N = Vec<T>::N, U = 4;
-  __shared__ Sums parts[WARPS];
-  __shared__ Sums block_parts[MAX_CLUSTER];       // first block: one of each block of the cluster
-  __shared__ __align__(16) uint8_t lists_raw[TOP ? sizeof(Lists) : 16];
+__global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T* __restrict__ x, const FwdArgs p) {
+  constexpr int N = Vec<T>::N, U = TURN;
+  __shared__ Sums parts[2][WARPS];                   // (by turns of rows: a row's are read while the next one's are made)
+  __shared__ Sums block_parts[2][MAX_CLUSTER];       // first block: one of each block of the cluster
+  __shared__ u64 block_best_of[TOP ? 2 : 1][TOP ? MAX_CLUSTER * MAX_TOP : 1];
   __shared__ u64 best[TOP ? MAX_TOP : 1];
-  __shared__ u64 block_best_of[TOP ? MAX_CLUSTER * MAX_TOP : 1];
-  Lists& l = *reinterpret_cast<Lists*>(lists_raw);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t block = blocks > 1 ? cluster_rank() : 0u;
-  const long long row = blockIdx.x / blocks;
-  const long long tok = tokens ? tokens[row] : 0;
-  if (tok < 0 || tok >= V) {     // (the same for every block of the row)
-    if (block == 0) {
-      const float v = tok == IGNORE ? 0.f : NAN;
-      if (tok != IGNORE && tid == 0) atomicCAS(status, 0, mb::ERR_BAD_ARG);
-      if (tid == 0) {
-        logprob[row] = v;
-        if (entropy) entropy[row] = v;
-        if (stats) stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+  extern __shared__ __align__(16) uint8_t dynamic[];
+  uint4* slots = reinterpret_cast<uint4*>(dynamic);  // [STAGES][U][THREADS]
+  Lists& l = *reinterpret_cast<Lists*>(dynamic + STAGES * U * THREADS * 16);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, blocks = p.blocks, top = p.top;
+  const int block = blocks > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const long long first = blockIdx.x / blocks, step = gridDim.x / blocks;
+  const float scale = p.scale, k = scale * LOG2E, far = fminf(FAR / scale, 3e38f);
+  auto skipped = [&](long long row) {
+    const long long t = p.tokens ? __ldg(p.tokens + row) : 0;
+    return t < 0 || t >= V;
+  };
+  if (TOP && tid == 0) l.survivors = l.queued = 0;
+  if (blocks > 1) {   // every block of the cluster has started before anything is stored into one
+    cluster_arrive();
+    cluster_wait();
+  }
+
+  // ---- copies: the turns of this block's rows one after the other
+  long long load_row = first;
+  int load_at = 0, load_end = 0, load_stage = 0;
+  const T* load_from = nullptr;
+  auto next_loads = [&]() {      // the next row that has something for this block
+    while (load_row < p.rows) {
+      if (!skipped(load_row)) {
+        const Part<T> q(x + load_row * p.ld, V, blocks, block);
+        if (q.v0 < q.v1) {
+          load_from = q.row + q.head;
+          load_at = q.v0;
+          load_end = q.v1;
+          return;
+        }
       }
-      for (int j = tid; j < top; j += THREADS) {
-        top_lp[row * top + j] = -INFINITY;
-        top_id[row * top + j] = -1;
-      }
+      load_row += step;
     }
-    return;
-  }
-  if (blocks > 1) cluster_arrive();   // (waited for before the first store into another block: it has started by then)
-  const T* xr = x + row * ld;
-  const float k = scale * LOG2E, far = fminf(FAR / scale, 3e38f);
-  // vectors start at the first 16-byte boundary of the row; what lies before it and behind the last one goes one by one
-  const int head = min(V, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / sizeof(T)));
-  const int vectors = (V - head) / N, per = (vectors + blocks - 1) / blocks;
-  const int v0 = min(vectors, static_cast<int>(block) * per), v1 = min(vectors, v0 + per);
-  const T* xv = xr + head;
-  Sums a{-INFINITY, 0.f, 0.f};
-  if (TOP) {
-    if (tid == 0) l.survivors = l.queued = 0;
-  }
-  // one value of a ragged end for some lanes of the first warp of the first block
-  float edge_v = -INFINITY;
-  uint32_t edge_at = 0;
-  bool has_edge = false;
-  {
-    const int tail0 = head + vectors * N, ends = head + V - tail0;   // (at most 14)
-    if (block == 0 && tid < ends) {
-      edge_at = tid < head ? tid : tail0 + tid - head;
-      has_edge = true;
-      const float v = edge_v = to_f(xr[edge_at]);
-      if (v != -INFINITY) {
-        a.m = v == v ? v : 0.f;
-        const float e = ex2((v - a.m) * k);
-        a.s = e;
-        a.t = e * (v - a.m);
-      }
-    }
-  }
-  float most = edge_v;    // largest value of this thread; NaN if there is one
-  for (int i0 = v0; i0 < v1; i0 += THREADS * U) {
-    Vec<T> v[U];
-    float cm = -INFINITY;
-    if (i0 + THREADS * U <= v1) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = load_vec(xv + static_cast<long long>(i0 + u * THREADS + tid) * N);
-    } else {
+  };
+  auto copy_turn = [&]() {
+    if (load_row < p.rows) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = i0 + u * THREADS + tid;
-        if (at < v1) {
-          v[u] = load_vec(xv + static_cast<long long>(at) * N);
-        } else {   // -inf: no weight
-          const uint32_t none = sizeof(T) == 4 ? 0xff800000u : sizeof(T) == 2 && __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
-          v[u].w[0] = v[u].w[1] = v[u].w[2] = v[u].w[3] = none;
+        const int at = load_at + u * THREADS + tid;
+        if (at < load_end) copy16(&slots[(load_stage * U + u) * THREADS + tid], load_from + static_cast<long long>(at) * N);
+      }
+      load_at += THREADS * U;
+      if (load_at >= load_end) {
+        load_row += step;
+        next_loads();
+      }
+    }
+    load_stage = load_stage + 1 == STAGES ? 0 : load_stage + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  next_loads();
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) copy_turn();
+
+  int stage = 0, phase = 0;
+  for (long long row = first; row < p.rows; row += step) {
+    const long long tok = p.tokens ? __ldg(p.tokens + row) : 0;
+    if (tok < 0 || tok >= V) {     // (the same for every block of the row)
+      if (block == 0) {
+        const float v = tok == IGNORE ? 0.f : NAN;
+        if (tok != IGNORE && tid == 0) atomicCAS(p.status, 0, mb::ERR_BAD_ARG);
+        if (tid == 0) {
+          p.logprob[row] = v;
+          if (p.entropy) p.entropy[row] = v;
+          if (p.stats) p.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (TOP && tid < top) {
+          p.top_lp[row * top + tid] = -INFINITY;
+          p.top_id[row * top + tid] = -1;
+        }
+      }
+      continue;
+    }
+    const Part<T> q(x + row * p.ld, V, blocks, block);
+    const float at_token = tid == 0 ? to_f(q.row[tok]) : 0.f;
+    Sums a{-INFINITY, 0.f, 0.f};
+    // one value of a ragged end for some lanes of the first warp of the first block
+    float edge_v = -INFINITY;
+    int edge_at = 0;
+    bool has_edge = false;
+    {
+      const int tail0 = q.head + q.vectors * N, ends = q.head + V - tail0;   // (at most 14)
+      if (block == 0 && tid < ends) {
+        edge_at = tid < q.head ? tid : tail0 + tid - q.head;
+        has_edge = true;
+        const float v = edge_v = to_f(q.row[edge_at]);
+        if (v != -INFINITY) {
+          a.m = v == v ? v : 0.f;
+          const float e = ex2((v - a.m) * k);
+          a.s = e;
+          a.t = e * (v - a.m);
         }
       }
     }
+    float most = edge_v;    // largest value of this thread; NaN if there is one
+    for (int i0 = q.v0; i0 < q.v1; i0 += THREADS * U) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      Vec<T> v[U];
+      float cm = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) cm = max_nan(cm, v[u].top());
-    if (TOP) most = max_nan(most, cm);
-    add_values<T, U, ENT>(a, v, cm, k, far);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    Sums b;
-    b.m = __shfl_xor_sync(~0u, a.m, o);
-    b.s = __shfl_xor_sync(~0u, a.s, o);
-    b.t = __shfl_xor_sync(~0u, a.t, o);
-    a = merge(a, b, k, far);
-  }
-  if (lane == 0) parts[warp] = a;
-  if (TOP) {
-    const uint32_t key = v0 + tid < v1 || has_edge ? order_of(most) : 0u;
-    l.maxima[tid] = key;
-    __syncthreads();
-    if (warp == 0) {
-      const uint32_t t = top_of_maxima(l.maxima, lane, top);
-      if (lane == 0) l.threshold = t ? (static_cast<u64>(t) << 32) - 1 : 0;   // (every entry of that value is above it)
-    }
-    __syncthreads();
-    const u64 thr = l.threshold;
-    if (key && key > static_cast<uint32_t>(thr >> 32)) l.queue[atomicAdd(&l.queued, 1)] = static_cast<uint16_t>(tid);
-    __syncthreads();
-    int listed = 0;
-    if (warp == 0) {   // the ragged ends: at most 14 values
-      const u64 e = has_edge ? entry_of(edge_v, edge_at) : 0;
-      const uint32_t kept = __ballot_sync(~0u, e > thr);
-      if (e > thr) l.entry[0][__popc(kept & ((1u << lane) - 1u))] = e;
-      listed = __popc(kept);
-    }
-    const int turns = (v1 - v0 + THREADS - 1) / THREADS, items = l.queued * turns;   // (at most the block's vectors and 255)
-    for (int i0 = warp * 32; i0 < items; i0 += THREADS * 2) {
-      Vec<T> v[2];
-      uint32_t j0[2];
-      bool valid[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int item = i0 + u * THREADS + lane, q = item / turns;
-        const int at = item < items ? v0 + l.queue[q] + (item - q * turns) * THREADS : v1;
-        valid[u] = at < v1;
-        j0[u] = static_cast<uint32_t>(head + at * N);
-        if (valid[u]) v[u] = load_vec(xv + static_cast<long long>(at) * N);
+      for (int u = 0; u < U; ++u) {
+        const uint4 w = slots[(stage * U + u) * THREADS + tid];
+        v[u].w[0] = w.x; v[u].w[1] = w.y; v[u].w[2] = w.z; v[u].w[3] = w.w;
+        if (i0 + u * THREADS + tid >= q.v1) {   // nothing there: -inf, no weight
+          const uint32_t none = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
+          v[u].w[0] = v[u].w[1] = v[u].w[2] = v[u].w[3] = none;
+        }
+        cm = max_nan(cm, v[u].top());
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) listed = offer<T>(l, v[u], valid[u], j0[u], listed, warp, lane, top);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      copy_turn();          // into the slots that were just read
+      if (TOP) most = max_nan(most, cm);
+      add_values<T, U, ENT>(a, v, cm, k, far);
     }
-    if (lane == 0) l.count[warp] = listed;
-    block_best(l, best, top, tid);
-  } else {
-    __syncthreads();
-  }
-  a = parts[0];
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) a = merge(a, parts[w], k, far);
-  if (blocks > 1) {
-    cluster_wait();
-    if (tid == 0) {
-      const uint32_t to = in_block(&block_parts[block], 0);
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(a.m) : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(a.s) : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a.t) : "memory");
+    for (int o = 16; o; o >>= 1) {
+      Sums b;
+      b.m = __shfl_xor_sync(~0u, a.m, o);
+      b.s = __shfl_xor_sync(~0u, a.s, o);
+      b.t = __shfl_xor_sync(~0u, a.t, o);
+      a = merge(a, b, k, far);
     }
-    if (TOP && tid < top)
-      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_block(&block_best_of[block * top + tid], 0)), "l"(best[tid]) : "memory");
-    cluster_arrive();
-    cluster_wait();
-    if (block) return;
-    a = block_parts[0];
-    for (int b = 1; b < blocks; ++b) a = merge(a, block_parts[b], k, far);
+    phase ^= 1;
+    if (lane == 0) parts[phase][warp] = a;
     if (TOP) {
-      const int n = blocks * top;
-      for (int i = tid; i < n; i += THREADS) {
-        const u64 e = block_best_of[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += block_best_of[j] > e;
-        if (e && rank < top) best[rank] = e;
+      const uint32_t key = q.v0 + tid < q.v1 || has_edge ? order_of(most) : 0u;
+      l.maxima[tid] = key;
+      __syncthreads();
+      if (warp == 0) {
+        const uint32_t t = top_of_maxima(l.maxima, lane, top);
+        if (lane == 0) l.threshold = t ? (static_cast<u64>(t) << 32) - 1 : 0;   // (every entry of that value is above it)
       }
       __syncthreads();
+      const u64 thr = l.threshold;
+      if (key && key > static_cast<uint32_t>(thr >> 32)) l.queue[atomicAdd(&l.queued, 1)] = static_cast<uint16_t>(tid);
+      __syncthreads();
+      int listed = 0;
+      if (warp == 0) {   // the ragged ends: at most 14 values
+        const u64 e = has_edge ? entry_of(edge_v, edge_at) : 0;
+        const uint32_t kept = __ballot_sync(~0u, e > thr);
+        if (e > thr) l.entry[0][__popc(kept & ((1u << lane) - 1u))] = e;
+        listed = __popc(kept);
+      }
+      const int turns = (q.v1 - q.v0 + THREADS - 1) / THREADS, items = l.queued * turns;   // (at most the block's vectors and 255)
+      for (int i0 = warp * 32; i0 < items; i0 += THREADS * 2) {
+        Vec<T> v[2];
+        uint32_t j0[2];
+        bool valid[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int item = i0 + u * THREADS + lane, w = item / turns;
+          const int at = item < items ? q.v0 + l.queue[w] + (item - w * turns) * THREADS : q.v1;
+          valid[u] = at < q.v1;
+          j0[u] = static_cast<uint32_t>(q.head + at * N);
+          if (valid[u]) v[u] = load_vec(q.row + j0[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) listed = offer<T>(l, v[u], valid[u], j0[u], listed, warp, lane, top);
+      }
+      if (lane == 0) l.count[warp] = listed;
+      block_best(l, best, top, tid);
+    } else {
+      __syncthreads();
+    }
+    if (blocks > 1) {
+      if (warp == 0) {
+        a = parts[phase][0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) a = merge(a, parts[phase][w], k, far);
+        if (lane == 0) {
+          const uint32_t to = in_block(&block_parts[phase][block], 0);
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(a.m) : "memory");
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(a.s) : "memory");
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a.t) : "memory");
+        }
+      }
+      if (TOP && tid < top)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_block(&block_best_of[phase][block * top + tid], 0)), "l"(best[tid])
+                     : "memory");
+      // the first block reads this row's results before it arrives for the next row, and the row after that is the first to
+      // use the same places again
+      cluster_arrive();
+      cluster_wait();
+      if (block) continue;
+      if (TOP) {
+        const int n = blocks * top;
+        for (int i = tid; i < n; i += THREADS) {
+          const u64 e = block_best_of[phase][i];
+          int rank = 0;
+          for (int j = 0; j < n; ++j) rank += block_best_of[phase][j] > e;
+          if (e && rank < top) best[rank] = e;
+        }
+        __syncthreads();
+      }
+    }
+    if (tid < (TOP ? max(top, 1) : 1)) {
+      const Sums* from = blocks > 1 ? block_parts[phase] : parts[phase];
+      a = from[0];
+      for (int w = 1; w < (blocks > 1 ? blocks : WARPS); ++w) a = merge(a, from[w], k, far);
+      const float log_s = logf(a.s);
+      if (tid == 0) {
+        const float h = log_s - a.t / a.s * scale;
+        if (p.tokens) p.logprob[row] = (at_token - a.m) * scale - log_s;
+        if (ENT && p.entropy) p.entropy[row] = h;
+        if (p.stats) p.stats[row] = make_float4(a.m, log_s, h, 0.f);
+      }
+      if (TOP && tid < top) {
+        const u64 e = best[tid];
+        p.top_id[row * top + tid] = index_of(e);
+        p.top_lp[row * top + tid] = (value_of(static_cast<uint32_t>(e >> 32)) - a.m) * scale - log_s;
+      }
     }
   }
-  const float log_s = logf(a.s);
-  if (tid == 0) {
-    const float h = log_s - a.t / a.s * scale;
-    if (tokens) logprob[row] = (to_f(xr[tok]) - a.m) * scale - log_s;
-    if (ENT && entropy) entropy[row] = h;
-    if (stats) stats[row] = make_float4(a.m, log_s, h, 0.f);
-  }
-  if (TOP && tid < top) {
-    const long long id = index_of(best[tid]);
-    top_id[row * top + tid] = id;
-    top_lp[row * top + tid] = (to_f(xr[id]) - a.m) * scale - log_s;
-  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Gradient: reads the logits once more and writes as much.  A block owns `per` vectors of a row (16 bytes of output); where
@@ -612,46 +703,48 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
   }
 }
 
-// Blocks of a row: enough of them for about six waves, so that the last, partial wave costs little; every block keeps at least
-// one full turn of its loop (1024 vectors).
+// Blocks of a row: the split with the shortest longest queue.  A block's rows cost their vectors and about 1500 more each (the
+// end of a row: reductions, the alternatives), a cluster's barrier some 500.
 int blocks_per_row(int rows, int V, int elem) {
-  const long long slots = 4ll * mbh::sm_count(), vectors = static_cast<long long>(V) * elem / 16;
-  int b = 1;
-  while (b < MAX_CLUSTER && rows * static_cast<long long>(b) < 6 * slots && vectors >= 2048ll * b) b *= 2;
-  return b;
+  const long long slots = static_cast<long long>(RESIDENT) * mbh::sm_count(), vectors = static_cast<long long>(V) * elem / 16;
+  int best = 1;
+  long long least = 0;
+  for (int b = 1; b <= MAX_CLUSTER; b *= 2) {
+    const long long clusters = slots / b, turns = (rows + clusters - 1) / clusters;
+    const long long cost = turns * ((vectors + b - 1) / b + 1500 + (b > 1 ? 500 : 0));
+    if (b == 1 || cost < least) {
+      least = cost;
+      best = b;
+    }
+  }
+  return best;
 }
 
 template <typename T, bool ENT, bool TOP>
-int launch_fwd(const void* x, const long long* tokens, int rows, int V, long long ld, float scale, float* logprob,
-               float* entropy, int top, float* top_lp, long long* top_id, float4* stats, cudaStream_t stream) {
-  int* status = mbh::status().dev;
-  if (!status) return -4;
-  const int blocks = blocks_per_row(rows, V, sizeof(T));
-  if (static_cast<long long>(rows) * blocks > 0x7fffffffll) return -3;
+int launch_fwd(const void* x, const FwdArgs& p, cudaStream_t stream) {
+  constexpr int smem = STAGES * TURN * THREADS * 16 + (TOP ? static_cast<int>(sizeof(Lists)) : 0);
+  const int clusters = RESIDENT * mbh::sm_count() / p.blocks;
+  MB_SET_MAX_SMEM_ONCE((logprobs_fwd_kernel<T, ENT, TOP>), smem);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows * blocks, 1, 1);
+  cfg.gridDim = dim3((p.rows < clusters ? p.rows : clusters) * p.blocks, 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.x = p.blocks;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = blocks > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, ENT, TOP>, static_cast<const T*>(x), tokens, V, ld, scale, blocks, logprob,
-                     entropy, top, top_lp, top_id, stats, status);
+  cfg.numAttrs = p.blocks > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, ENT, TOP>, static_cast<const T*>(x), p);
   return mbh::check_launch("logprobs_fwd");
 }
 template <typename T>
-int fwd(const void* x, const long long* tokens, int rows, int V, long long ld, float scale, float* logprob, float* entropy,
-        int top, float* top_lp, long long* top_id, float4* stats, cudaStream_t stream) {
-  const bool ent = entropy || stats;   // (the entropy's gradient needs the entropy)
-  if (top)
-    return ent ? launch_fwd<T, true, true>(x, tokens, rows, V, ld, scale, logprob, entropy, top, top_lp, top_id, stats, stream)
-               : launch_fwd<T, false, true>(x, tokens, rows, V, ld, scale, logprob, entropy, top, top_lp, top_id, stats, stream);
-  return ent ? launch_fwd<T, true, false>(x, tokens, rows, V, ld, scale, logprob, entropy, top, top_lp, top_id, stats, stream)
-             : launch_fwd<T, false, false>(x, tokens, rows, V, ld, scale, logprob, entropy, top, top_lp, top_id, stats, stream);
+int fwd(const void* x, const FwdArgs& p, cudaStream_t stream) {
+  const bool ent = p.entropy || p.stats;   // (the entropy's gradient needs the entropy)
+  if (p.top) return ent ? launch_fwd<T, true, true>(x, p, stream) : launch_fwd<T, false, true>(x, p, stream);
+  return ent ? launch_fwd<T, true, false>(x, p, stream) : launch_fwd<T, false, false>(x, p, stream);
 }
 
 }  // namespace
@@ -663,11 +756,12 @@ extern "C" int mb_logprobs_fwd(const void* x, const long long* tokens, int type,
                                cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (V <= 0 || V > 0x7fffffff - 65536 || top < 0 || top > MAX_TOP || top > V) return -3;
-  float4* f4 = static_cast<float4*>(stats);
-  if (type == T_BF16) return fwd<__nv_bfloat16>(x, tokens, rows, V, ld, scale, logprob, entropy, top, top_lp, top_id, f4, stream);
-  if (type == T_F16) return fwd<__half>(x, tokens, rows, V, ld, scale, logprob, entropy, top, top_lp, top_id, f4, stream);
-  if (type == T_F32) return fwd<float>(x, tokens, rows, V, ld, scale, logprob, entropy, top, top_lp, top_id, f4, stream);
-  return -3;
+  if (type < T_BF16 || type > T_F32) return -3;
+  int* status = mbh::status().dev;
+  if (!status) return -4;
+  const FwdArgs p{tokens, rows, V, ld, scale, blocks_per_row(rows, V, type == T_F32 ? 4 : 2), logprob, entropy, top, top_lp, top_id,
+                  static_cast<float4*>(stats), status};
+  return type == T_BF16 ? fwd<__nv_bfloat16>(x, p, stream) : type == T_F16 ? fwd<__half>(x, p, stream) : fwd<float>(x, p, stream);
 }
 
 namespace {
