@@ -6,10 +6,12 @@
 // Statistics are 32-bit whatever the type of the logits.  -inf logits have probability 0 and gradient 0; a row without a
 // finite logit, or with NaN or +inf, has no distribution and comes out as NaN.
 //
-// Forward: one pass over the logits by resident blocks of 256 threads that take row after row; with few rows a cluster of 2, 4
-// or 8 blocks shares each (their results meet in the first block's shared memory).  Every thread copies its own next vectors
-// into its own slots of shared memory (cp.async), STAGES turns ahead and across the ends of rows, so that loads go on while a
-// row's results are put together; no thread waits for another's copy.  It keeps its own running (max, sum, weighted sum) and
+// Forward: one pass over the logits.  A row belongs to one block of 256 threads, or to a cluster of 2, 4 or 8 of them when
+// rows are few (their results meet in the first block's shared memory).  Every thread copies its own next vectors into its own
+// slots of shared memory (cp.async), STAGES turns ahead: no thread waits for another's copy, and four blocks an SM keep 128 KiB
+// on the way while one of them puts a row's results together.  (Resident blocks that take row after row, with copies across
+// the ends of rows, were slower: SMs differ in their distance to memory, and a fixed share of the rows leaves the fast ones
+// idle at the end; 176 against 163 us for 4099 x 128256 bf16.)  A thread keeps its own running (max, sum, weighted sum) and
 // takes the maximum of 32 values first, so the sums are rescaled once for 32.
 // The alternatives need the threads' maxima only: at least `top` values reach the top-th largest of the 256, and hardly more
 // do, so the second look goes to the values of some `top` threads (a 256th of the row each, mostly still in L2).  What
@@ -31,7 +33,7 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int CAP = 96;            // entries of a warp's list: more than MAX_TOP and a vector
 constexpr int TURN = 4;            // vectors of a thread's turn
 constexpr int STAGES = 2;          // turns in flight
-constexpr int RESIDENT = 4;        // blocks of an SM
+constexpr int RESIDENT = 4;        // blocks of an SM (64 registers a thread, 55 KiB a block)
 constexpr int MAX_CLUSTER = 8;
 typedef unsigned long long u64;
 
@@ -139,11 +141,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
   return r;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
-  return r;
-}
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<u64&>(r))
@@ -151,66 +148,81 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// Running (maximum m of x, sum s of exp(scale (x - m)), sum t of (x - m) exp(scale (x - m))).
+// Running maximum m of x, sum s of 2^z and sum t of z 2^z with z = k x - base(m), k = scale log2(e).  base(m) is k m as rounded:
+// one fused operation gives z, and the difference to k m is taken out of log s at the end.  Where k m could overflow
+// (logits of 1e30 and more, such as the lowest finite value as a mask) z = k (x - m), the base is k m itself.
 struct Sums {
   float m, s, t;
 };
-// two parts of a row.  t + s d: with d <= 0 the old terms move by d each.  (A part without a finite value has m = -inf and
-// s = t = 0, or NaN, which has to survive.)
-__device__ __forceinline__ Sums merge(const Sums& a, const Sums& b, float k, float far) {
-  Sums r;
-  r.m = fmaxf(a.m, b.m);
-  if (r.m == -INFINITY) {
-    r.s = a.s + b.s;
-    r.t = a.t + b.t;
-    return r;
+constexpr float HUGE_LOGIT = 1e30f, ZFAR = -1500.f;      // 2^-1500 is 0
+__device__ __forceinline__ bool plain(float m) { return fabsf(m) < HUGE_LOGIT; }
+// base(from) - base(to), at least ZFAR; `from` <= `to`, `to` finite or +inf, `from` may be -inf
+__device__ __forceinline__ float base_step(float from, float to, float k) {
+  const float d = plain(from) && plain(to) ? from * k - to * k : (from - to) * k;
+  return fmaxf(d, ZFAR);
+}
+// the sums of `a` on the base of m >= a.m.  (t + s d: every old z moves by d.)
+__device__ __forceinline__ void rebase(Sums& a, float m, float k) {
+  const float d = base_step(a.m, m, k), c = ex2(d);
+  a.t = (a.t + a.s * d) * c;
+  a.s *= c;
+  a.m = m;
+}
+// over n = 32 or 8 lanes; a part without a finite value has m = -inf and s = t = 0, or NaN, which has to survive
+template <int LANES>
+__device__ __forceinline__ Sums merge_lanes(Sums a, float k) {
+  float m = a.m;
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (m != -INFINITY) rebase(a, m, k);
+#pragma unroll
+  for (int o = LANES / 2; o; o >>= 1) {
+    a.s += __shfl_xor_sync(~0u, a.s, o);
+    a.t += __shfl_xor_sync(~0u, a.t, o);
   }
-  const float da = fmaxf(a.m - r.m, -far), db = fmaxf(b.m - r.m, -far);
-  const float ca = ex2(da * k), cb = ex2(db * k);
-  r.t = (a.t + a.s * da) * ca + (b.t + b.s * db) * cb;
-  r.s = a.s * ca + b.s * cb;
-  return r;
+  return a;
 }
 
-// Add the values of `v` (largest: cm) to the sums.
+// Add the values of `v` (largest: cm, NaN if there is one) to the sums.
 template <typename T, int U, bool ENT>
 __device__ __forceinline__ void add_values(Sums& a, const Vec<T> (&v)[U], float cm, float k, float far) {
-  if (cm > a.m || a.m == -INFINITY) {
+  if (!(cm <= a.m) || a.m == -INFINITY) {
     if (cm == -INFINITY) return;               // nothing but -inf so far (NaN goes on: it has to reach the sums)
-    if (a.m != -INFINITY && cm == cm) {
-      const float d = fmaxf(a.m - cm, -far), c = ex2(d * k);
-      a.t = (a.t + a.s * d) * c;
-      a.s *= c;
-    }
-    a.m = cm == cm ? cm : fmaxf(a.m, 0.f);
+    const float m = cm == cm ? cm : fmaxf(a.m, 0.f);
+    if (a.m == -INFINITY) a.m = m;
+    else rebase(a, fmaxf(m, a.m), k);
   }
   // Two values an instruction.  What is so far below the maximum that its weight is 0 is lifted to a finite value first, so
-  // that -inf does not meet the weight 0 in the entropy's sum; 16-bit logits in packed form where there is room below m
+  // that -inf does not meet the weight 0 in the entropy's sum: 16-bit logits in packed form where there is room below m
   const float m = a.m, low = m - fmaxf(far, 0.02f * fabsf(m));
   float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
-  const float2 nm = make_float2(-m, -m), k2 = make_float2(k, k);
-  if (Vec<T>::PACKED && ENT && low >= Vec<T>::LOWEST) {
+  const float2 k2 = make_float2(k, k);
+  if (plain(m) && (!ENT || (Vec<T>::PACKED && low >= Vec<T>::LOWEST))) {
     const uint32_t low2 = Vec<T>::both(low);
+    const float2 nb = make_float2(-(m * k), -(m * k));
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < Vec<T>::N / 2; ++i) {
-        const float2 d = add2(v[u].pair(i, low2), nm), z = mul2(d, k2), e = make_float2(ex2(z.x), ex2(z.y));
+        const float2 x = ENT ? v[u].pair(i, low2) : make_float2(v[u].at(2 * i), v[u].at(2 * i + 1));
+        const float2 z = fma2(x, k2, nb), e = make_float2(ex2(z.x), ex2(z.y));
         s = add2(s, e);
-        t = fma2(e, d, t);
+        if (ENT) t = fma2(e, z, t);
       }
   } else {
+    const bool p = plain(m);
+    const float2 nm = p ? make_float2(0.f, 0.f) : make_float2(-m, -m), nb = p ? make_float2(-(m * k), -(m * k)) : make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < Vec<T>::N / 2; ++i) {
-        float2 d = add2(make_float2(v[u].at(2 * i), v[u].at(2 * i + 1)), nm);
-        const float2 z = mul2(d, k2), e = make_float2(ex2(z.x), ex2(z.y));
+        float2 z = fma2(add2(make_float2(v[u].at(2 * i), v[u].at(2 * i + 1)), nm), k2, nb);
+        const float2 e = make_float2(ex2(z.x), ex2(z.y));
         s = add2(s, e);
         if (ENT) {
-          d.x = fmaxf(d.x, -far);
-          d.y = fmaxf(d.y, -far);
-          t = fma2(e, d, t);
+          z.x = fmaxf(z.x, ZFAR);
+          z.y = fmaxf(z.y, ZFAR);
+          t = fma2(e, z, t);
         }
       }
   }
@@ -221,9 +233,9 @@ __device__ __forceinline__ void add_values(Sums& a, const Vec<T> (&v)[U], float 
 // ---- lists of candidates
 struct Lists {
   u64 entry[WARPS][CAP];
-  alignas(16) u64 merged[WARPS * CAP];   // survivors of this block
+  u64 merged[WARPS * CAP];   // survivors of this block
   u64 threshold;                 // an entry below it is not among the best
-  uint32_t maxima[THREADS];      // of the threads' values (as ordered whole numbers, 0: none)
+  uint32_t maxima[THREADS / 2];  // of groups of 2 or 4 threads (as ordered whole numbers, 0: none)
   uint16_t queue[THREADS];       // threads that reach the threshold
   int queued;
   int count[WARPS];
@@ -255,17 +267,23 @@ __device__ __noinline__ void cut_list(Lists& l, int warp, int lane, int n, int t
   __syncwarp();
 }
 
-// Largest key that at least `top` of the 256 maxima reach (0: fewer have a value).  One warp.
+// Largest key, as far as its upper half goes, that at least `top` of 32 G maxima reach (0: fewer have a value); two bits a step.
+template <int G>
 __device__ __forceinline__ uint32_t top_of_maxima(const uint32_t* maxima, int lane, int top) {
-  uint32_t key[THREADS / 32], t = 0;
+  uint32_t key[G], t = 0;
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) key[i] = maxima[i * 32 + lane];
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = t | (1u << bit);
+  for (int i = 0; i < G; ++i) key[i] = maxima[i * 32 + lane];
+  auto reach = [&](uint32_t c) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) n += __popc(__ballot_sync(~0u, key[i] >= c));
-    if (n >= top) t = c;
+    for (int i = 0; i < G; ++i) n += __popc(__ballot_sync(~0u, key[i] >= c));
+    return n >= top;
+  };
+#pragma unroll
+  for (int bit = 30; bit >= 16; bit -= 2) {
+    const uint32_t c1 = t | (1u << bit), c2 = t | (2u << bit), c3 = t | (3u << bit);
+    const bool r1 = reach(c1), r2 = reach(c2), r3 = reach(c3);
+    t = r3 ? c3 : r2 ? c2 : r1 ? c1 : t;
   }
   return t;
 }
@@ -317,23 +335,15 @@ __device__ __forceinline__ void block_best(Lists& l, u64* out, int top, int tid)
   if (tid < top) out[tid] = 0;
   __syncthreads();
   const int n = l.survivors;
-  if (tid == 0) {
-    if (n & 1) l.merged[n] = 0;     // (an odd n is below the array's size)
-    l.queued = 0;
-  }
-  __syncthreads();
-  if (tid == 0) l.survivors = 0;
   for (int i = tid; i < n; i += THREADS) {
     const u64 e = l.merged[i];
     int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; j += 2) {
-      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&l.merged[j]);
-      rank += (o.x > e) + (o.y > e);
-    }
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += l.merged[j] > e;
     if (rank < top) out[rank] = e;
   }
   __syncthreads();
+
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -384,225 +394,184 @@ struct FwdArgs {
 template <typename T, bool ENT, bool TOP>
 __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T* __restrict__ x, const FwdArgs p) {
   constexpr int N = Vec<T>::N, U = TURN;
-  __shared__ Sums parts[2][WARPS];                   // (by turns of rows: a row's are read while the next one's are made)
-  __shared__ Sums block_parts[2][MAX_CLUSTER];       // first block: one of each block of the cluster
-  __shared__ u64 block_best_of[TOP ? 2 : 1][TOP ? MAX_CLUSTER * MAX_TOP : 1];
+  __shared__ Sums parts[WARPS];
+  __shared__ Sums block_parts[MAX_CLUSTER];          // first block: one of each block of the cluster
+  __shared__ u64 block_best_of[TOP ? MAX_CLUSTER * MAX_TOP : 1];
   __shared__ u64 best[TOP ? MAX_TOP : 1];
   extern __shared__ __align__(16) uint8_t dynamic[];
   uint4* slots = reinterpret_cast<uint4*>(dynamic);  // [STAGES][U][THREADS]
   Lists& l = *reinterpret_cast<Lists*>(dynamic + STAGES * U * THREADS * 16);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, blocks = p.blocks, top = p.top;
   const int block = blocks > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const long long first = blockIdx.x / blocks, step = gridDim.x / blocks;
+  const long long row = blockIdx.x / blocks;
   const float scale = p.scale, k = scale * LOG2E, far = fminf(FAR / scale, 3e38f);
-  auto skipped = [&](long long row) {
-    const long long t = p.tokens ? __ldg(p.tokens + row) : 0;
-    return t < 0 || t >= V;
-  };
-  if (TOP && tid == 0) l.survivors = l.queued = 0;
-  if (blocks > 1) {   // every block of the cluster has started before anything is stored into one
-    cluster_arrive();
-    cluster_wait();
+  const long long tok = p.tokens ? __ldg(p.tokens + row) : 0;
+  if (tok < 0 || tok >= V) {     // (the same for every block of the row)
+    if (block == 0) {
+      const float v = tok == IGNORE ? 0.f : NAN;
+      if (tok != IGNORE && tid == 0) atomicCAS(p.status, 0, mb::ERR_BAD_ARG);
+      if (tid == 0) {
+        p.logprob[row] = v;
+        if (p.entropy) p.entropy[row] = v;
+        if (p.stats) p.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (TOP && tid < top) {
+        p.top_lp[row * top + tid] = -INFINITY;
+        p.top_id[row * top + tid] = -1;
+      }
+    }
+    return;
   }
-
-  // ---- copies: the turns of this block's rows one after the other
-  long long load_row = first;
-  int load_at = 0, load_end = 0, load_stage = 0;
-  const T* load_from = nullptr;
-  auto next_loads = [&]() {      // the next row that has something for this block
-    while (load_row < p.rows) {
-      if (!skipped(load_row)) {
-        const Part<T> q(x + load_row * p.ld, V, blocks, block);
-        if (q.v0 < q.v1) {
-          load_from = q.row + q.head;
-          load_at = q.v0;
-          load_end = q.v1;
-          return;
-        }
-      }
-      load_row += step;
-    }
-  };
+  if (blocks > 1) cluster_arrive();   // (waited for before the first store into another block: it has started by then)
+  if (TOP && tid == 0) l.survivors = l.queued = 0;
+  const Part<T> q(x + row * p.ld, V, blocks, block);
+  const T* from = q.row + q.head;
+  int copied = q.v0, into = 0;
   auto copy_turn = [&]() {
-    if (load_row < p.rows) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int at = load_at + u * THREADS + tid;
-        if (at < load_end) copy16(&slots[(load_stage * U + u) * THREADS + tid], load_from + static_cast<long long>(at) * N);
-      }
-      load_at += THREADS * U;
-      if (load_at >= load_end) {
-        load_row += step;
-        next_loads();
-      }
+    for (int u = 0; u < U; ++u) {
+      const int at = copied + u * THREADS + tid;
+      if (at < q.v1) copy16(&slots[(into * U + u) * THREADS + tid], from + static_cast<long long>(at) * N);
     }
-    load_stage = load_stage + 1 == STAGES ? 0 : load_stage + 1;
+    copied += THREADS * U;
+    into = into + 1 == STAGES ? 0 : into + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  next_loads();
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) copy_turn();
 
-  int stage = 0, phase = 0;
-  for (long long row = first; row < p.rows; row += step) {
-    const long long tok = p.tokens ? __ldg(p.tokens + row) : 0;
-    if (tok < 0 || tok >= V) {     // (the same for every block of the row)
-      if (block == 0) {
-        const float v = tok == IGNORE ? 0.f : NAN;
-        if (tok != IGNORE && tid == 0) atomicCAS(p.status, 0, mb::ERR_BAD_ARG);
-        if (tid == 0) {
-          p.logprob[row] = v;
-          if (p.entropy) p.entropy[row] = v;
-          if (p.stats) p.stats[row] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        if (TOP && tid < top) {
-          p.top_lp[row * top + tid] = -INFINITY;
-          p.top_id[row * top + tid] = -1;
-        }
-      }
-      continue;
-    }
-    const Part<T> q(x + row * p.ld, V, blocks, block);
-    const float at_token = tid == 0 ? to_f(q.row[tok]) : 0.f;
-    Sums a{-INFINITY, 0.f, 0.f};
-    // one value of a ragged end for some lanes of the first warp of the first block
-    float edge_v = -INFINITY;
-    int edge_at = 0;
-    bool has_edge = false;
-    {
-      const int tail0 = q.head + q.vectors * N, ends = q.head + V - tail0;   // (at most 14)
-      if (block == 0 && tid < ends) {
-        edge_at = tid < q.head ? tid : tail0 + tid - q.head;
-        has_edge = true;
-        const float v = edge_v = to_f(q.row[edge_at]);
-        if (v != -INFINITY) {
-          a.m = v == v ? v : 0.f;
-          const float e = ex2((v - a.m) * k);
-          a.s = e;
-          a.t = e * (v - a.m);
-        }
-      }
-    }
-    float most = edge_v;    // largest value of this thread; NaN if there is one
-    for (int i0 = q.v0; i0 < q.v1; i0 += THREADS * U) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-      Vec<T> v[U];
-      float cm = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint4 w = slots[(stage * U + u) * THREADS + tid];
-        v[u].w[0] = w.x; v[u].w[1] = w.y; v[u].w[2] = w.z; v[u].w[3] = w.w;
-        if (i0 + u * THREADS + tid >= q.v1) {   // nothing there: -inf, no weight
-          const uint32_t none = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
-          v[u].w[0] = v[u].w[1] = v[u].w[2] = v[u].w[3] = none;
-        }
-        cm = max_nan(cm, v[u].top());
-      }
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
-      copy_turn();          // into the slots that were just read
-      if (TOP) most = max_nan(most, cm);
-      add_values<T, U, ENT>(a, v, cm, k, far);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      Sums b;
-      b.m = __shfl_xor_sync(~0u, a.m, o);
-      b.s = __shfl_xor_sync(~0u, a.s, o);
-      b.t = __shfl_xor_sync(~0u, a.t, o);
-      a = merge(a, b, k, far);
-    }
-    phase ^= 1;
-    if (lane == 0) parts[phase][warp] = a;
-    if (TOP) {
-      const uint32_t key = q.v0 + tid < q.v1 || has_edge ? order_of(most) : 0u;
-      l.maxima[tid] = key;
-      __syncthreads();
-      if (warp == 0) {
-        const uint32_t t = top_of_maxima(l.maxima, lane, top);
-        if (lane == 0) l.threshold = t ? (static_cast<u64>(t) << 32) - 1 : 0;   // (every entry of that value is above it)
-      }
-      __syncthreads();
-      const u64 thr = l.threshold;
-      if (key && key > static_cast<uint32_t>(thr >> 32)) l.queue[atomicAdd(&l.queued, 1)] = static_cast<uint16_t>(tid);
-      __syncthreads();
-      int listed = 0;
-      if (warp == 0) {   // the ragged ends: at most 14 values
-        const u64 e = has_edge ? entry_of(edge_v, edge_at) : 0;
-        const uint32_t kept = __ballot_sync(~0u, e > thr);
-        if (e > thr) l.entry[0][__popc(kept & ((1u << lane) - 1u))] = e;
-        listed = __popc(kept);
-      }
-      const int turns = (q.v1 - q.v0 + THREADS - 1) / THREADS, items = l.queued * turns;   // (at most the block's vectors and 255)
-      for (int i0 = warp * 32; i0 < items; i0 += THREADS * 2) {
-        Vec<T> v[2];
-        uint32_t j0[2];
-        bool valid[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int item = i0 + u * THREADS + lane, w = item / turns;
-          const int at = item < items ? q.v0 + l.queue[w] + (item - w * turns) * THREADS : q.v1;
-          valid[u] = at < q.v1;
-          j0[u] = static_cast<uint32_t>(q.head + at * N);
-          if (valid[u]) v[u] = load_vec(q.row + j0[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) listed = offer<T>(l, v[u], valid[u], j0[u], listed, warp, lane, top);
-      }
-      if (lane == 0) l.count[warp] = listed;
-      block_best(l, best, top, tid);
-    } else {
-      __syncthreads();
-    }
-    if (blocks > 1) {
-      if (warp == 0) {
-        a = parts[phase][0];
-#pragma unroll
-        for (int w = 1; w < WARPS; ++w) a = merge(a, parts[phase][w], k, far);
-        if (lane == 0) {
-          const uint32_t to = in_block(&block_parts[phase][block], 0);
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(a.m) : "memory");
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(a.s) : "memory");
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a.t) : "memory");
-        }
-      }
-      if (TOP && tid < top)
-        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_block(&block_best_of[phase][block * top + tid], 0)), "l"(best[tid])
-                     : "memory");
-      // the first block reads this row's results before it arrives for the next row, and the row after that is the first to
-      // use the same places again
-      cluster_arrive();
-      cluster_wait();
-      if (block) continue;
-      if (TOP) {
-        const int n = blocks * top;
-        for (int i = tid; i < n; i += THREADS) {
-          const u64 e = block_best_of[phase][i];
-          int rank = 0;
-          for (int j = 0; j < n; ++j) rank += block_best_of[phase][j] > e;
-          if (e && rank < top) best[rank] = e;
-        }
-        __syncthreads();
-      }
-    }
-    if (tid < (TOP ? max(top, 1) : 1)) {
-      const Sums* from = blocks > 1 ? block_parts[phase] : parts[phase];
-      a = from[0];
-      for (int w = 1; w < (blocks > 1 ? blocks : WARPS); ++w) a = merge(a, from[w], k, far);
-      const float log_s = logf(a.s);
-      if (tid == 0) {
-        const float h = log_s - a.t / a.s * scale;
-        if (p.tokens) p.logprob[row] = (at_token - a.m) * scale - log_s;
-        if (ENT && p.entropy) p.entropy[row] = h;
-        if (p.stats) p.stats[row] = make_float4(a.m, log_s, h, 0.f);
-      }
-      if (TOP && tid < top) {
-        const u64 e = best[tid];
-        p.top_id[row * top + tid] = index_of(e);
-        p.top_lp[row * top + tid] = (value_of(static_cast<uint32_t>(e >> 32)) - a.m) * scale - log_s;
+  const float at_token = tid == 0 ? to_f(q.row[tok]) : 0.f;
+  Sums a{-INFINITY, 0.f, 0.f};
+  // one value of a ragged end for some lanes of the first warp of the first block
+  float edge_v = -INFINITY;
+  int edge_at = 0;
+  bool has_edge = false;
+  {
+    const int tail0 = q.head + q.vectors * N, ends = q.head + V - tail0;   // (at most 14)
+    if (block == 0 && tid < ends) {
+      edge_at = tid < q.head ? tid : tail0 + tid - q.head;
+      has_edge = true;
+      const float v = edge_v = to_f(q.row[edge_at]);
+      if (v != -INFINITY) {
+        a.m = v == v ? v : 0.f;
+        const float z = plain(a.m) ? fmaf(v, k, -(a.m * k)) : (v - a.m) * k, e = ex2(z);
+        a.s = e;
+        a.t = e * z;
       }
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  float most = edge_v;    // largest value of this thread; NaN if there is one
+  int stage = 0;
+  for (int i0 = q.v0; i0 < q.v1; i0 += THREADS * U) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    Vec<T> v[U];
+    float cm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint4 w = slots[(stage * U + u) * THREADS + tid];
+      v[u].w[0] = w.x; v[u].w[1] = w.y; v[u].w[2] = w.z; v[u].w[3] = w.w;
+      if (i0 + u * THREADS + tid >= q.v1) {   // nothing there: -inf, no weight
+        const uint32_t none = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
+        v[u].w[0] = v[u].w[1] = v[u].w[2] = v[u].w[3] = none;
+      }
+      cm = max_nan(cm, v[u].top());
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    copy_turn();          // into the slots that were just read
+    if (TOP) most = max_nan(most, cm);
+    add_values<T, U, ENT>(a, v, cm, k, far);
+  }
+  a = merge_lanes<32>(a, k);
+  if (lane == 0) parts[warp] = a;
+  if (TOP) {
+    const uint32_t key = q.v0 + tid < q.v1 || has_edge ? order_of(most) : 0u;
+    // groups of four threads where `top` is at most half their number, else of two: the fewer, the shorter the search, and
+    // only threads that reach the threshold themselves are looked at again
+    uint32_t group = max(key, __shfl_xor_sync(~0u, key, 1));
+    if (top <= 32) group = max(group, __shfl_xor_sync(~0u, group, 2));
+    if (!(tid & (top <= 32 ? 3 : 1))) l.maxima[top <= 32 ? tid >> 2 : tid >> 1] = group;
+    __syncthreads();
+    const uint32_t reached = top <= 32 ? top_of_maxima<2>(l.maxima, lane, top) : top_of_maxima<4>(l.maxima, lane, top);
+    const u64 thr = reached ? (static_cast<u64>(reached) << 32) - 1 : 0;   // (every entry of that value is above it)
+    if (tid == 0) l.threshold = thr;
+    if (key && key > static_cast<uint32_t>(thr >> 32)) l.queue[atomicAdd(&l.queued, 1)] = static_cast<uint16_t>(tid);
+    __syncthreads();
+    int listed = 0;
+    if (warp == 0) {   // the ragged ends: at most 14 values
+      const u64 e = has_edge ? entry_of(edge_v, edge_at) : 0;
+      const uint32_t kept = __ballot_sync(~0u, e > thr);
+      if (e > thr) l.entry[0][__popc(kept & ((1u << lane) - 1u))] = e;
+      listed = __popc(kept);
+    }
+    const int turns = (q.v1 - q.v0 + THREADS - 1) / THREADS, items = l.queued * turns;   // (at most the block's vectors and 255)
+    for (int i0 = warp * 32; i0 < items; i0 += THREADS * 2) {
+      Vec<T> v[2];
+      uint32_t j0[2];
+      bool valid[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int item = i0 + u * THREADS + lane, w = item / turns;
+        const int at = item < items ? q.v0 + l.queue[w] + (item - w * turns) * THREADS : q.v1;
+        valid[u] = at < q.v1;
+        j0[u] = static_cast<uint32_t>(q.head + at * N);
+        if (valid[u]) v[u] = load_vec(q.row + j0[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) listed = offer<T>(l, v[u], valid[u], j0[u], listed, warp, lane, top);
+    }
+    if (lane == 0) l.count[warp] = listed;
+    block_best(l, best, top, tid);
+  } else {
+    __syncthreads();
+  }
+  if (blocks > 1) {
+    cluster_wait();
+    if (warp == 0) {
+      a = merge_lanes<WARPS>(parts[lane & (WARPS - 1)], k);
+      if (lane == 0) {
+        const uint32_t to = in_block(&block_parts[block], 0);
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(a.m) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(a.s) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a.t) : "memory");
+      }
+    }
+    if (TOP && tid < top)
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_block(&block_best_of[block * top + tid], 0)), "l"(best[tid])
+                   : "memory");
+    cluster_arrive();
+    cluster_wait();
+    if (block) return;
+    if (TOP) {
+      const int n = blocks * top;
+      for (int i = tid; i < n; i += THREADS) {
+        const u64 e = block_best_of[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += block_best_of[j] > e;
+        if (e && rank < top) best[rank] = e;
+      }
+      __syncthreads();
+    }
+  }
+  if (warp < (TOP ? (top + 31) / 32 : 1)) {
+    const int at = lane & (WARPS - 1);
+    Sums part{-INFINITY, 0.f, 0.f};
+    if (blocks == 1) part = parts[at];
+    else if (at < blocks) part = block_parts[at];
+    a = merge_lanes<WARPS>(part, k);
+    // (log s on the base of m: what k m lost in its rounding is taken out)
+    const float base = a.m * k, log_s = logf(a.s) - (plain(a.m) ? fmaf(a.m, k, -base) * LN2 : 0.f);
+    if (tid == 0) {
+      const float h = logf(a.s) - a.t / a.s * LN2;
+      if (p.tokens) p.logprob[row] = (at_token - a.m) * scale - log_s;
+      if (ENT && p.entropy) p.entropy[row] = h;
+      if (p.stats) p.stats[row] = make_float4(a.m, log_s, h, 0.f);
+    }
+    if (TOP && tid < top) {
+      const u64 e = best[tid];
+      p.top_id[row * top + tid] = index_of(e);
+      p.top_lp[row * top + tid] = (value_of(static_cast<uint32_t>(e >> 32)) - a.m) * scale - log_s;
+    }
+  }
 }
 
 // Gradient: reads the logits once more and writes as much.  A block owns `per` vectors of a row (16 bytes of output); where
@@ -703,8 +672,8 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
   }
 }
 
-// Blocks of a row: the split with the shortest longest queue.  A block's rows cost their vectors and about 1500 more each (the
-// end of a row: reductions, the alternatives), a cluster's barrier some 500.
+// Blocks of a row: the split with the fewest waves times the length of one.  A block costs its vectors and about 1500 more (its
+// start, the reductions, the alternatives), a cluster's barrier some 500.
 int blocks_per_row(int rows, int V, int elem) {
   const long long slots = static_cast<long long>(RESIDENT) * mbh::sm_count(), vectors = static_cast<long long>(V) * elem / 16;
   int best = 1;
@@ -723,10 +692,9 @@ int blocks_per_row(int rows, int V, int elem) {
 template <typename T, bool ENT, bool TOP>
 int launch_fwd(const void* x, const FwdArgs& p, cudaStream_t stream) {
   constexpr int smem = STAGES * TURN * THREADS * 16 + (TOP ? static_cast<int>(sizeof(Lists)) : 0);
-  const int clusters = RESIDENT * mbh::sm_count() / p.blocks;
   MB_SET_MAX_SMEM_ONCE((logprobs_fwd_kernel<T, ENT, TOP>), smem);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.rows < clusters ? p.rows : clusters) * p.blocks, 1, 1);
+  cfg.gridDim = dim3(p.rows * p.blocks, 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -755,7 +723,7 @@ extern "C" int mb_logprobs_fwd(const void* x, const long long* tokens, int type,
                                float* logprob, float* entropy, int top, float* top_lp, long long* top_id, void* stats,
                                cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (V <= 0 || V > 0x7fffffff - 65536 || top < 0 || top > MAX_TOP || top > V) return -3;
+  if (V <= 0 || V > 0x7fffffff - 65536 || rows > 0x7fffffff / MAX_CLUSTER || top < 0 || top > MAX_TOP || top > V) return -3;
   if (type < T_BF16 || type > T_F32) return -3;
   int* status = mbh::status().dev;
   if (!status) return -4;
