@@ -8,11 +8,12 @@
 // second moment needs (e4m3 then spans 2^34 of v inside a block), and a root that is not zero never becomes zero: the
 // smallest code stands in, so m / r stays bounded where a block holds very different gradients.
 //
-// Every operation is rounded to 32 bits on its own (no contraction), in the order written above: the codes do not depend
-// on what the compiler fuses, and equal inputs give equal bits on every path.
+// The moments are rounded to 32 bits operation by operation (no contraction), in the order written above: the codes do not
+// depend on what the compiler fuses.  The root is a reciprocal root with one Newton step, whose remainder is exact (the rounded
+// root but for one value in a million); the quotient m / (...) is off by two steps of its own at most, a fraction of a step of p.
 //
-// The step moves 18 bytes a value with 8-bit states beside 32-bit parameters and their 16-bit copy (30 with 32-bit
-// states) and is bound by that.  A warp owns 256 consecutive values, so a block's maximum is one warp reduction.
+// The step moves 18 bytes a value with 8-bit states beside 32-bit parameters and their 16-bit copy (30 with 32-bit states) and
+// is bound by that.  A warp owns 256 consecutive values at a time, so a block's maximum is one warp reduction.
 #include "host_common.cuh"
 #include "sm100.cuh"
 #include <cuda_fp8.h>
@@ -21,7 +22,8 @@
 namespace {
 
 constexpr int BLOCK = 256;    // values that share an exponent; one warp
-constexpr int CHUNK = 8192;   // values of one thread block
+constexpr int WARP_BLOCKS = 8;                          // neighbouring blocks of a warp
+constexpr int CHUNK = 8 * WARP_BLOCKS * BLOCK;          // values of one thread block
 constexpr int THREADS = 256;
 constexpr int CAP = 512;      // tensors of one launch (the table travels as a kernel argument)
 
@@ -42,11 +44,6 @@ struct Hyper {
   float b1, omb1, b2, omb2, decay, step, inv_root, eps;
 };
 
-__device__ __forceinline__ float ld_f(const float* p) { return *p; }
-__device__ __forceinline__ float ld_f(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void st_f(float* p, float v) { *p = v; }
-__device__ __forceinline__ void st_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
-
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
 
 // smallest k in [k_min, 120] with amax <= 448 * 2^k = 1.75 * 2^(k + 8)
@@ -55,43 +52,47 @@ __device__ __forceinline__ int block_exponent(uint32_t amax_bits, int k_min) {
   const int k = (amax_bits & 0x7fffffu) <= 0x600000u ? e - 8 : e - 7;
   return min(max(k, k_min), 120);
 }
-__device__ __forceinline__ uint32_t finite_bits(float x) {                      // |x| as an ordered whole number; 0 if not finite
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
-}
-__device__ __forceinline__ uint8_t encode(float y) {
-  if (!(fabsf(y) <= 3.4028234e38f)) return 0x7f;                                // NaN and infinities
-  return static_cast<uint8_t>(__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3));
-}
-__device__ __forceinline__ float decode(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-}
 __device__ __forceinline__ float floored(float y) { return y > 0.f ? fmaxf(y, 0.001953125f) : y; }   // (NaN stays)
-// four codes in a word; finite values
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+// four codes in a word; an infinity has become NaN before
+__device__ __forceinline__ uint32_t encode4(float2 a, float2 b) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
-__device__ __forceinline__ float4 decode4(uint32_t w) {
-  const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3)));
-  const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3)));
-  return make_float4(lo.x, lo.y, hi.x, hi.y);
+__device__ __forceinline__ void decode4(uint32_t w, float2& a, float2& b) {
+  a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3)));
+  b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3)));
 }
 
-struct Moments {
-  float m, v, root;
-};
-__device__ __forceinline__ Moments moments(float m, float v, float g, const Hyper& h) {
-  Moments o;
-  o.m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(g, h.omb1));
-  o.v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(g, g), h.omb2));
-  o.root = __fsqrt_rn(o.v);
-  return o;
+// two fp32 operations an instruction
+typedef unsigned long long u64;
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
+  return r;
 }
-__device__ __forceinline__ float update(float p, const Moments& o, const Hyper& h) {
-  const float den = __fadd_rn(__fmul_rn(o.root, h.inv_root), h.eps);
-  return __fsub_rn(__fmul_rn(p, h.decay), __fmul_rn(__fdiv_rn(o.m, den), h.step));
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float b) { return mul2(a, make_float2(b, b)); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<u64&>(r))
+      : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)), "l"(reinterpret_cast<u64&>(c)));
+  return r;
+}
+__device__ __forceinline__ float rsqrt_approx(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^12 sqrt(v) for v < 2^104: on 2^24 v, which is a normal number or 0
+__device__ __forceinline__ float2 root2(float2 v) {
+  const float2 w = mul2(v, 16777216.f);
+  const float2 y = make_float2(rsqrt_approx(fmaxf(w.x, 1.1754944e-38f)), rsqrt_approx(fmaxf(w.y, 1.1754944e-38f)));
+  const float2 s = mul2(w, y), left = fma2(make_float2(-s.x, -s.y), s, w);
+  return fma2(left, mul2(y, 0.5f), s);
 }
 
 // four neighbouring values, read or written once
@@ -111,165 +112,163 @@ struct States {
   float *m32, *v32;                   // 32 bits
 };
 
-// A block of 256 values, its tensor's last one, or one that does not start on a 16-byte boundary: value by value.
-template <typename P, bool EIGHT>
-__device__ __noinline__ void block_by_value(P* p, const P* g, __nv_bfloat16* copy, int n, long long s0, const States& st,
-                                            const Hyper& h, int lane) {
-  Moments o[BLOCK / 32];
-  float scale_m = 0.f, scale_r = 0.f;
-  if (EIGHT) {
-    scale_m = pow2(static_cast<int>(st.m_exp[s0 / BLOCK]) - 127);
-    scale_r = pow2(static_cast<int>(st.r_exp[s0 / BLOCK]) - 127);
-  }
-  uint32_t am = 0, ar = 0;
-#pragma unroll
-  for (int j = 0; j < BLOCK / 32; ++j) {
-    const int e = j * 32 + lane;
-    o[j] = Moments{0.f, 0.f, 0.f};
-    if (e < n) {
-      float m, v;
-      if (EIGHT) {
-        m = decode(st.m8[s0 + e]) * scale_m;
-        const float r = decode(st.r8[s0 + e]) * scale_r;
-        v = __fmul_rn(r, r);
-      } else {
-        m = st.m32[s0 + e];
-        v = st.v32[s0 + e];
-      }
-      o[j] = moments(m, v, ld_f(g + e), h);
-      const float np = update(ld_f(p + e), o[j], h);
-      st_f(p + e, np);
-      if (copy) copy[e] = __float2bfloat16(np);
-      if (!EIGHT) {
-        st.m32[s0 + e] = o[j].m;
-        st.v32[s0 + e] = o[j].v;
-      }
-      am = max(am, finite_bits(o[j].m));
-      ar = max(ar, finite_bits(o[j].root));
-    }
-  }
-  if (EIGHT) {
-    const int km = block_exponent(__reduce_max_sync(~0u, am), -117), kr = block_exponent(__reduce_max_sync(~0u, ar), -54);
-    if (lane == 0) {
-      st.m_exp[s0 / BLOCK] = static_cast<uint8_t>(km + 127);
-      st.r_exp[s0 / BLOCK] = static_cast<uint8_t>(kr + 127);
-    }
-    const float im = pow2(-km), ir = pow2(-kr);
-#pragma unroll
-    for (int j = 0; j < BLOCK / 32; ++j) {
-      const int e = j * 32 + lane;
-      if (e < n) {
-        st.m8[s0 + e] = encode(__fmul_rn(o[j].m, im));
-        st.r8[s0 + e] = encode(floored(__fmul_rn(o[j].root, ir)));
-      }
-    }
-  }
+// n of four neighbouring values one by one (the end of a tensor, or off its 16-byte boundaries); 0 where there is none
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void narrow(float* p, float v) { *p = v; }
+__device__ __forceinline__ void narrow(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+template <typename P>
+__device__ __forceinline__ void load_some(const P* p, int n, float2& a, float2& b) {
+  a = make_float2(n > 0 ? widen(p[0]) : 0.f, n > 1 ? widen(p[1]) : 0.f);
+  b = make_float2(n > 2 ? widen(p[2]) : 0.f, n > 3 ? widen(p[3]) : 0.f);
 }
+template <typename P>
+__device__ __forceinline__ void store_some(P* p, int n, float2 a, float2 b) {
+  if (n > 0) narrow(p, a.x);
+  if (n > 1) narrow(p + 1, a.y);
+  if (n > 2) narrow(p + 2, b.x);
+  if (n > 3) narrow(p + 3, b.y);
+}
+template <typename P>
+__device__ __forceinline__ void load_all(const P* p, float2& a, float2& b) {
+  const float4 v = load4(p);
+  a = make_float2(v.x, v.y);
+  b = make_float2(v.z, v.w);
+}
+template <typename P>
+__device__ __forceinline__ void store_all(P* p, float2 a, float2 b) { store4(p, make_float4(a.x, a.y, b.x, b.y)); }
 
-// A whole block on 16-byte boundaries: a lane owns values 4 lane .. and 128 + 4 lane .., so that every access is a line.
+// The next block of 256 values (n of them exist; `lines`: all, on 16-byte boundaries).  A lane owns values 4 lane .. and
+// 128 + 4 lane .., so that every access of a whole block is a line.  The states behind the end of a tensor stay as they are.
+// exps: biased exponents of m and r, before and after.
 template <typename P, bool EIGHT>
-__device__ __forceinline__ void block_by_line(P* p, const P* g, __nv_bfloat16* copy, long long s0, const States& st, const Hyper& h,
-                                              int lane) {
+__device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* copy, long long s0, int n, bool lines, const States& st,
+                                            const Hyper& h, uint2 exps, int lane) {
   const int e0 = 4 * lane;
-  float4 pv[2], gv[2], mv[2], vv[2];
+  float2 x[4], d[4], m[4], v[4];
+  uint32_t mw[2], rw[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    gv[j] = load4(g + e0 + 128 * j);
-    pv[j] = load4(p + e0 + 128 * j);
-  }
-  if (EIGHT) {
-    uint32_t mw[2], rw[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      mw[j] = __ldcs(reinterpret_cast<const uint32_t*>(st.m8 + s0 + e0 + 128 * j));
-      rw[j] = __ldcs(reinterpret_cast<const uint32_t*>(st.r8 + s0 + e0 + 128 * j));
+    const int e = e0 + 128 * j;
+    if (lines) {
+      load_all(g + e, d[2 * j], d[2 * j + 1]);
+      load_all(p + e, x[2 * j], x[2 * j + 1]);
+    } else {
+      load_some(g + e, n - e, d[2 * j], d[2 * j + 1]);
+      load_some(p + e, n - e, x[2 * j], x[2 * j + 1]);
     }
-    const float sm = pow2(static_cast<int>(st.m_exp[s0 / BLOCK]) - 127), sr = pow2(static_cast<int>(st.r_exp[s0 / BLOCK]) - 127);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      mv[j] = decode4(mw[j]);
-      vv[j] = decode4(rw[j]);
-      float* m = &mv[j].x;
-      float* v = &vv[j].x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m[i] = __fmul_rn(m[i], sm);
-        const float r = __fmul_rn(v[i], sr);
-        v[i] = __fmul_rn(r, r);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      mv[j] = load4(st.m32 + s0 + e0 + 128 * j);
-      vv[j] = load4(st.v32 + s0 + e0 + 128 * j);
-    }
-  }
-  uint32_t am = 0, ar = 0;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    float* m = &mv[j].x;
-    float* v = &vv[j].x;
-    float* x = &pv[j].x;
-    const float* d = &gv[j].x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const Moments o = moments(m[i], v[i], d[i], h);
-      x[i] = update(x[i], o, h);
-      m[i] = o.m;
-      v[i] = EIGHT ? o.root : o.v;
-      if (EIGHT) {
-        am = max(am, __float_as_uint(o.m) & 0x7fffffffu);
-        ar = max(ar, __float_as_uint(o.root) & 0x7fffffffu);
-      }
-    }
-    store4(p + e0 + 128 * j, pv[j]);
-    if (copy) store4(copy + e0 + 128 * j, pv[j]);
-    if (!EIGHT) {
-      store4(st.m32 + s0 + e0 + 128 * j, mv[j]);
-      store4(st.v32 + s0 + e0 + 128 * j, vv[j]);
+    if (EIGHT) {     // (the state buffers go on to the end of the block, zeros there)
+      mw[j] = __ldcs(reinterpret_cast<const uint32_t*>(st.m8 + s0 + e));
+      rw[j] = __ldcs(reinterpret_cast<const uint32_t*>(st.r8 + s0 + e));
+    } else {
+      load_all(st.m32 + s0 + e, m[2 * j], m[2 * j + 1]);
+      load_all(st.v32 + s0 + e, v[2 * j], v[2 * j + 1]);
     }
   }
   if (EIGHT) {
-    am = __reduce_max_sync(~0u, am);
-    ar = __reduce_max_sync(~0u, ar);
-    if (am >= 0x7f800000u || ar >= 0x7f800000u) {   // something is not finite: it becomes the NaN code and sets no scale
-      am = ar = 0;
+    const float sm = pow2(static_cast<int>(exps.x) - 127), sr = pow2(static_cast<int>(exps.y) - 127);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float* m = &mv[j].x;
-        float* r = &vv[j].x;
+    for (int j = 0; j < 2; ++j) {
+      decode4(mw[j], m[2 * j], m[2 * j + 1]);
+      decode4(rw[j], v[2 * j], v[2 * j + 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = mul2(m[j], sm);
+      const float2 r = mul2(v[j], sr);
+      v[j] = mul2(r, r);
+    }
+  }
+  float am = 0.f, av = 0.f;     // largest finite or infinite value (fmaxf passes NaN over)
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    // (one by one: a packed product and sum are contracted, and ties between two codes then go the other way)
+    m[j].x = __fadd_rn(__fmul_rn(m[j].x, h.b1), __fmul_rn(d[j].x, h.omb1));
+    m[j].y = __fadd_rn(__fmul_rn(m[j].y, h.b1), __fmul_rn(d[j].y, h.omb1));
+    v[j].x = __fadd_rn(__fmul_rn(v[j].x, h.b2), __fmul_rn(__fmul_rn(d[j].x, d[j].x), h.omb2));
+    v[j].y = __fadd_rn(__fmul_rn(v[j].y, h.b2), __fmul_rn(__fmul_rn(d[j].y, d[j].y), h.omb2));
+    if (EIGHT) am = fmaxf(fmaxf(am, fabsf(m[j].x)), fabsf(m[j].y));
+    av = fmaxf(fmaxf(av, v[j].x), v[j].y);
+  }
+  if (!EIGHT) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int e = e0 + 128 * j;
+      if (lines) {
+        store_all(st.m32 + s0 + e, m[2 * j], m[2 * j + 1]);
+        store_all(st.v32 + s0 + e, v[2 * j], v[2 * j + 1]);
+      } else {
+        store_some(st.m32 + s0 + e, n - e, m[2 * j], m[2 * j + 1]);
+        store_some(st.v32 + s0 + e, n - e, v[2 * j], v[2 * j + 1]);
+      }
+    }
+  }
+  const bool vast = !(av < 2.028241e31f);      // 2^104 and more
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {    // v becomes 2^12 times its root
+    if (vast) v[j] = make_float2(__fmul_rn(__fsqrt_rn(v[j].x), 4096.f), __fmul_rn(__fsqrt_rn(v[j].y), 4096.f));
+    else v[j] = root2(v[j]);
+    const float2 den = add2(mul2(v[j], h.inv_root * 0.000244140625f), make_float2(h.eps, h.eps));
+    const float2 u = mul2(make_float2(__fdividef(m[j].x, den.x), __fdividef(m[j].y, den.y)), -h.step);
+    x[j] = add2(mul2(x[j], h.decay), u);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int e = e0 + 128 * j;
+    if (lines) {
+      store_all(p + e, x[2 * j], x[2 * j + 1]);
+      if (copy) store_all(copy + e, x[2 * j], x[2 * j + 1]);
+    } else {
+      store_some(p + e, n - e, x[2 * j], x[2 * j + 1]);
+      if (copy) store_some(copy + e, n - e, x[2 * j], x[2 * j + 1]);
+    }
+  }
+  if (EIGHT) {
+    uint32_t bm = __float_as_uint(am), br = __float_as_uint(av);
+    bm = __reduce_max_sync(~0u, bm);
+    br = __reduce_max_sync(~0u, br);
+    if (bm >= 0x7f800000u || br >= 0x7f800000u) {   // an infinity: it becomes the NaN code and sets no scale
+      bm = br = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float* a[4] = {&m[j].x, &m[j].y, &v[j].x, &v[j].y};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          am = max(am, finite_bits(m[i]));
-          ar = max(ar, finite_bits(r[i]));
-          if (!finite_bits(m[i]) && m[i] != 0.f) m[i] = __uint_as_float(0x7fffffffu);
-          if (!finite_bits(r[i]) && r[i] != 0.f) r[i] = __uint_as_float(0x7fffffffu);
+          const uint32_t b = __float_as_uint(*a[i]) & 0x7fffffffu;
+          if (b >= 0x7f800000u) *a[i] = __uint_as_float(0x7fffffffu);
+          else if (i < 2) bm = max(bm, b);
+          else br = max(br, b);
         }
       }
-      am = __reduce_max_sync(~0u, am);
-      ar = __reduce_max_sync(~0u, ar);
+      bm = __reduce_max_sync(~0u, bm);
+      br = __reduce_max_sync(~0u, br);
+      br = __float_as_uint(__fmul_rn(__uint_as_float(br), 0.000244140625f));
+    } else {        // the largest root is the root of the largest v
+      const float2 r = root2(make_float2(__uint_as_float(br), 0.f));
+      br = __float_as_uint(br >= 0x73800000u /* 2^104 */ ? __fsqrt_rn(__uint_as_float(br)) : __fmul_rn(r.x, 0.000244140625f));
     }
-    const int km = block_exponent(am, -117), kr = block_exponent(ar, -54);
-    const float im = pow2(-km), ir = pow2(-kr);
-    if (lane == 0) {
-      st.m_exp[s0 / BLOCK] = static_cast<uint8_t>(km + 127);
-      st.r_exp[s0 / BLOCK] = static_cast<uint8_t>(kr + 127);
+    const int km = block_exponent(bm, -117), kr = block_exponent(br, -54);
+    const float im = pow2(-km), ir = pow2(-kr) * 0.000244140625f;
+    exps = make_uint2(km + 127, kr + 127);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = mul2(m[j], im);
+      v[j] = mul2(v[j], ir);
+      v[j] = make_float2(floored(v[j].x), floored(v[j].y));
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float* m = &mv[j].x;
-      const float* r = &vv[j].x;
-      __stcs(reinterpret_cast<uint32_t*>(st.m8 + s0 + e0 + 128 * j),
-             encode4(__fmul_rn(m[0], im), __fmul_rn(m[1], im), __fmul_rn(m[2], im), __fmul_rn(m[3], im)));
-      __stcs(reinterpret_cast<uint32_t*>(st.r8 + s0 + e0 + 128 * j),
-             encode4(floored(__fmul_rn(r[0], ir)), floored(__fmul_rn(r[1], ir)), floored(__fmul_rn(r[2], ir)), floored(__fmul_rn(r[3], ir))));
+      const int e = e0 + 128 * j;
+      // behind the end everything was 0 and stays 0: whole words
+      __stcs(reinterpret_cast<uint32_t*>(st.m8 + s0 + e), encode4(m[2 * j], m[2 * j + 1]));
+      __stcs(reinterpret_cast<uint32_t*>(st.r8 + s0 + e), encode4(v[2 * j], v[2 * j + 1]));
     }
   }
+  return exps;
 }
 
 template <typename P, bool EIGHT>
-__global__ void __launch_bounds__(THREADS, 4) adamw_multi_kernel(const __grid_constant__ Table tab, const Hyper h, const States st) {
+__global__ void __launch_bounds__(THREADS, 3) adamw_multi_kernel(const __grid_constant__ Table tab, const Hyper h, const States st) {
   int lo = 0, hi = tab.count - 1;
   const int chunk = blockIdx.x;
   while (lo < hi) {
@@ -285,15 +284,26 @@ __global__ void __launch_bounds__(THREADS, 4) adamw_multi_kernel(const __grid_co
   const long long off = t.off;
   const bool lines = !((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(P) - 1)) &&
                      !(reinterpret_cast<uintptr_t>(copy) & 7);
-  for (int b = warp; b < CHUNK / BLOCK; b += THREADS / 32) {
-    const long long i0 = c0 + static_cast<long long>(b) * BLOCK;
-    if (i0 >= n) break;
-    if (lines && i0 + BLOCK <= n)
-      block_by_line<P, EIGHT>(p + i0, g + i0, copy ? copy + i0 : nullptr, off + i0, st, h, lane);
-    else
-      block_by_value<P, EIGHT>(p + i0, g + i0, copy ? copy + i0 : nullptr, static_cast<int>(min(n - i0, static_cast<long long>(BLOCK))),
-                               off + i0, st, h, lane);
+  // A warp's blocks are neighbours: their exponents are read together before the first and written together after the last.
+  // (Read and written block by block, bytes of one 32-byte sector were on their way in both directions all the time: 1247
+  // instead of 565 us for 200M values.)
+  const long long w0 = c0 + static_cast<long long>(warp) * WARP_BLOCKS * BLOCK;
+  if (w0 >= n) return;
+  const int blocks = static_cast<int>(min(static_cast<long long>(WARP_BLOCKS), (n - w0 + BLOCK - 1) / BLOCK));
+  uint8_t* exp_at = nullptr;
+  uint32_t exps = 0;               // lane b: m's exponent of block b, lane 16 + b: r's
+  if (EIGHT && (lane & 15) < blocks) {
+    exp_at = (lane < 16 ? st.m_exp : st.r_exp) + (off + w0) / BLOCK + (lane & 15);
+    exps = *exp_at;
   }
+  for (int b = 0; b < blocks; ++b) {
+    const long long i0 = w0 + static_cast<long long>(b) * BLOCK;
+    uint2 e = make_uint2(__shfl_sync(~0u, exps, b), __shfl_sync(~0u, exps, 16 + b));
+    const int have = static_cast<int>(min(n - i0, static_cast<long long>(BLOCK)));
+    e = next_block<P, EIGHT>(p + i0, g + i0, copy ? copy + i0 : nullptr, off + i0, have, lines && have == BLOCK, st, h, e, lane);
+    if ((lane & 15) == b) exps = lane < 16 ? e.x : e.y;
+  }
+  if (EIGHT && exp_at) *exp_at = static_cast<uint8_t>(exps);
 }
 
 }  // namespace

@@ -1,7 +1,9 @@
-"""``AdamWMulti`` on the GPU: bit for bit against the plain definition, whose operations are rounded one by one.
+"""``AdamWMulti`` on the GPU against the plain definition, whose operations are rounded one by one.
 
-The plain form runs on GPU tensors too: its square root and division are correctly rounded there, while the CPU's vector
-library may return a neighbour of a square root (one value in some hundred, seen in the parameters but not in the codes).
+The moments (codes, exponents, 32-bit states) agree bit for bit.  A parameter's update u is m / (root * c + eps) * step: the
+kernel's quotient is off by two steps of fp32 (2^-22 relative) at most, its root by one in rare cases, and adding it rounds p
+once: per step |p| 2^-23 + 3 |u| 2^-23 with |u| <= |p before| + |p after|; a 16-bit parameter may round to its neighbour.
+The plain form runs on GPU tensors too: its square root and division are correctly rounded there.
 """
 import pytest
 import torch
@@ -56,6 +58,22 @@ def _same(a, b):
     return torch.equal(a.nan_to_num(9.0, 8.0, 7.0), b.nan_to_num(9.0, 8.0, 7.0)) if a.is_floating_point() else torch.equal(a, b)
 
 
+class _Near:
+    """The bound above, summed over the steps."""
+
+    def __init__(self, params):
+        self.before = [p.detach().double().abs() for p in params]
+        self.tol = [torch.zeros_like(b) for b in self.before]
+
+    def check(self, a, b):
+        for i, (p, q) in enumerate(zip(a, b)):
+            x, y = p.detach().double(), q.detach().double()
+            step = 2.0 ** (-23 if p.dtype == torch.float32 else -7)
+            self.tol[i] += step * y.abs().nan_to_num(0.0) + 3 * 2.0 ** -23 * (y.abs() + self.before[i]).nan_to_num(0.0)
+            self.before[i] = y.abs()
+            assert torch.equal(x.isnan(), y.isnan()) and ((x - y).abs() <= self.tol[i])[~x.isnan()].all()
+
+
 SIZES = [(1,), (255, 256, 257), (3, 8191, 8192, 8193, 1), (100_003, 17, 65536, 5), tuple(range(1, 700, 7)), (1 << 20,)]
 
 
@@ -68,7 +86,7 @@ def test_steps(sizes, dtype, bits, shift):
     b = _twin(a)
     kw = dict(lr=1e-2, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1, state_bits=bits)
     oa, ob = AdamWMulti(a, **kw), _plain(AdamWMulti(b, **kw))
-    copies = {}
+    near, copies = _Near(b), {}
     if dtype == torch.float32:
         copies = {p: torch.zeros(p.numel() + shift, device="cuda", dtype=torch.bfloat16)[shift:] for p in a[::2]}
         oa.attach_copies(copies)
@@ -80,8 +98,7 @@ def test_steps(sizes, dtype, bits, shift):
             a[0].grad = b[0].grad = None                     # left alone, its step number too
         oa.step()
         ob.step()
-        for p, q in zip(a, b):
-            assert _same(p, q)
+        near.check(a, b)
         for k, v in oa.state_buffers().items():
             assert _same(v, ob.state_buffers()[k]), k
     for p, c in copies.items():
@@ -98,13 +115,14 @@ def test_groups_and_many_tensors(bits):
         return AdamWMulti([{"params": ps[:700], "lr": 1e-2, "weight_decay": 0.3}, {"params": ps[700:], "betas": (0.8, 0.99)}],
                           lr=3e-3, state_bits=bits)
     oa, ob = make(a), _plain(make(b))
+    near = _Near(b)
     for step in range(3):
         _grads(a, step)
         for p, q in zip(a, b):
             q.grad = p.grad
         oa.step()
         ob.step()
-    assert all(_same(p, q) for p, q in zip(a, b))
+        near.check(a, b)
     assert all(_same(v, ob.state_buffers()[k]) for k, v in oa.state_buffers().items())
 
 
