@@ -22,10 +22,10 @@
 namespace {
 
 constexpr int BLOCK = 256;    // values that share an exponent; one warp
-constexpr int WARP_BLOCKS = 8;                          // neighbouring blocks of a warp
+constexpr int WARP_BLOCKS = 4;                          // neighbouring blocks of a warp
 constexpr int CHUNK = 8 * WARP_BLOCKS * BLOCK;          // values of one thread block
 constexpr int THREADS = 256;
-constexpr int CAP = 512;      // tensors of one launch (the table travels as a kernel argument)
+constexpr int CAP_SMALL = 32, CAP_LARGE = 512;   // tensors of one launch: the table travels as a kernel argument (1.5 or 24 KiB)
 
 struct Tensor {   // one row of the caller's table
   void* p;
@@ -36,13 +36,15 @@ struct Tensor {   // one row of the caller's table
   int first_chunk;       // filled by the launcher
   int pad;
 };
+template <int CAP>
 struct Table {
   Tensor t[CAP];
   int count;
 };
 struct Hyper {
   float b1, omb1, b2, omb2, decay, step, inv_root, eps;
-};
+  float one;   // 1, unknown to the compiler: a packed product and sum would be contracted, and ties between two codes go the
+};             // other way then; a fused operation with it is a plain sum
 
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
 
@@ -65,11 +67,6 @@ __device__ __forceinline__ void decode4(uint32_t w, float2& a, float2& b) {
 
 // two fp32 operations an instruction
 typedef unsigned long long u64;
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
-  return r;
-}
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<u64&>(r)) : "l"(reinterpret_cast<u64&>(a)), "l"(reinterpret_cast<u64&>(b)));
@@ -87,24 +84,47 @@ __device__ __forceinline__ float rsqrt_approx(float x) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^12 sqrt(v) for v < 2^104: on 2^24 v, which is a normal number or 0
+__device__ __forceinline__ float rcp_approx(float x) {   // 0 above 2^126
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// sqrt(v) for v in [2^-102, 2^104): the remainder v - s^2 is exact
+constexpr float ROOT_FROM = 1.9721523e-31f, ROOT_TO = 2.028241e31f;
 __device__ __forceinline__ float2 root2(float2 v) {
-  const float2 w = mul2(v, 16777216.f);
-  const float2 y = make_float2(rsqrt_approx(fmaxf(w.x, 1.1754944e-38f)), rsqrt_approx(fmaxf(w.y, 1.1754944e-38f)));
-  const float2 s = mul2(w, y), left = fma2(make_float2(-s.x, -s.y), s, w);
+  const float2 y = make_float2(rsqrt_approx(v.x), rsqrt_approx(v.y));
+  const float2 s = mul2(v, y), left = fma2(make_float2(-s.x, -s.y), s, v);
   return fma2(left, mul2(y, 0.5f), s);
 }
-
-// four neighbouring values, read or written once
-__device__ __forceinline__ float4 load4(const float* p) { return __ldcs(reinterpret_cast<const float4*>(p)); }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 w = __ldcs(reinterpret_cast<const uint2*>(p));
-  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                     __uint_as_float(w.y & 0xffff0000u));
+// any v: 0, tiny and vast ones, infinities and NaN too
+__device__ __forceinline__ float any_root(float v) {
+  if (v >= ROOT_FROM && v < ROOT_TO) return root2(make_float2(v, 1.f)).x;
+  return __fsqrt_rn(v);
 }
-__device__ __forceinline__ void store4(float* p, float4 v) { __stcs(reinterpret_cast<float4*>(p), v); }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
-  __stcs(reinterpret_cast<uint2*>(p), make_uint2(mb::pack_bf16(v.x, v.y), mb::pack_bf16(v.z, v.w)));
+
+// Eight neighbouring values, read or written once: 32 bytes of fp32 or 16 of bf16 in one access
+__device__ __forceinline__ void load_all(const float* p, float2 (&a)[4]) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(a[0].x), "=f"(a[0].y), "=f"(a[1].x), "=f"(a[1].y), "=f"(a[2].x), "=f"(a[2].y), "=f"(a[3].x), "=f"(a[3].y)
+               : "l"(p));
+}
+__device__ __forceinline__ void widen_all(uint4 w, float2 (&a)[4]) {
+  a[0] = make_float2(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u));
+  a[1] = make_float2(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+  a[2] = make_float2(__uint_as_float(w.z << 16), __uint_as_float(w.z & 0xffff0000u));
+  a[3] = make_float2(__uint_as_float(w.w << 16), __uint_as_float(w.w & 0xffff0000u));
+}
+__device__ __forceinline__ void load_all(const __nv_bfloat16* p, float2 (&a)[4]) {
+  widen_all(__ldcs(reinterpret_cast<const uint4*>(p)), a);
+}
+__device__ __forceinline__ void store_all(float* p, const float2 (&a)[4]) {
+  asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+               ::"f"(a[0].x), "f"(a[0].y), "f"(a[1].x), "f"(a[1].y), "f"(a[2].x), "f"(a[2].y), "f"(a[3].x), "f"(a[3].y), "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store_all(__nv_bfloat16* p, const float2 (&a)[4]) {
+  __stcs(reinterpret_cast<uint4*>(p), make_uint4(mb::pack_bf16(a[0].x, a[0].y), mb::pack_bf16(a[1].x, a[1].y),
+                                                 mb::pack_bf16(a[2].x, a[2].y), mb::pack_bf16(a[3].x, a[3].y)));
 }
 
 struct States {
@@ -112,66 +132,73 @@ struct States {
   float *m32, *v32;                   // 32 bits
 };
 
-// n of four neighbouring values one by one (the end of a tensor, or off its 16-byte boundaries); 0 where there is none
+// n of eight neighbouring values one by one (the end of a tensor, or off its 32-byte boundaries); 0 where there is none
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void narrow(float* p, float v) { *p = v; }
 __device__ __forceinline__ void narrow(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
 template <typename P>
-__device__ __forceinline__ void load_some(const P* p, int n, float2& a, float2& b) {
-  a = make_float2(n > 0 ? widen(p[0]) : 0.f, n > 1 ? widen(p[1]) : 0.f);
-  b = make_float2(n > 2 ? widen(p[2]) : 0.f, n > 3 ? widen(p[3]) : 0.f);
+__device__ __forceinline__ void load_some(const P* p, int n, float2 (&a)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = make_float2(n > 2 * i ? widen(p[2 * i]) : 0.f, n > 2 * i + 1 ? widen(p[2 * i + 1]) : 0.f);
 }
 template <typename P>
-__device__ __forceinline__ void store_some(P* p, int n, float2 a, float2 b) {
-  if (n > 0) narrow(p, a.x);
-  if (n > 1) narrow(p + 1, a.y);
-  if (n > 2) narrow(p + 2, b.x);
-  if (n > 3) narrow(p + 3, b.y);
+__device__ __forceinline__ void store_some(P* p, int n, const float2 (&a)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (n > 2 * i) narrow(p + 2 * i, a[i].x);
+    if (n > 2 * i + 1) narrow(p + 2 * i + 1, a[i].y);
+  }
 }
-template <typename P>
-__device__ __forceinline__ void load_all(const P* p, float2& a, float2& b) {
-  const float4 v = load4(p);
-  a = make_float2(v.x, v.y);
-  b = make_float2(v.z, v.w);
-}
-template <typename P>
-__device__ __forceinline__ void store_all(P* p, float2 a, float2 b) { store4(p, make_float4(a.x, a.y, b.x, b.y)); }
 
-// The next block of 256 values (n of them exist; `lines`: all, on 16-byte boundaries).  A lane owns values 4 lane .. and
-// 128 + 4 lane .., so that every access of a whole block is a line.  The states behind the end of a tensor stay as they are.
-// exps: biased exponents of m and r, before and after.
+// What a lane reads of a block of 16-bit values with 8-bit states.  Such a block is few bytes and much arithmetic: the next one
+// is read while one is worked on (446 -> 397 us for 200M values; with 32-bit values the registers are worth more).
+struct Ahead {
+  uint4 x, d;
+  uint2 m, r;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, const __nv_bfloat16* g, const States& st, long long s0, int e) {
+    d = __ldcs(reinterpret_cast<const uint4*>(g + e));
+    x = __ldcs(reinterpret_cast<const uint4*>(p + e));
+    m = __ldcs(reinterpret_cast<const uint2*>(st.m8 + s0 + e));
+    r = __ldcs(reinterpret_cast<const uint2*>(st.r8 + s0 + e));
+  }
+  __device__ __forceinline__ void load(const float*, const float*, const States&, long long, int) {}
+};
+
+// A block of 256 values (n of them exist; `lines`: all, on 32-byte boundaries), 8 of them a lane's.  The states behind the end
+// of a tensor stay as they are.  exps: biased exponents of m and r, before and after.  read: this block if AHEAD and lines;
+// the following one afterwards, if it is whole (`more`).
 template <typename P, bool EIGHT>
 __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* copy, long long s0, int n, bool lines, const States& st,
-                                            const Hyper& h, uint2 exps, int lane) {
-  const int e0 = 4 * lane;
+                                            const Hyper& h, uint2 exps, int lane, Ahead& read, bool more) {
+  constexpr bool AHEAD = EIGHT && sizeof(P) == 2;
+  const int e = 8 * lane;
   float2 x[4], d[4], m[4], v[4];
-  uint32_t mw[2], rw[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int e = e0 + 128 * j;
-    if (lines) {
-      load_all(g + e, d[2 * j], d[2 * j + 1]);
-      load_all(p + e, x[2 * j], x[2 * j + 1]);
-    } else {
-      load_some(g + e, n - e, d[2 * j], d[2 * j + 1]);
-      load_some(p + e, n - e, x[2 * j], x[2 * j + 1]);
-    }
-    if (EIGHT) {     // (the state buffers go on to the end of the block, zeros there)
-      mw[j] = __ldcs(reinterpret_cast<const uint32_t*>(st.m8 + s0 + e));
-      rw[j] = __ldcs(reinterpret_cast<const uint32_t*>(st.r8 + s0 + e));
-    } else {
-      load_all(st.m32 + s0 + e, m[2 * j], m[2 * j + 1]);
-      load_all(st.v32 + s0 + e, v[2 * j], v[2 * j + 1]);
-    }
+  uint2 mw, rw;
+  if (AHEAD && lines) {
+    widen_all(read.d, d);
+    widen_all(read.x, x);
+  } else if (lines) {
+    load_all(g + e, d);
+    load_all(p + e, x);
+  } else {
+    load_some(g + e, n - e, d);
+    load_some(p + e, n - e, x);
+  }
+  if (EIGHT) {     // (the state buffers go on to the end of the block, zeros there)
+    mw = AHEAD && lines ? read.m : __ldcs(reinterpret_cast<const uint2*>(st.m8 + s0 + e));
+    rw = AHEAD && lines ? read.r : __ldcs(reinterpret_cast<const uint2*>(st.r8 + s0 + e));
+    if (AHEAD && more) read.load(p + BLOCK, g + BLOCK, st, s0 + BLOCK, e);
+  } else {
+    load_all(st.m32 + s0 + e, m);
+    load_all(st.v32 + s0 + e, v);
   }
   if (EIGHT) {
     const float sm = pow2(static_cast<int>(exps.x) - 127), sr = pow2(static_cast<int>(exps.y) - 127);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      decode4(mw[j], m[2 * j], m[2 * j + 1]);
-      decode4(rw[j], v[2 * j], v[2 * j + 1]);
-    }
+    decode4(mw.x, m[0], m[1]);
+    decode4(mw.y, m[2], m[3]);
+    decode4(rw.x, v[0], v[1]);
+    decode4(rw.y, v[2], v[3]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       m[j] = mul2(m[j], sm);
@@ -179,49 +206,45 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
       v[j] = mul2(r, r);
     }
   }
-  float am = 0.f, av = 0.f;     // largest finite or infinite value (fmaxf passes NaN over)
+  float am = 0.f, av = 0.f, least = INFINITY;     // over what is not NaN
+  const float2 one = make_float2(h.one, h.one);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    // (one by one: a packed product and sum are contracted, and ties between two codes then go the other way)
-    m[j].x = __fadd_rn(__fmul_rn(m[j].x, h.b1), __fmul_rn(d[j].x, h.omb1));
-    m[j].y = __fadd_rn(__fmul_rn(m[j].y, h.b1), __fmul_rn(d[j].y, h.omb1));
-    v[j].x = __fadd_rn(__fmul_rn(v[j].x, h.b2), __fmul_rn(__fmul_rn(d[j].x, d[j].x), h.omb2));
-    v[j].y = __fadd_rn(__fmul_rn(v[j].y, h.b2), __fmul_rn(__fmul_rn(d[j].y, d[j].y), h.omb2));
+    m[j] = fma2(mul2(m[j], h.b1), one, mul2(d[j], h.omb1));
+    v[j] = fma2(mul2(v[j], h.b2), one, mul2(mul2(d[j], d[j]), h.omb2));
     if (EIGHT) am = fmaxf(fmaxf(am, fabsf(m[j].x)), fabsf(m[j].y));
     av = fmaxf(fmaxf(av, v[j].x), v[j].y);
+    least = fminf(fminf(least, v[j].x), v[j].y);
   }
   if (!EIGHT) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int e = e0 + 128 * j;
-      if (lines) {
-        store_all(st.m32 + s0 + e, m[2 * j], m[2 * j + 1]);
-        store_all(st.v32 + s0 + e, v[2 * j], v[2 * j + 1]);
-      } else {
-        store_some(st.m32 + s0 + e, n - e, m[2 * j], m[2 * j + 1]);
-        store_some(st.v32 + s0 + e, n - e, v[2 * j], v[2 * j + 1]);
-      }
-    }
-  }
-  const bool vast = !(av < 2.028241e31f);      // 2^104 and more
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {    // v becomes 2^12 times its root
-    if (vast) v[j] = make_float2(__fmul_rn(__fsqrt_rn(v[j].x), 4096.f), __fmul_rn(__fsqrt_rn(v[j].y), 4096.f));
-    else v[j] = root2(v[j]);
-    const float2 den = add2(mul2(v[j], h.inv_root * 0.000244140625f), make_float2(h.eps, h.eps));
-    const float2 u = mul2(make_float2(__fdividef(m[j].x, den.x), __fdividef(m[j].y, den.y)), -h.step);
-    x[j] = add2(mul2(x[j], h.decay), u);
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int e = e0 + 128 * j;
     if (lines) {
-      store_all(p + e, x[2 * j], x[2 * j + 1]);
-      if (copy) store_all(copy + e, x[2 * j], x[2 * j + 1]);
+      store_all(st.m32 + s0 + e, m);
+      store_all(st.v32 + s0 + e, v);
     } else {
-      store_some(p + e, n - e, x[2 * j], x[2 * j + 1]);
-      if (copy) store_some(copy + e, n - e, x[2 * j], x[2 * j + 1]);
+      store_some(st.m32 + s0 + e, n - e, m);
+      store_some(st.v32 + s0 + e, n - e, v);
     }
+  }
+  if (least >= ROOT_FROM && av < ROOT_TO) {      // v becomes its root (NaN stays)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = root2(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = make_float2(any_root(v[j].x), any_root(v[j].y));
+  }
+  const float2 c = make_float2(h.inv_root, h.inv_root), eps = make_float2(h.eps, h.eps), step = make_float2(-h.step, -h.step);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 den = fma2(v[j], c, eps);
+    const float2 u = mul2(m[j], make_float2(rcp_approx(den.x), rcp_approx(den.y)));
+    x[j] = fma2(u, step, mul2(x[j], h.decay));
+  }
+  if (lines) {
+    store_all(p + e, x);
+    if (copy) store_all(copy + e, x);
+  } else {
+    store_some(p + e, n - e, x);
+    if (copy) store_some(copy + e, n - e, x);
   }
   if (EIGHT) {
     uint32_t bm = __float_as_uint(am), br = __float_as_uint(av);
@@ -242,33 +265,32 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
       }
       bm = __reduce_max_sync(~0u, bm);
       br = __reduce_max_sync(~0u, br);
-      br = __float_as_uint(__fmul_rn(__uint_as_float(br), 0.000244140625f));
-    } else {        // the largest root is the root of the largest v
-      const float2 r = root2(make_float2(__uint_as_float(br), 0.f));
-      br = __float_as_uint(br >= 0x73800000u /* 2^104 */ ? __fsqrt_rn(__uint_as_float(br)) : __fmul_rn(r.x, 0.000244140625f));
+    } else {
+      br = __float_as_uint(any_root(__uint_as_float(br)));       // the largest root is the root of the largest v
     }
     const int km = block_exponent(bm, -117), kr = block_exponent(br, -54);
-    const float im = pow2(-km), ir = pow2(-kr) * 0.000244140625f;
+    const float im = pow2(-km), ir = pow2(-kr);
     exps = make_uint2(km + 127, kr + 127);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       m[j] = mul2(m[j], im);
       v[j] = mul2(v[j], ir);
-      v[j] = make_float2(floored(v[j].x), floored(v[j].y));
     }
+    // a lane whose smallest root is at least the smallest code has nothing to lift (the margin covers the roots' roundings)
+    if (!(least * (ir * ir) >= 3.9e-6f)) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int e = e0 + 128 * j;
-      // behind the end everything was 0 and stays 0: whole words
-      __stcs(reinterpret_cast<uint32_t*>(st.m8 + s0 + e), encode4(m[2 * j], m[2 * j + 1]));
-      __stcs(reinterpret_cast<uint32_t*>(st.r8 + s0 + e), encode4(v[2 * j], v[2 * j + 1]));
+      for (int j = 0; j < 4; ++j) v[j] = make_float2(floored(v[j].x), floored(v[j].y));
     }
+    // (behind the end everything was 0 and stays 0: whole words)
+    __stcs(reinterpret_cast<uint2*>(st.m8 + s0 + e), make_uint2(encode4(m[0], m[1]), encode4(m[2], m[3])));
+    __stcs(reinterpret_cast<uint2*>(st.r8 + s0 + e), make_uint2(encode4(v[0], v[1]), encode4(v[2], v[3])));
   }
   return exps;
 }
 
-template <typename P, bool EIGHT>
-__global__ void __launch_bounds__(THREADS, 3) adamw_multi_kernel(const __grid_constant__ Table tab, const Hyper h, const States st) {
+template <typename P, bool EIGHT, int CAP>
+__global__ void __launch_bounds__(THREADS, 4)
+adamw_multi_kernel(const __grid_constant__ Table<CAP> tab, const Hyper h, const States st) {
   int lo = 0, hi = tab.count - 1;
   const int chunk = blockIdx.x;
   while (lo < hi) {
@@ -282,8 +304,8 @@ __global__ void __launch_bounds__(THREADS, 3) adamw_multi_kernel(const __grid_co
   const P* g = static_cast<const P*>(t.g);
   __nv_bfloat16* copy = t.copy;
   const long long off = t.off;
-  const bool lines = !((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(P) - 1)) &&
-                     !(reinterpret_cast<uintptr_t>(copy) & 7);
+  const bool lines = !((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (8 * sizeof(P) - 1)) &&
+                     !(reinterpret_cast<uintptr_t>(copy) & 15);
   // A warp's blocks are neighbours: their exponents are read together before the first and written together after the last.
   // (Read and written block by block, bytes of one 32-byte sector were on their way in both directions all the time: 1247
   // instead of 565 us for 200M values.)
@@ -296,14 +318,49 @@ __global__ void __launch_bounds__(THREADS, 3) adamw_multi_kernel(const __grid_co
     exp_at = (lane < 16 ? st.m_exp : st.r_exp) + (off + w0) / BLOCK + (lane & 15);
     exps = *exp_at;
   }
+  Ahead read;
+  if (EIGHT && lines && w0 + BLOCK <= n) read.load(p + w0, g + w0, st, off + w0, 8 * lane);
   for (int b = 0; b < blocks; ++b) {
     const long long i0 = w0 + static_cast<long long>(b) * BLOCK;
     uint2 e = make_uint2(__shfl_sync(~0u, exps, b), __shfl_sync(~0u, exps, 16 + b));
     const int have = static_cast<int>(min(n - i0, static_cast<long long>(BLOCK)));
-    e = next_block<P, EIGHT>(p + i0, g + i0, copy ? copy + i0 : nullptr, off + i0, have, lines && have == BLOCK, st, h, e, lane);
+    e = next_block<P, EIGHT>(p + i0, g + i0, copy ? copy + i0 : nullptr, off + i0, have, lines && have == BLOCK, st, h, e, lane, read,
+                             lines && b + 1 < blocks && i0 + 2 * BLOCK <= n);
     if ((lane & 15) == b) exps = lane < 16 ? e.x : e.y;
   }
   if (EIGHT && exp_at) *exp_at = static_cast<uint8_t>(exps);
+}
+
+// Launches for rows [at, count) of the caller's table, as many as one takes; returns 0 and moves `at` on.
+template <int CAP>
+int launch(const Tensor* rows, int& at, int count, bool bf16, bool eight, const Hyper& h, const States& st, cudaStream_t stream) {
+  Table<CAP> tab;
+  tab.count = 0;
+  long long chunks = 0;
+  while (at < count && tab.count < CAP) {
+    Tensor t = rows[at];
+    if (t.n < 0 || (t.off & (BLOCK - 1))) return -3;
+    const long long c = (t.n + CHUNK - 1) / CHUNK;
+    if (chunks + c > 0x7fffffffll) {
+      if (!tab.count) return -3;
+      break;
+    }
+    ++at;
+    if (!c) continue;
+    t.first_chunk = static_cast<int>(chunks);
+    tab.t[tab.count++] = t;
+    chunks += c;
+  }
+  if (!tab.count) return 0;
+  const unsigned grid = static_cast<unsigned>(chunks);
+  if (eight) {
+    if (bf16) adamw_multi_kernel<__nv_bfloat16, true, CAP><<<grid, THREADS, 0, stream>>>(tab, h, st);
+    else adamw_multi_kernel<float, true, CAP><<<grid, THREADS, 0, stream>>>(tab, h, st);
+  } else {
+    if (bf16) adamw_multi_kernel<__nv_bfloat16, false, CAP><<<grid, THREADS, 0, stream>>>(tab, h, st);
+    else adamw_multi_kernel<float, false, CAP><<<grid, THREADS, 0, stream>>>(tab, h, st);
+  }
+  return mbh::check_launch("adamw_multi");
 }
 
 }  // namespace
@@ -318,37 +375,12 @@ extern "C" int mb_adamw_multi(const void* tensors, int count, int p_bf16, int bi
   Hyper h;
   h.b1 = hyper[0]; h.omb1 = hyper[1]; h.b2 = hyper[2]; h.omb2 = hyper[3];
   h.decay = hyper[4]; h.step = hyper[5]; h.inv_root = hyper[6]; h.eps = hyper[7];
-  int at = 0;
-  while (at < count) {
-    Table tab;
-    tab.count = 0;
-    long long chunks = 0;
-    while (at < count && tab.count < CAP) {
-      Tensor t = rows[at];
-      if (t.n < 0 || (t.off & (BLOCK - 1))) return -3;
-      const long long c = (t.n + CHUNK - 1) / CHUNK;
-      if (chunks + c > 0x7fffffffll) {
-        if (!tab.count) return -3;
-        break;
-      }
-      ++at;
-      if (!c) continue;
-      t.first_chunk = static_cast<int>(chunks);
-      tab.t[tab.count++] = t;
-      chunks += c;
-    }
-    if (!tab.count) continue;
-    const unsigned grid = static_cast<unsigned>(chunks);
-    const States st{static_cast<uint8_t*>(m), static_cast<uint8_t*>(m_exp), static_cast<uint8_t*>(r), static_cast<uint8_t*>(r_exp),
-                    static_cast<float*>(m), static_cast<float*>(r)};
-    if (bits == 8) {
-      if (p_bf16) adamw_multi_kernel<__nv_bfloat16, true><<<grid, THREADS, 0, stream>>>(tab, h, st);
-      else adamw_multi_kernel<float, true><<<grid, THREADS, 0, stream>>>(tab, h, st);
-    } else {
-      if (p_bf16) adamw_multi_kernel<__nv_bfloat16, false><<<grid, THREADS, 0, stream>>>(tab, h, st);
-      else adamw_multi_kernel<float, false><<<grid, THREADS, 0, stream>>>(tab, h, st);
-    }
-    const int e = mbh::check_launch("adamw_multi");
+  h.one = 1.f;
+  const States st{static_cast<uint8_t*>(m), static_cast<uint8_t*>(m_exp), static_cast<uint8_t*>(r), static_cast<uint8_t*>(r_exp),
+                  static_cast<float*>(m), static_cast<float*>(r)};
+  for (int at = 0; at < count;) {
+    const int e = count - at <= CAP_SMALL ? launch<CAP_SMALL>(rows, at, count, p_bf16, bits == 8, h, st, stream)
+                                          : launch<CAP_LARGE>(rows, at, count, p_bf16, bits == 8, h, st, stream);
     if (e) return e;
   }
   return 0;

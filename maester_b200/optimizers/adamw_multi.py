@@ -20,6 +20,22 @@ from maester_b200.ops import reference as ref
 _TYPES = (torch.float32, torch.bfloat16)
 
 
+class _Slot:
+    """A parameter, where its states lie, and how many steps it has taken."""
+
+    __slots__ = ("param", "offset", "numel", "step", "copy")
+
+    def __init__(self, param, offset: int, numel: int):
+        self.param, self.offset, self.numel, self.step, self.copy = param, offset, numel, 0, None
+
+
+class _Batch:
+    __slots__ = ("group", "dtype", "slots", "params", "table")
+
+    def __init__(self, group: int, dtype: torch.dtype):
+        self.group, self.dtype, self.slots = group, dtype, []
+
+
 class AdamWMulti(Optimizer):
     """``state_bits``: 8 or 32.  All parameters on one device, contiguous, fp32 or bf16, with gradients of their own type; a
     parameter without a gradient is left alone and its step number stays.  bf16 parameters are read, updated in fp32 and
@@ -41,8 +57,10 @@ class AdamWMulti(Optimizer):
         self.state_bits = state_bits
         every = [p for g in self.param_groups for p in g["params"]]
         self.device = every[0].device
-        self._off: dict[torch.Tensor, tuple[int, int]] = {}   # parameter -> (state offset, elements)
+        self._slots: dict[torch.Tensor, _Slot] = {}
+        self._batches: list[_Batch] = []                      # parameters of one group and type: one table, one launch
         total = 0
+        of = {id(p): gi for gi, g in enumerate(self.param_groups) for p in g["params"]}
         for p in every:
             if p.device != self.device:
                 raise ValueError(f"parameters on {self.device} and on {p.device}: one optimizer drives one device")
@@ -50,7 +68,12 @@ class AdamWMulti(Optimizer):
                 raise TypeError(f"fp32 or bf16 parameters are wanted, got {p.dtype}")
             if not p.is_contiguous():
                 raise ValueError(f"a parameter of shape {tuple(p.shape)} is not contiguous (strides {p.stride()})")
-            self._off[p] = (total, p.numel())
+            batch = next((b for b in self._batches if b.group == of[id(p)] and b.dtype == p.dtype), None)
+            if batch is None:
+                batch = _Batch(of[id(p)], p.dtype)
+                self._batches.append(batch)
+            self._slots[p] = slot = _Slot(p, total, p.numel())
+            batch.slots.append(slot)
             total += -(-p.numel() // ref.STATE_BLOCK) * ref.STATE_BLOCK
         if state_bits == 8:
             blocks = total // ref.STATE_BLOCK
@@ -60,8 +83,9 @@ class AdamWMulti(Optimizer):
                              "exp_avg_root": code(), "exp_avg_root_exp": exps(ref.ROOT_MIN_EXP)}
         else:
             self._buffers = {k: torch.zeros(total, device=self.device) for k in ("exp_avg", "exp_avg_sq")}
-        self._steps: dict[torch.Tensor, int] = {p: 0 for p in every}
-        self._copies: dict[torch.Tensor, torch.Tensor] = {}
+        for b in self._batches:
+            b.params = [s.param for s in b.slots]
+            b.table = np.array([(0, 0, 0, s.numel, s.offset, 0) for s in b.slots], dtype=np.int64)
         self.writes_lowp = False    # the sharding runtime's 16-bit parameters are written by step()
         self._sealed = True
 
@@ -79,12 +103,13 @@ class AdamWMulti(Optimizer):
     def attach_copies(self, copies: dict) -> None:
         """{fp32 parameter: bf16 tensor of as many elements}: ``step()`` also writes the updated value there, rounded."""
         for p, c in copies.items():
-            if p not in self._off or p.dtype != torch.float32:
+            if p not in self._slots or p.dtype != torch.float32:
                 raise ValueError("a 16-bit copy belongs to an fp32 parameter of this optimizer")
             if c.dtype != torch.bfloat16 or c.numel() != p.numel() or not c.is_contiguous() or c.device != self.device:
                 raise ValueError(f"the copy of a parameter of {p.numel()} elements has to be a contiguous bf16 tensor of as "
                                  f"many on {self.device}")
-        self._copies.update(copies)
+        for p, c in copies.items():
+            self._slots[p].copy = c
 
     def attach_sharding(self, sharded) -> None:
         """Write the sharding runtime's 16-bit shard with the update (called by the optimizer builder)."""
@@ -93,7 +118,7 @@ class AdamWMulti(Optimizer):
                 or sharded.cpu_offload:
             return
         seg = sharded.flat_segments()
-        self.attach_copies({p: lp[seg[p][0]:seg[p][0] + n] for p, (_, n) in self._off.items() if n})
+        self.attach_copies({p: lp[seg[p][0]:seg[p][0] + s.numel] for p, s in self._slots.items() if s.numel})
         self.writes_lowp = True
 
     # ---- stepping
@@ -105,53 +130,60 @@ class AdamWMulti(Optimizer):
                 loss = closure()
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWMulti.step() cannot be captured: learning rate and step number are launch arguments")
-        work: dict[tuple, list] = {}
-        for gi, group in enumerate(self.param_groups):
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    continue
-                if g.layout is not torch.strided or g.dtype != p.dtype or g.device != p.device:
-                    raise RuntimeError(f"the gradient of a {p.dtype} parameter on {p.device} has to be a dense tensor of its "
-                                       f"type there, got {g.dtype} on {g.device} ({g.layout})")
-                if p.dtype not in _TYPES or p.device != self.device or p.numel() != self._off[p][1] or not p.is_contiguous():
-                    raise RuntimeError("a parameter was replaced by one of another type, device or layout")
-                work.setdefault((gi, p.dtype, self._steps[p] + 1), []).append((p, g if g.is_contiguous() else g.contiguous()))
-        for (gi, dtype, t), pairs in work.items():
-            group = self.param_groups[gi]
+        for batch in self._batches:
+            grads = [p.grad for p in batch.params]
+            live = [i for i, g in enumerate(grads) if g is not None]
+            if not live:
+                continue
+            for i in live:
+                p, g, n = batch.params[i], grads[i], batch.slots[i].numel
+                if g.dtype is not batch.dtype or g.layout is not torch.strided or g.numel() != n or g.device != self.device:
+                    raise RuntimeError(f"the gradient of a {batch.dtype} parameter on {self.device} has to be a dense tensor of "
+                                       f"its type and size there, got {g.dtype} {tuple(g.shape)} on {g.device} ({g.layout})")
+                if p.dtype is not batch.dtype or p.numel() != n or p.device != self.device or not p.is_contiguous():
+                    raise RuntimeError("a parameter was replaced by one of another type, size, device or layout")
+                if not g.is_contiguous():
+                    grads[i] = g.contiguous()
+            group = self.param_groups[batch.group]
             b1, b2 = group["betas"]
             lr = float(group["lr"])
-            hyper = dict(b1=b1, b2=b2, decay=1 - lr * group["weight_decay"], step_size=lr / (1 - b1 ** t),
-                         inv_root=1 / math.sqrt(1 - b2 ** t), eps=group["eps"])
-            (self._launch if self.device.type == "cuda" else self._plain)(pairs, dtype, hyper)
-            for p, _ in pairs:
-                self._steps[p] = t
+            steps = {batch.slots[i].step + 1 for i in live}     # one number, unless some had no gradient before
+            for t in sorted(steps):
+                now = live if len(steps) == 1 else [i for i in live if batch.slots[i].step + 1 == t]
+                hyper = dict(b1=b1, b2=b2, decay=1 - lr * group["weight_decay"], step_size=lr / (1 - b1 ** t),
+                             inv_root=1 / math.sqrt(1 - b2 ** t), eps=group["eps"])
+                (self._launch if self.device.type == "cuda" else self._plain)(batch, now, grads, hyper)
+                for i in now:
+                    batch.slots[i].step = t
         return loss
 
-    def _launch(self, pairs, dtype, h) -> None:
+    def _launch(self, batch, now, grads, h) -> None:
         from maester_b200.ops import cuda as C
-        off, copies = self._off, self._copies
-        rows = [(p.data_ptr(), g.data_ptr(), copies[p].data_ptr() if p in copies else 0, off[p][1], off[p][0], 0)
-                for p, g in pairs]
+        table, slots = batch.table, batch.slots
+        if len(now) < len(slots):
+            table, slots, grads = table[now], [slots[i] for i in now], [grads[i] for i in now]
+        table[:, 0] = [s.param.data_ptr() for s in slots]
+        table[:, 1] = [g.data_ptr() for g in grads]
+        table[:, 2] = [0 if s.copy is None else s.copy.data_ptr() for s in slots]
         f = self._buffers
-        m, r = f["exp_avg"], f["exp_avg_root" if self.state_bits == 8 else "exp_avg_sq"]
-        C.adamw_multi(np.array(rows, dtype=np.int64), dtype == torch.bfloat16, self.state_bits, m, f.get("exp_avg_exp"), r,
-                      f.get("exp_avg_root_exp"),
+        C.adamw_multi(table, batch.dtype is torch.bfloat16, self.state_bits, f["exp_avg"], f.get("exp_avg_exp"),
+                      f["exp_avg_root" if self.state_bits == 8 else "exp_avg_sq"], f.get("exp_avg_root_exp"),
                       (h["b1"], 1 - h["b1"], h["b2"], 1 - h["b2"], h["decay"], h["step_size"], h["inv_root"], h["eps"]))
 
-    def _plain(self, pairs, dtype, h) -> None:
-        for p, g in pairs:
+    def _plain(self, batch, now, grads, h) -> None:
+        for i in now:
+            s, p, g = batch.slots[i], batch.params[i], grads[i]
             m, v = self._moments(p)
-            new, m, root, v = ref.adamw_multi_step(p.data.float().view(-1), g.float().view(-1), m, v, **h)
+            new, m, root, v = ref.adamw_multi_step(p.data.float().view(-1), g.float().reshape(-1), m, v, **h)
             p.copy_(new.view(p.shape))
-            if p in self._copies:
-                self._copies[p].view(-1).copy_(p.view(-1))
+            if s.copy is not None:
+                s.copy.view(-1).copy_(p.view(-1))
             self._store(p, m, root, v)
 
     # ---- states
     def _moments(self, p) -> tuple[torch.Tensor, torch.Tensor]:
         """fp32 (exp_avg, exp_avg_sq) of one parameter, flat."""
-        off, n = self._off[p]
+        off, n = self._slots[p].offset, self._slots[p].numel
         f = self._buffers
         if self.state_bits == 32:
             return f["exp_avg"][off:off + n], f["exp_avg_sq"][off:off + n]
@@ -161,7 +193,7 @@ class AdamWMulti(Optimizer):
         return m, r * r
 
     def _store(self, p, m=None, root=None, v=None) -> None:
-        off, n = self._off[p]
+        off, n = self._slots[p].offset, self._slots[p].numel
         f = self._buffers
         if n == 0:
             return
@@ -184,7 +216,7 @@ class AdamWMulti(Optimizer):
     def param_state(self, p) -> dict[str, torch.Tensor]:
         """What a checkpoint holds of one parameter: ``step``, and fp32 ``exp_avg`` and ``exp_avg_sq`` of its shape."""
         m, v = self._moments(p)
-        return {"step": torch.tensor(float(self._steps[p])), "exp_avg": m.clone().view(p.shape),
+        return {"step": torch.tensor(float(self._slots[p].step)), "exp_avg": m.clone().view(p.shape),
                 "exp_avg_sq": v.clone().view(p.shape)}
 
     @torch.no_grad()
@@ -200,7 +232,7 @@ class AdamWMulti(Optimizer):
                 flat[k] = x.detach().to(device=self.device, dtype=torch.float32).reshape(-1)
         self._store(p, m=flat.get("exp_avg"), v=flat.get("exp_avg_sq"))
         if "step" in state:
-            self._steps[p] = int(state["step"])
+            self._slots[p].step = int(state["step"])
 
     def state_dict(self) -> dict:
         sd = super().state_dict()

@@ -254,7 +254,7 @@ def test_checkpoint_through_the_container(tmp_path):
     a, b = opt.optimizers[0], opt2.optimizers[0]
     for p, q in zip(m.parameters(), m2.parameters()):
         assert all(torch.equal(x, y) for x, y in zip(a._moments(p), b._moments(q))) and a._moments(p)[1].any()
-    assert list(b._steps.values()) == [2] * 4
+    assert [s.step for s in b._slots.values()] == [2] * 4
     # the files of a 32-bit run have the same keys
     m3, opt3 = make("FusedAdamW")
     m3(torch.randn(4, 20)).square().sum().backward()
