@@ -285,6 +285,201 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   }
 }
 
+// ---- few rows of A (tokens of a decoding step): bound by reading B once
+//
+// The roles are swapped: 128 rows of B (output columns) are the M side of the instruction, the rows of A, rounded up to
+// 16, 32 or 64, its N side, so nothing of the accumulator is wasted on rows that do not exist.  A cluster of `split` CTAs shares
+// the contraction of a tile, in whole groups of four k-blocks; three CTAs an SM keep 144 KiB on the way.  The partial sums meet
+// in shared memory over the cluster: CTA r receives the columns of its share of A's rows from all of them and adds them up in
+// the order of the CTAs, so the bits do not depend on timing.
+namespace few {
+
+constexpr int ROWS = 128, STAGES = 3, MAX_N = 64, MAX_SPLIT = 8;
+constexpr int W_BYTES = ROWS * BK, COLS = 128, SF_A = 64, SF_SETS = 16;   // columns: accumulator, then two sets of 4 + 4
+constexpr int SF_STAGE = 1024;
+constexpr int recv_rows(int n) { return n + MAX_SPLIT; }    // split * (n / split rounded up) is less
+constexpr int smem_bytes(int n) { return STAGES * (W_BYTES + n * BK + SF_STAGE) + recv_rows(n) * ROWS * 4 + 1024 + 128; }
+
+struct FewParams {
+  Params p;
+  int n;          // rows of A in the instruction: 16, 32 or 64
+  int split;
+};
+
+__device__ __forceinline__ void umma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void sf_copy(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(const void* ptr, uint32_t cta) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(ptr)), "r"(cta));
+  return a;
+}
+
+__global__ void __launch_bounds__(THREADS, 3)
+fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                    const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb, const FewParams fp) {
+  extern __shared__ uint8_t smem_raw[];
+  const Params& p = fp.p;
+  const int n = fp.n, split = fp.split;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = W_BYTES + n * BK;
+  uint8_t* sf = smem + STAGES * stage_bytes;
+  float* recv = reinterpret_cast<float*>(sf + STAGES * SF_STAGE);     // [split][n / split rounded up][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(recv + recv_rows(n) * ROWS);
+  uint64_t *full = bars, *empty = bars + STAGES, *done = bars + 2 * STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = split > 1 ? cluster_ctarank() : 0u;
+  const int tile = blockIdx.x / split, n0 = tile * ROWS;
+  const int groups = (p.kblocks + 3) / 4;
+  const int kb0 = min(p.kblocks, static_cast<int>(static_cast<long long>(groups) * rank / split) * 4);
+  const int kb1 = min(p.kblocks, static_cast<int>(static_cast<long long>(groups) * (rank + 1) / split) * 4);
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    prefetch_tmap(&tmap_sa);
+    prefetch_tmap(&tmap_sb);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (split > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");   // waited for before the first store into another CTA
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        const int it = kb - kb0, s = it % STAGES;
+        if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1)) {
+          atomicCAS(p.status, 0, ERR_WAIT_EMPTY);
+          ok = false;
+          break;
+        }
+        uint8_t* w = smem + s * stage_bytes;
+        const bool first = (kb & 3) == 0;
+        mbar_expect_tx(&full[s], stage_bytes + (first ? SF_STAGE : 0));
+        tma_load_2d(w, &tmap_b, &full[s], kb * BK, n0);
+        tma_load_2d(w + W_BYTES, &tmap_a, &full[s], kb * BK, 0);
+        if (first) {
+          tma_load_3d(sf + s * SF_STAGE, &tmap_sb, &full[s], 0, kb >> 2, tile);
+          tma_load_3d(sf + s * SF_STAGE + 512, &tmap_sa, &full[s], 0, kb >> 2, 0);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && kb0 < kb1) {
+      const uint32_t idesc = idesc_mxf8(ROWS, 16) + (static_cast<uint32_t>(n - 16) >> 3 << 17);
+      bool ok = true;
+      uint32_t set = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int it = kb - kb0, s = it % STAGES;
+        if (!mbar_wait(&full[s], (it / STAGES) & 1)) {
+          atomicCAS(p.status, 0, ERR_WAIT_FULL);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if ((kb & 3) == 0) {
+          ++set;
+          const uint32_t ss = smem_u32(sf + s * SF_STAGE), col = tmem + SF_A + (set & 1) * SF_SETS;
+          sf_copy(col, sf_desc(ss));
+          sf_copy(col + 4, sf_desc(ss + 512));
+        }
+        const uint32_t sfc = tmem + SF_A + (set & 1) * SF_SETS;
+        const uint32_t id = idesc | (static_cast<uint32_t>(kb & 3) << 29) | (static_cast<uint32_t>(kb & 3) << 4);
+        const uint32_t w = smem_u32(smem + s * stage_bytes);
+        const uint64_t da = make_smem_desc(w, 16, 1024), db = make_smem_desc(w + W_BYTES, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_mxf8(tmem, smem_desc_advance(da, k * 32), smem_desc_advance(db, k * 32), id, sfc, sfc + 4, (it | k) ? 1u : 0u);
+        umma_commit(&empty[s]);
+      }
+      if (ok) umma_commit(done);
+    }
+  } else {
+    const int q = warp & 3, row = q * 32 + lane, col = n0 + row;
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    bool ok = kb0 < kb1;       // (a CTA without k-blocks contributes zeros)
+    if (ok && !mbar_wait(done, 0)) {
+      atomicCAS(p.status, 0, ERR_WAIT_ACC_FULL);
+      ok = false;
+    }
+    tc_fence_after();
+    const int share = (n + split - 1) / split;      // rows of A that a CTA adds up
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    for (int c0 = 0; c0 < n; c0 += 16) {
+      uint32_t r[16];
+      if (kb0 < kb1) {
+        tmem_ld_32x16(taddr + c0, r);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int t = c0 + i;
+        const float v = ok ? __uint_as_float(r[i]) : 0.f;
+        if (split == 1) {
+          if (t < p.M && col < p.N) {
+            const long long at = static_cast<long long>(t) * p.ldc + col;
+            if (p.out == OUT_BF16) static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16(v);
+            else if (p.out == OUT_F32) static_cast<float*>(p.C)[at] = v;
+            else static_cast<float*>(p.C)[at] += v;
+          }
+        } else if (t < p.M) {
+          const uint32_t to = in_cta(recv + (static_cast<int>(rank) * share + t % share) * ROWS + row, t / share);
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+        }
+      }
+    }
+  }
+  if (split > 1) {
+    if (warp < 2) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    const int share = (n + split - 1) / split, t0 = static_cast<int>(rank) * share;
+    if (warp >= 2) {
+      const int row = (warp & 3) * 32 + lane, col = n0 + row;
+      for (int t = t0; t < min(p.M, t0 + share) && col < p.N; ++t) {
+        float v = 0.f;
+        for (int r = 0; r < split; ++r) v += recv[(r * share + t - t0) * ROWS + row];
+        const long long at = static_cast<long long>(t) * p.ldc + col;
+        if (p.out == OUT_BF16) static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16(v);
+        else if (p.out == OUT_F32) static_cast<float*>(p.C)[at] = v;
+        else static_cast<float*>(p.C)[at] += v;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, COLS);
+  }
+}
+
+}  // namespace few
+
 int make_codes_tmap(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t ld, uint32_t box_rows) {
   mbh::EncodeTiledFn fn = mbh::encode_fn();
   if (!fn) return -1;
@@ -329,11 +524,43 @@ extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const v
   if (tiles > 0x7fffffffll / 2) return -3;
   CUtensorMap ta, tb, tsa, tsb;
   const uint64_t cols = static_cast<uint64_t>(kblocks) * 128, groups = (kblocks + 3) / 4;
-  int e = make_codes_tmap(&ta, a, cols, M, lda, BM);
+  const bool few_rows = M <= few::MAX_N;
+  const int n = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  int e = make_codes_tmap(&ta, a, cols, M, lda, few_rows ? n : BM);
   if (!e) e = make_codes_tmap(&tb, b, cols, N, ldb, BNH);
   if (!e) e = make_scales_tmap(&tsa, sa, (M + 127) / 128, groups, 1);
-  if (!e) e = make_scales_tmap(&tsb, sb, (N + 127) / 128, groups, 2);
+  if (!e) e = make_scales_tmap(&tsb, sb, (N + 127) / 128, groups, few_rows ? 1 : 2);
   if (e) return e;
+  if (few_rows) {
+    few::FewParams fp;
+    fp.p = p;
+    fp.n = n;
+    // CTAs of a tile: about two an SM altogether
+    const int rows_tiles = (N + few::ROWS - 1) / few::ROWS;
+    int split = 2 * mbh::sm_count() / rows_tiles;
+    split = split < 1 ? 1 : split > few::MAX_SPLIT ? few::MAX_SPLIT : split;
+    if (split > static_cast<int>(groups)) split = static_cast<int>(groups);
+    fp.split = split;
+    const int smem = few::smem_bytes(n);
+    MB_SET_MAX_SMEM_ONCE(few::fp8_gemm_few_kernel, few::smem_bytes(few::MAX_N));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(rows_tiles * split, 1, 1);
+    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, few::fp8_gemm_few_kernel, ta, tb, tsa, tsb, fp) != cudaSuccess) {
+      const int e2 = mbh::check_launch("fp8_gemm_few");
+      return e2 ? e2 : -100;
+    }
+    return mbh::check_launch("fp8_gemm_few");
+  }
   MB_SET_MAX_SMEM_ONCE(fp8_gemm_kernel, SMEM_BYTES);
   const int max_pairs = mbh::sm_count() / 2;
   const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
