@@ -34,7 +34,8 @@ constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int SF_BYTES = SFA_BYTES + SFB_BYTES;
 constexpr int SF_STRIDE = 2048;
 constexpr int THREADS = 192;
-constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SF_STRIDE) + 1024 + 256;
+constexpr int OUT_STAGE = 4096;                         // 32 x 32 values of an epilogue warp
+constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SF_STRIDE) + 4 * OUT_STAGE + 1024 + 256;
 constexpr int GROUP_M = 8;
 constexpr uint32_t ACC1 = 224, SF_COL = 480, SF_SET = 16, SFB_COL = 4;
 
@@ -81,46 +82,69 @@ constexpr uint32_t idesc_mxf8(int m, int n) {
   return (1u << 23) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)[32], int row, int col0) {
-  if (row >= p.M || col0 >= p.N) return;
-  MB_CHECK_OR(p.status, row >= 0 && col0 >= 0 && static_cast<long long>(min(col0 + 32, p.N)) <= p.ldc, return);
-  const bool whole = p.vec && col0 + 32 <= p.N;
-  const long long at = static_cast<long long>(row) * p.ldc + col0;
+// 32 x 32 accumulators of a warp (lane = row, r = columns) -> C through the warp's 4 KiB of shared memory, so that rows leave
+// as whole sectors: 16 bytes a lane where C allows it, else a value a lane.  16-byte chunks of a row are swizzled so that neither
+// side meets a bank twice.
+__device__ __forceinline__ void store_chunk(const Params& p, const uint32_t (&r)[32], int row0, int col0, uint8_t* stage, int lane) {
+  if (row0 >= p.M || col0 >= p.N) return;          // (the same for the whole warp)
+  MB_CHECK_OR(p.status, row0 >= 0 && col0 >= 0 && static_cast<long long>(min(col0 + 32, p.N)) <= p.ldc, return);
+  const int rows = min(32, p.M - row0), cols = min(32, p.N - col0);
+  const bool whole = p.vec && cols == 32;
+  __syncwarp();
   if (p.out == OUT_BF16) {
-    __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.C) + at;
+    uint4* line = reinterpret_cast<uint4*>(stage + lane * 64);
+    const int x = (lane >> 1) & 3;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint4 o;
+      o.x = pack_bf16(__uint_as_float(r[j * 8 + 0]), __uint_as_float(r[j * 8 + 1]));
+      o.y = pack_bf16(__uint_as_float(r[j * 8 + 2]), __uint_as_float(r[j * 8 + 3]));
+      o.z = pack_bf16(__uint_as_float(r[j * 8 + 4]), __uint_as_float(r[j * 8 + 5]));
+      o.w = pack_bf16(__uint_as_float(r[j * 8 + 6]), __uint_as_float(r[j * 8 + 7]));
+      line[j ^ x] = o;
+    }
+    __syncwarp();
+    __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.C) + static_cast<long long>(row0) * p.ldc + col0;
     if (whole) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint4 o;
-        o.x = pack_bf16(__uint_as_float(r[j * 8 + 0]), __uint_as_float(r[j * 8 + 1]));
-        o.y = pack_bf16(__uint_as_float(r[j * 8 + 2]), __uint_as_float(r[j * 8 + 3]));
-        o.z = pack_bf16(__uint_as_float(r[j * 8 + 4]), __uint_as_float(r[j * 8 + 5]));
-        o.w = pack_bf16(__uint_as_float(r[j * 8 + 6]), __uint_as_float(r[j * 8 + 7]));
-        reinterpret_cast<uint4*>(c)[j] = o;
+        const int row = j * 8 + (lane >> 2), part = lane & 3;
+        const uint4 o = reinterpret_cast<const uint4*>(stage + row * 64)[part ^ ((row >> 1) & 3)];
+        if (row < rows) *reinterpret_cast<uint4*>(c + row * p.ldc + part * 8) = o;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (col0 + i < p.N) c[i] = __float2bfloat16(__uint_as_float(r[i]));
+    } else if (lane < cols) {
+#pragma unroll 4
+      for (int row = 0; row < rows; ++row)
+        c[row * p.ldc + lane] = reinterpret_cast<const __nv_bfloat16*>(stage + row * 64)[(((lane >> 3) ^ ((row >> 1) & 3)) << 3) + (lane & 7)];
     }
   } else {
-    float* c = static_cast<float*>(p.C) + at;
+    uint4* line = reinterpret_cast<uint4*>(stage + lane * 128);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) line[j ^ (lane & 7)] = make_uint4(r[j * 4], r[j * 4 + 1], r[j * 4 + 2], r[j * 4 + 3]);
+    __syncwarp();
+    float* c = static_cast<float*>(p.C) + static_cast<long long>(row0) * p.ldc + col0;
     const bool acc = p.out == OUT_F32_ACC;
     if (whole) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float4 o = make_float4(__uint_as_float(r[j * 4]), __uint_as_float(r[j * 4 + 1]), __uint_as_float(r[j * 4 + 2]),
-                               __uint_as_float(r[j * 4 + 3]));
-        if (acc) {
-          const float4 old = reinterpret_cast<const float4*>(c)[j];
-          o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
+        const int row = j * 4 + (lane >> 3), part = lane & 7;
+        float4 o = reinterpret_cast<const float4*>(stage + row * 128)[part ^ (row & 7)];
+        if (row < rows) {
+          float4* to = reinterpret_cast<float4*>(c + row * p.ldc + part * 4);
+          if (acc) {
+            const float4 old = *to;
+            o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
+          }
+          *to = o;
         }
-        reinterpret_cast<float4*>(c)[j] = o;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (col0 + i < p.N) c[i] = (acc ? c[i] : 0.f) + __uint_as_float(r[i]);
+    } else if (lane < cols) {
+#pragma unroll 4
+      for (int row = 0; row < rows; ++row) {
+        const float v = reinterpret_cast<const float*>(stage + row * 128)[(((lane >> 2) ^ (row & 7)) << 2) + (lane & 3)];
+        float* to = c + row * p.ldc + lane;
+        *to = (acc ? *to : 0.f) + v;
+      }
     }
   }
 }
@@ -131,7 +155,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf = smem + STAGES * STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sf + STAGES * SF_STRIDE);
+  uint8_t* out_stage = sf + STAGES * SF_STRIDE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(out_stage + 4 * OUT_STAGE);
   uint64_t* full = bars;                        // [STAGES] used in the even CTA
   uint64_t* empty = bars + STAGES;              // [STAGES] one per CTA
   uint64_t* acc_full = bars + 2 * STAGES;       // [2]      one per CTA
@@ -255,7 +280,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         break;
       }
       tc_fence_after();
-      const int row = mt * 2 * BM + static_cast<int>(cta) * BM + q * 32 + lane;
+      const int row0 = mt * 2 * BM + static_cast<int>(cta) * BM + q * 32;
       const uint32_t taddr = tmem + (acc ? ACC1 : 0u) + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll 1
       for (int i = 0; i < BN / 32; ++i) {
@@ -268,7 +293,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
           __syncwarp();
           if (lane == 0) mbar_arrive_leader(shared_free);
         }
-        store_chunk(p, r, row, nt * BN + c * 32);
+        store_chunk(p, r, row0, nt * BN + c * 32, out_stage + q * OUT_STAGE, lane);
       }
       tc_fence_before();
       __syncwarp();
@@ -289,16 +314,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 //
 // The roles are swapped: 128 rows of B (output columns) are the M side of the instruction, the rows of A, rounded up to
 // 16, 32 or 64, its N side, so nothing of the accumulator is wasted on rows that do not exist.  A cluster of `split` CTAs shares
-// the contraction of a tile, in whole groups of four k-blocks; three CTAs an SM keep 144 KiB on the way.  The partial sums meet
+// the contraction of a tile, in whole groups of four k-blocks; two CTAs an SM keep 160 KiB on the way.  The partial sums meet
 // in shared memory over the cluster: CTA r receives the columns of its share of A's rows from all of them and adds them up in
 // the order of the CTAs, so the bits do not depend on timing.
 namespace few {
 
-constexpr int ROWS = 128, STAGES = 3, MAX_N = 64, MAX_SPLIT = 8;
+constexpr int ROWS = 128, MAX_STAGES = 5, MAX_N = 64, MAX_SPLIT = 8;
 constexpr int W_BYTES = ROWS * BK, COLS = 128, SF_A = 64, SF_SETS = 16;   // columns: accumulator, then two sets of 4 + 4
 constexpr int SF_STAGE = 1024;
 constexpr int recv_rows(int n) { return n + MAX_SPLIT; }    // split * (n / split rounded up) is less
-constexpr int smem_bytes(int n) { return STAGES * (W_BYTES + n * BK + SF_STAGE) + recv_rows(n) * ROWS * 4 + 1024 + 128; }
+constexpr int stages_of(int n) { return n == 16 ? 5 : n == 32 ? 4 : 3; }   // two CTAs an SM
+constexpr int smem_bytes(int n) { return stages_of(n) * (W_BYTES + n * BK + SF_STAGE) + recv_rows(n) * ROWS * 4 + 1024 + 128; }
+static_assert(smem_bytes(16) <= 113 * 1024 && smem_bytes(32) <= 113 * 1024 && smem_bytes(64) <= 113 * 1024, "");
 
 struct FewParams {
   Params p;
@@ -324,12 +351,19 @@ __device__ __forceinline__ uint32_t in_cta(const void* ptr, uint32_t cta) {
   return a;
 }
 
-__global__ void __launch_bounds__(THREADS, 3)
+__device__ __forceinline__ void store_one(const Params& p, int row, int col, float v) {
+  const long long at = static_cast<long long>(row) * p.ldc + col;
+  if (p.out == OUT_BF16) static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16(v);
+  else if (p.out == OUT_F32) static_cast<float*>(p.C)[at] = v;
+  else static_cast<float*>(p.C)[at] += v;
+}
+
+__global__ void __launch_bounds__(THREADS, 2)
 fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb, const FewParams fp) {
   extern __shared__ uint8_t smem_raw[];
   const Params& p = fp.p;
-  const int n = fp.n, split = fp.split;
+  const int n = fp.n, split = fp.split, STAGES = stages_of(n);
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_bytes = W_BYTES + n * BK;
   uint8_t* sf = smem + STAGES * stage_bytes;
@@ -340,7 +374,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = split > 1 ? cluster_ctarank() : 0u;
-  const int tile = blockIdx.x / split, n0 = tile * ROWS;
+  const int tile = blockIdx.x / split, n0 = tile * ROWS, m0 = blockIdx.y * n;     // columns and rows of C
   const int groups = (p.kblocks + 3) / 4;
   const int kb0 = min(p.kblocks, static_cast<int>(static_cast<long long>(groups) * rank / split) * 4);
   const int kb1 = min(p.kblocks, static_cast<int>(static_cast<long long>(groups) * (rank + 1) / split) * 4);
@@ -381,16 +415,17 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         const bool first = (kb & 3) == 0;
         mbar_expect_tx(&full[s], stage_bytes + (first ? SF_STAGE : 0));
         tma_load_2d(w, &tmap_b, &full[s], kb * BK, n0);
-        tma_load_2d(w + W_BYTES, &tmap_a, &full[s], kb * BK, 0);
+        tma_load_2d(w + W_BYTES, &tmap_a, &full[s], kb * BK, m0);
         if (first) {
           tma_load_3d(sf + s * SF_STAGE, &tmap_sb, &full[s], 0, kb >> 2, tile);
-          tma_load_3d(sf + s * SF_STAGE + 512, &tmap_sa, &full[s], 0, kb >> 2, 0);
+          tma_load_3d(sf + s * SF_STAGE + 512, &tmap_sa, &full[s], 0, kb >> 2, m0 >> 7);
         }
       }
     }
   } else if (warp == 1) {
     if (lane == 0 && kb0 < kb1) {
       const uint32_t idesc = idesc_mxf8(ROWS, 16) + (static_cast<uint32_t>(n - 16) >> 3 << 17);
+      const uint32_t sfb = 4 + ((m0 & 127) >> 5);      // exponents of 32 rows a column
       bool ok = true;
       uint32_t set = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -413,7 +448,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         const uint64_t da = make_smem_desc(w, 16, 1024), db = make_smem_desc(w + W_BYTES, 16, 1024);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_mxf8(tmem, smem_desc_advance(da, k * 32), smem_desc_advance(db, k * 32), id, sfc, sfc + 4, (it | k) ? 1u : 0u);
+          umma_mxf8(tmem, smem_desc_advance(da, k * 32), smem_desc_advance(db, k * 32), id, sfc, sfc + sfb, (it | k) ? 1u : 0u);
         umma_commit(&empty[s]);
       }
       if (ok) umma_commit(done);
@@ -427,9 +462,11 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       ok = false;
     }
     tc_fence_after();
-    const int share = (n + split - 1) / split;      // rows of A that a CTA adds up
+    const int share = (n + split - 1) / split, have = min(n, p.M - m0);      // rows of A that a CTA adds up, and that exist
     if (split > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-    for (int c0 = 0; c0 < n; c0 += 16) {
+    int to_cta = 0, to_row = 0;
+    uint32_t to = split > 1 ? in_cta(recv + static_cast<int>(rank) * share * ROWS + row, 0) : 0u;
+    for (int c0 = 0; c0 < have; c0 += 16) {
       uint32_t r[16];
       if (kb0 < kb1) {
         tmem_ld_32x16(taddr + c0, r);
@@ -440,15 +477,13 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         const int t = c0 + i;
         const float v = ok ? __uint_as_float(r[i]) : 0.f;
         if (split == 1) {
-          if (t < p.M && col < p.N) {
-            const long long at = static_cast<long long>(t) * p.ldc + col;
-            if (p.out == OUT_BF16) static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16(v);
-            else if (p.out == OUT_F32) static_cast<float*>(p.C)[at] = v;
-            else static_cast<float*>(p.C)[at] += v;
+          if (t < have && col < p.N) store_one(p, m0 + t, col, v);
+        } else if (t < have) {
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + to_row * ROWS * 4), "f"(v) : "memory");
+          if (++to_row == share) {
+            to_row = 0;
+            to = in_cta(recv + static_cast<int>(rank) * share * ROWS + row, ++to_cta < split ? to_cta : 0);
           }
-        } else if (t < p.M) {
-          const uint32_t to = in_cta(recv + (static_cast<int>(rank) * share + t % share) * ROWS + row, t / share);
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
         }
       }
     }
@@ -460,13 +495,11 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     const int share = (n + split - 1) / split, t0 = static_cast<int>(rank) * share;
     if (warp >= 2) {
       const int row = (warp & 3) * 32 + lane, col = n0 + row;
-      for (int t = t0; t < min(p.M, t0 + share) && col < p.N; ++t) {
+      const int t1 = min(min(n, p.M - m0), t0 + share);
+      for (int t = t0; t < t1 && col < p.N; ++t) {
         float v = 0.f;
         for (int r = 0; r < split; ++r) v += recv[(r * share + t - t0) * ROWS + row];
-        const long long at = static_cast<long long>(t) * p.ldc + col;
-        if (p.out == OUT_BF16) static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16(v);
-        else if (p.out == OUT_F32) static_cast<float*>(p.C)[at] = v;
-        else static_cast<float*>(p.C)[at] += v;
+        store_one(p, m0 + t, col, v);
       }
     }
   }
@@ -524,8 +557,11 @@ extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const v
   if (tiles > 0x7fffffffll / 2) return -3;
   CUtensorMap ta, tb, tsa, tsb;
   const uint64_t cols = static_cast<uint64_t>(kblocks) * 128, groups = (kblocks + 3) / 4;
-  const bool few_rows = M <= few::MAX_N;
-  const int n = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  // Tiles of 256 x 256 need some 37 of them (half the pairs) to be worth their size; below that, and for few rows, 128 x 64 tiles
+  // with a split contraction put more SMs to work.
+  const int row_tiles = (N + few::ROWS - 1) / few::ROWS;
+  const int n = M <= 16 ? 16 : M <= 32 ? 32 : 64, m_tiles = (M + n - 1) / n;
+  const bool few_rows = (M <= few::MAX_N || tiles < mbh::sm_count() / 4) && m_tiles <= 65535;
   int e = make_codes_tmap(&ta, a, cols, M, lda, few_rows ? n : BM);
   if (!e) e = make_codes_tmap(&tb, b, cols, N, ldb, BNH);
   if (!e) e = make_scales_tmap(&tsa, sa, (M + 127) / 128, groups, 1);
@@ -535,16 +571,16 @@ extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const v
     few::FewParams fp;
     fp.p = p;
     fp.n = n;
-    // CTAs of a tile: about two an SM altogether
-    const int rows_tiles = (N + few::ROWS - 1) / few::ROWS;
-    int split = 2 * mbh::sm_count() / rows_tiles;
+    // CTAs of a tile: two an SM altogether at the most
+    const long long units = static_cast<long long>(row_tiles) * m_tiles;
+    int split = static_cast<int>(2 * mbh::sm_count() / units);
     split = split < 1 ? 1 : split > few::MAX_SPLIT ? few::MAX_SPLIT : split;
     if (split > static_cast<int>(groups)) split = static_cast<int>(groups);
     fp.split = split;
     const int smem = few::smem_bytes(n);
-    MB_SET_MAX_SMEM_ONCE(few::fp8_gemm_few_kernel, few::smem_bytes(few::MAX_N));
+    MB_SET_MAX_SMEM_ONCE(few::fp8_gemm_few_kernel, 113 * 1024);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(rows_tiles * split, 1, 1);
+    cfg.gridDim = dim3(row_tiles * split, m_tiles, 1);
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;

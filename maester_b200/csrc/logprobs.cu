@@ -544,9 +544,19 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
     if (TOP) {
       const int n = blocks * top;
       for (int i = tid; i < n; i += THREADS) {
+        // its place in its own list, and what is greater in the others (each is sorted, best first)
         const u64 e = block_best_of[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += block_best_of[j] > e;
+        int rank = i % top;
+        for (int b = 0; b < blocks && rank < top; ++b) {
+          if (b == i / top) continue;
+          const u64* list = block_best_of + b * top;
+          int lo = 0, hi = top;
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (list[mid] > e) lo = mid + 1; else hi = mid;
+          }
+          rank += lo;
+        }
         if (e && rank < top) best[rank] = e;
       }
       __syncthreads();
