@@ -14,12 +14,13 @@
 //
 // The step moves 18 bytes a value with 8-bit states beside 32-bit parameters and their 16-bit copy (30 with 32-bit states) and
 // is bound by that.  A warp owns 256 consecutive values at a time, so a block's maximum is one warp reduction.
+#include "fp8_common.cuh"
 #include "host_common.cuh"
-#include "sm100.cuh"
-#include <cuda_fp8.h>
 #include <math.h>
 
 namespace {
+
+using namespace mbf8;
 
 constexpr int BLOCK = 256;    // values that share an exponent; one warp
 constexpr int WARP_BLOCKS = 4;                          // neighbouring blocks of a warp
@@ -46,20 +47,9 @@ struct Hyper {
   float one;   // 1, unknown to the compiler: a packed product and sum would be contracted, and ties between two codes go the
 };             // other way then; a fused operation with it is a plain sum
 
-__device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
-
-// smallest k in [k_min, 120] with amax <= 448 * 2^k = 1.75 * 2^(k + 8)
-__device__ __forceinline__ int block_exponent(uint32_t amax_bits, int k_min) {
-  const int e = static_cast<int>(amax_bits >> 23) - 127;                       // amax in [2^e, 2^(e+1)), or below 2^-126
-  const int k = (amax_bits & 0x7fffffu) <= 0x600000u ? e - 8 : e - 7;
-  return min(max(k, k_min), 120);
-}
 __device__ __forceinline__ float floored(float y) { return y > 0.f ? fmaxf(y, 0.001953125f) : y; }   // (NaN stays)
 // four codes in a word; an infinity has become NaN before
-__device__ __forceinline__ uint32_t encode4(float2 a, float2 b) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
+__device__ __forceinline__ uint32_t encode4(float2 a, float2 b) { return encode2(a) | (encode2(b) << 16); }
 __device__ __forceinline__ void decode4(uint32_t w, float2& a, float2& b) {
   a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffffu), __NV_E4M3)));
   b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3)));

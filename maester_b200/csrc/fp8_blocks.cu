@@ -9,29 +9,17 @@
 // tile as one block), of its transpose (blocks along a column), or of both.  A thread holds 8 x 8 values: maxima along rows
 // meet within 16 lanes, maxima along columns through shared memory, and the transposed codes go through a swizzled 16 KiB
 // tile so that both outputs leave as whole 128-byte lines.
+#include "fp8_common.cuh"
 #include "host_common.cuh"
-#include "sm100.cuh"
-#include <cuda_fp8.h>
 
 namespace {
+
+using namespace mbf8;
 
 constexpr int B = 128;
 enum { ROWS = 1, COLS = 2, SQUARE = 4 };
 
 constexpr int THREADS = 256;
-constexpr uint32_t INF16 = 0x7f80u, INF32 = 0x7f800000u;
-
-__device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
-// smallest k in [-117, 120] with amax <= 448 * 2^k = 1.75 * 2^(k + 8)
-__device__ __forceinline__ int block_exponent(uint32_t amax_bits) {
-  const int e = static_cast<int>(amax_bits >> 23) - 127;
-  const int k = (amax_bits & 0x7fffffu) <= 0x600000u ? e - 8 : e - 7;
-  return min(max(k, -117), 120);
-}
-// e4m3 codes of two values (x in the low byte); NaN gives the NaN code
-__device__ __forceinline__ uint32_t encode2(float2 v) {
-  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3));
-}
 
 // 8 x 8 values of one thread.  Maxima are the ordered bits of |x| (16 bits for bf16), over what is finite: a thread that
 // holds an infinity or NaN (seen from its maxima) turns infinities into NaN and takes its maxima again without them.
@@ -231,15 +219,13 @@ struct Patch<float> {
   }
 };
 
-// where the exponent byte of row r (of this 128-row tile) and block b (of this group of 4) lies among 512
-__device__ __forceinline__ int scale_at(int r, int b) { return (r & 31) * 16 + (r >> 5) * 4 + b; }
-
 template <typename T, int MODE>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : MODE == (ROWS | COLS) ? 1 : 2)
 fp8_quantize_kernel(const T* __restrict__ src, int rows, int cols, long long ld, int vec, uint8_t* q, uint8_t* sq, uint8_t* qt,
                     uint8_t* sqt) {
   __shared__ __align__(16) uint8_t tile[(MODE & COLS) ? B * B : 16];
   __shared__ __align__(16) uint32_t maxima[(MODE & COLS) ? 8 * 128 : 8];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (a kernel that was launched to start beside this one may)
   const int rt = blockIdx.y, ct = blockIdx.x, tid = threadIdx.x;
   const int ctiles = (cols + B - 1) / B, rtiles = (rows + B - 1) / B;
   if (rt >= rtiles || ct >= ctiles) {  // past the matrix: only the padding of the exponent bytes

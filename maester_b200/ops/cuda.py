@@ -793,6 +793,22 @@ def fp8_gemm(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tenso
     return out
 
 
+FP8_FEW = 8     # tokens that one pass over a laid-out weight takes without quantising x first
+
+
+def fp8_linear_few(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """``Q(x) @ W.T`` for ``x`` [M <= 8, K] of unit column stride and a weight's codes [N, Kp]."""
+    M, K = x.shape
+    N, Kp = codes.shape
+    y = torch.empty(M, N, device=x.device, dtype=x.dtype)
+    work = torch.empty(M * Kp + (Kp + 511) // 512 * 512, device=x.device, dtype=torch.uint8)   # codes and exponents of x
+    with on_device(x):
+        _ck(_lib.lib().mb_fp8_linear_few(x.data_ptr(), _LOGITS_TYPE[x.dtype], x.stride(0), M, K, work.data_ptr(),
+                                         codes.data_ptr(), scales.data_ptr(), N, codes.stride(0), y.data_ptr(), N, _stream_of(x)),
+            "fp8_linear_few")
+    return y
+
+
 # ------------------------------------------------------------------ AdamW over many tensors
 ADAMW_ROW = 48   # bytes of one row of the tensor table: p, g, copy, n, off (8 bytes each), 8 bytes for the launcher
 

@@ -185,6 +185,8 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor | Fp8Blocks) -> torch.Tensor:
     if grad:
         return _LinearFp8.apply(x, w)
     x2 = _as_matrix(x)
+    if held and x.is_cuda and x2.shape[0] <= _C().FP8_FEW:
+        return _C().fp8_linear_few(x2, w.data, w.scales).view(*x.shape[:-1], N)
     wq = (w.data, w.scales) if held else _quantize(w if w.stride(1) == 1 or K == 1 else w.contiguous(), square=True)[0]
     y = torch.empty(x2.shape[0], N, device=x.device, dtype=x.dtype)
     return _product(_quantize(x2)[0], wq, y).view(*x.shape[:-1], N)
