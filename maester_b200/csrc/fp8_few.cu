@@ -2,10 +2,10 @@
 // tokens: a decoding step, bound by reading the weight's codes once (14336 x 4096: 9 us at the copy rate).
 //
 // Everything else is kept off their way: no staging, no tensor memory, no barrier but one at the end.  A warp takes 32 rows of w
-// and every fourth block of the contraction, with the next block on its way.  The matrix instruction (16 x 8 x 32) does not care
+// and every 4th, 8th or 16th block of the contraction (as many warps share them), with the next block on its way.  The matrix instruction (16 x 8 x 32) does not care
 // in which order the contraction comes, as long as both operands agree: the 16 neighbouring bytes that a lane reads are its
-// values of two instructions, of w and of x alike, so neither operand is ever rearranged.  The four warps' sums meet in shared
-// memory and are added in order.
+// values of two instructions, of w and of x alike, so neither operand is ever rearranged.  The warps' sums meet in shared memory
+// and are added in order.
 //
 // The tokens are quantised by the kernel of fp8_blocks.cu (doing it here instead, once for every 32 rows of w, took longer than
 // the weight: 18.6 us).  This kernel starts while that one runs (programmatic launch): what it reads of w was there before
@@ -15,12 +15,14 @@
 
 extern "C" int mb_fp8_quantize(const void* x, int type, int rows, int cols, long long ld, int mode, void* q, void* sq, void* qt,
                                void* sqt, cudaStream_t stream);
+extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const void* sb, void* c, int M, int N, int kblocks,
+                           long long lda, long long ldb, long long ldc, int out, cudaStream_t stream);
 
 namespace {
 
 using namespace mbf8;
 
-constexpr int TOKENS = 8, ROWS = 32, WARPS = 4, THREADS = WARPS * 32, BLOCK = 128;
+constexpr int TOKENS = 8, ROWS = 32, BLOCK = 128;
 
 __device__ __forceinline__ uint4 load_codes(const uint8_t* p) {
   uint4 v;
@@ -57,8 +59,8 @@ struct Tokens {
   }
 };
 
-template <typename O>
-__global__ void __launch_bounds__(THREADS, 4)
+template <typename O, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS)
 fp8_few_kernel(const uint8_t* x, const uint8_t* sx, int M, int blocks, const uint8_t* __restrict__ w, const uint8_t* __restrict__ sw,
                int N, long long ldw, O* __restrict__ y, long long ldy) {
   __shared__ float sums[WARPS][TOKENS][ROWS + 1];
@@ -110,9 +112,8 @@ fp8_few_kernel(const uint8_t* x, const uint8_t* sx, int M, int blocks, const uin
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[warp][2 * t + (i & 1)][m * 16 + (i >> 1) * 8 + g] = acc[m][i];
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < TOKENS * ROWS / THREADS; ++i) {
-    const int at = i * THREADS + threadIdx.x, to = at / ROWS, r = at % ROWS;
+  for (int at = threadIdx.x; at < TOKENS * ROWS; at += WARPS * 32) {
+    const int to = at / ROWS, r = at % ROWS;
     if (to < M && n0 + r < N) {
       float v = sums[0][to][r];
 #pragma unroll
@@ -123,37 +124,51 @@ fp8_few_kernel(const uint8_t* x, const uint8_t* sx, int M, int blocks, const uin
   }
 }
 
-}  // namespace
-
-// x: [M <= 8, K], row pitch ldx, bf16 (type 0) or fp32 (type 2); work: M x (K rounded up to 128) bytes, rounded up to 16, and
-// 512 bytes for every 512 of K, on a 16-byte boundary; w: [N, K rounded up to 128] codes with row pitch ldw and exponents sw as
-// mb_fp8_quantize writes them; y: [M, N] of x's type, row pitch ldy
-extern "C" int mb_fp8_linear_few(const void* x, int type, long long ldx, int M, int K, void* work, const void* w, const void* sw,
-                                 int N, long long ldw, void* y, long long ldy, cudaStream_t stream) {
-  if (M <= 0 || N <= 0) return 0;
-  if (M > TOKENS || K <= 0 || K > (1 << 30) || (type != 0 && type != 2) || (ldw & 15) || (reinterpret_cast<uintptr_t>(w) & 15) ||
-      (reinterpret_cast<uintptr_t>(work) & 15))
-    return -3;
-  const int blocks = (K + BLOCK - 1) / BLOCK;
-  uint8_t* codes = static_cast<uint8_t*>(work);
-  uint8_t* exps = codes + static_cast<long long>(M) * blocks * BLOCK;
-  const int e = mb_fp8_quantize(x, type, M, K, ldx, 1, codes, exps, nullptr, nullptr, stream);
-  if (e) return e;
+template <typename O, int WARPS>
+int launch(const uint8_t* x, const uint8_t* ex, int M, int blocks, const uint8_t* w, const uint8_t* ew, int N, long long ldw, void* y,
+           long long ldy, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((N + ROWS - 1) / ROWS, 1, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.blockDim = dim3(WARPS * 32, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, fp8_few_kernel<O, WARPS>, x, ex, M, blocks, w, ew, N, ldw, static_cast<O*>(y), ldy);
+  return mbh::check_launch("fp8_few");
+}
+template <typename O>
+int few(const uint8_t* x, const uint8_t* ex, int M, int blocks, const uint8_t* w, const uint8_t* ew, int N, long long ldw, void* y,
+        long long ldy, cudaStream_t stream) {
+  // twelve warps an SM hide the reads (1 x 4096 x 4096: 11.1 us with 4 warps a tile, 8.5 with 8; 4 x 14336 x 4096: 15.0 and 16.5)
+  const long long tiles = (N + ROWS - 1) / ROWS, want = 12ll * mbh::sm_count();
+  if (tiles * 4 >= want || blocks <= 4) return launch<O, 4>(x, ex, M, blocks, w, ew, N, ldw, y, ldy, stream);
+  if (tiles * 8 >= want || blocks <= 8) return launch<O, 8>(x, ex, M, blocks, w, ew, N, ldw, y, ldy, stream);
+  return launch<O, 16>(x, ex, M, blocks, w, ew, N, ldw, y, ldy, stream);
+}
+
+}  // namespace
+
+// y = Q(x) W^T for a weight that was laid out once.  x: [M, K], row pitch ldx, bf16 (type 0) or fp32 (type 2); work (16-byte
+// boundary): M x (K rounded up to 128) bytes and the exponents of as many blocks as mb_fp8_quantize writes them; w: [N, K rounded
+// up to 128] codes with row pitch ldw and exponents sw; y: [M, N] of x's type, row pitch ldy
+extern "C" int mb_fp8_linear(const void* x, int type, long long ldx, int M, int K, void* work, const void* w, const void* sw, int N,
+                             long long ldw, void* y, long long ldy, cudaStream_t stream) {
+  if (M <= 0 || N <= 0) return 0;
+  if (K <= 0 || K > (1 << 30) || (type != 0 && type != 2) || (ldw & 15) || (reinterpret_cast<uintptr_t>(w) & 15) ||
+      (reinterpret_cast<uintptr_t>(work) & 15))
+    return -3;
+  const int blocks = (K + BLOCK - 1) / BLOCK;
+  uint8_t* xc = static_cast<uint8_t*>(work);
+  uint8_t* ec = xc + static_cast<long long>(M) * blocks * BLOCK;
+  const int e = mb_fp8_quantize(x, type, M, K, ldx, 1, xc, ec, nullptr, nullptr, stream);
+  if (e) return e;
+  if (M > TOKENS)
+    return mb_fp8_gemm(xc, ec, w, sw, y, M, N, blocks, static_cast<long long>(blocks) * BLOCK, ldw, ldy, type == 0 ? 0 : 1, stream);
   const uint8_t* wc = static_cast<const uint8_t*>(w);
   const uint8_t* sc = static_cast<const uint8_t*>(sw);
-  const uint8_t *xc = codes, *ec = exps;
-  if (type == 0)
-    cudaLaunchKernelEx(&cfg, fp8_few_kernel<__nv_bfloat16>, xc, ec, M, blocks, wc, sc, N, ldw, static_cast<__nv_bfloat16*>(y), ldy);
-  else
-    cudaLaunchKernelEx(&cfg, fp8_few_kernel<float>, xc, ec, M, blocks, wc, sc, N, ldw, static_cast<float*>(y), ldy);
-  return mbh::check_launch("fp8_few");
+  return type == 0 ? few<__nv_bfloat16>(xc, ec, M, blocks, wc, sc, N, ldw, y, ldy, stream)
+                   : few<float>(xc, ec, M, blocks, wc, sc, N, ldw, y, ldy, stream);
 }

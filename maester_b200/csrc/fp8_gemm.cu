@@ -195,6 +195,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the set-up above may run beside the kernel that writes the operands
 
   if (warp == 0) {
     if (lane == 0) {
@@ -319,7 +320,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 // the order of the CTAs, so the bits do not depend on timing.
 namespace few {
 
-constexpr int ROWS = 128, MAX_STAGES = 5, MAX_N = 64, MAX_SPLIT = 8;
+constexpr int ROWS = 128, MAX_N = 64, MAX_SPLIT = 8;
 constexpr int W_BYTES = ROWS * BK, COLS = 128, SF_A = 64, SF_SETS = 16;   // columns: accumulator, then two sets of 4 + 4
 constexpr int SF_STAGE = 1024;
 constexpr int recv_rows(int n) { return n + MAX_SPLIT; }    // split * (n / split rounded up) is less
@@ -400,6 +401,7 @@ fp8_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   if (split > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");   // waited for before the first store into another CTA
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp == 0) {
     if (lane == 0) {
@@ -584,13 +586,15 @@ extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const v
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = split > 1 ? 1 : 0;
+    cfg.numAttrs = split > 1 ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, few::fp8_gemm_few_kernel, ta, tb, tsa, tsb, fp) != cudaSuccess) {
       const int e2 = mbh::check_launch("fp8_gemm_few");
       return e2 ? e2 : -100;
@@ -605,13 +609,15 @@ extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const v
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, fp8_gemm_kernel, ta, tb, tsa, tsb, p) != cudaSuccess) {
     const int e2 = mbh::check_launch("fp8_gemm");
     return e2 ? e2 : -100;

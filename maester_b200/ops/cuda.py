@@ -725,15 +725,15 @@ _SAME_DEVICE = contextlib.nullcontext()
 def logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor | None, scale: float, entropy: bool, top: int, stats: bool):
     """Rows of ``logits`` [R, V] -> (logprobs | None, entropy | None, top_logprobs | None, top_tokens | None, stats | None)."""
     R, V = logits.shape
-    f32 = dict(device=logits.device, dtype=torch.float32)
-    lp = torch.empty(R, **f32) if tokens is not None else None
-    ent = torch.empty(R, **f32) if entropy else None
-    top_lp = torch.empty(R, top, **f32) if top else None
-    top_id = torch.empty(R, top, device=logits.device, dtype=torch.int64) if top else None
-    st = torch.empty(R, 4, **f32) if stats else None
+    dev, f32, empty = logits.device, torch.float32, torch.empty
+    lp = empty(R, device=dev, dtype=f32) if tokens is not None else None
+    ent = empty(R, device=dev, dtype=f32) if entropy else None
+    top_lp = empty(R, top, device=dev, dtype=f32) if top else None
+    top_id = empty(R, top, device=dev, dtype=torch.int64) if top else None
+    st = empty(R, 4, device=dev, dtype=f32) if stats else None
     with on_device(logits):
         _ck(_lib.lib().mb_logprobs_fwd(logits.data_ptr(), _ptr(tokens), _LOGITS_TYPE[logits.dtype], R, V, logits.stride(0),
-                                       float(scale), _ptr(lp), _ptr(ent), top, _ptr(top_lp), _ptr(top_id), _ptr(st),
+                                       scale, _ptr(lp), _ptr(ent), top, _ptr(top_lp), _ptr(top_id), _ptr(st),
                                        _stream_of(logits)), "logprobs_fwd")
     return lp, ent, top_lp, top_id, st
 
@@ -793,19 +793,49 @@ def fp8_gemm(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tenso
     return out
 
 
-FP8_FEW = 8     # tokens that one pass over a laid-out weight takes without quantising x first
+def _fp8_bytes(rows: int, blocks: int) -> int:
+    """Codes of a matrix and the exponents behind them, in one buffer."""
+    return rows * blocks * 128 + (rows + 127) // 128 * ((blocks + 3) // 4) * 512
 
 
-def fp8_linear_few(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
-    """``Q(x) @ W.T`` for ``x`` [M <= 8, K] of unit column stride and a weight's codes [N, Kp]."""
+def fp8_quantize_packed(x: torch.Tensor, rows: bool = True, cols: bool = False, square: bool = False):
+    """As ``fp8_quantize``, with codes and exponents of an orientation in one uint8 buffer (or None)."""
+    R, C = x.shape
+    rb, cb = (R + 127) // 128, (C + 127) // 128
+    q = torch.empty(_fp8_bytes(R, cb), device=x.device, dtype=torch.uint8) if rows else None
+    qt = torch.empty(_fp8_bytes(C, rb), device=x.device, dtype=torch.uint8) if cols else None
+    p, pt = (q.data_ptr() if rows else 0), (qt.data_ptr() if cols else 0)
+    with on_device(x):
+        _ck(_lib.lib().mb_fp8_quantize(x.data_ptr(), _LOGITS_TYPE[x.dtype], R, C, x.stride(0),
+                                       FP8_ROWS * rows + FP8_COLS * cols + FP8_SQUARE * square, p, p + R * cb * 128,
+                                       pt, pt + C * rb * 128, _stream_of(x)), "fp8_quantize")
+    return q, qt
+
+
+def fp8_gemm_packed(a: torch.Tensor, b: torch.Tensor, blocks: int, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
+    """``out (+)= A @ B.T`` of packed buffers with ``blocks`` blocks of the contraction."""
+    M, N = out.shape
+    Kp = blocks * 128
+    assert a.numel() == _fp8_bytes(M, blocks) and b.numel() == _fp8_bytes(N, blocks) and (out.stride(1) == 1 or N == 1)
+    pa, pb = a.data_ptr(), b.data_ptr()
+    with on_device(out):
+        _ck(_lib.lib().mb_fp8_gemm(pa, pa + M * Kp, pb, pb + N * Kp, out.data_ptr(), M, N, blocks, Kp, Kp, out.stride(0),
+                                   FP8_OUT_F32_ACC if accumulate else FP8_OUT[out.dtype], _stream_of(out)), "fp8_gemm")
+    return out
+
+
+FP8_FEW = 8     # tokens that take the kernel for a decoding step
+
+
+def fp8_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """``Q(x) @ W.T`` for ``x`` [M, K] of unit column stride and a weight's codes [N, Kp]."""
     M, K = x.shape
     N, Kp = codes.shape
     y = torch.empty(M, N, device=x.device, dtype=x.dtype)
-    work = torch.empty(M * Kp + (Kp + 511) // 512 * 512, device=x.device, dtype=torch.uint8)   # codes and exponents of x
+    work = torch.empty(_fp8_bytes(M, Kp // 128), device=x.device, dtype=torch.uint8)   # codes and exponents of x
     with on_device(x):
-        _ck(_lib.lib().mb_fp8_linear_few(x.data_ptr(), _LOGITS_TYPE[x.dtype], x.stride(0), M, K, work.data_ptr(),
-                                         codes.data_ptr(), scales.data_ptr(), N, codes.stride(0), y.data_ptr(), N, _stream_of(x)),
-            "fp8_linear_few")
+        _ck(_lib.lib().mb_fp8_linear(x.data_ptr(), _LOGITS_TYPE[x.dtype], x.stride(0), M, K, work.data_ptr(), codes.data_ptr(),
+                                     scales.data_ptr(), N, codes.stride(0), y.data_ptr(), N, _stream_of(x)), "fp8_linear")
     return y
 
 

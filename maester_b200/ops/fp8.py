@@ -67,22 +67,18 @@ class Fp8Blocks:
 
 
 def _quantize(x: torch.Tensor, rows: bool = True, cols: bool = False, square: bool = False):
-    """(codes and scales of x | None, of x.T | None) of a matrix with unit column stride."""
+    """(x | None, x.T | None) quantised, as ``_product`` takes them, from a matrix with unit column stride: on the GPU one
+    buffer of codes and exponents each."""
     if x.is_cuda:
-        return _C().fp8_quantize(x, rows, cols, square)
-    out = []
-    for want, t in ((rows, x), (cols, x.T)):
-        codes, exps = ref.fp8_quantize(t, square) if want else (None, None)
-        out.append((codes, ref.fp8_pack_exponents(exps)) if want else None)
-    return tuple(out)
+        return _C().fp8_quantize_packed(x, rows, cols, square)
+    return tuple(ref.fp8_dequantize(*ref.fp8_quantize(t, square))[:, :t.shape[1]] if want else None for want, t in ((rows, x), (cols, x.T)))
 
 
-def _product(a, b, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
-    """``out (+)= A @ B.T`` of (codes, scales) pairs."""
+def _product(a, b, K: int, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
+    """``out (+)= A @ B.T`` of two results of ``_quantize`` over a contraction of K values."""
     if out.is_cuda:
-        return _C().fp8_gemm(*a, *b, out, accumulate)
-    va, vb = (ref.fp8_dequantize(c, ref.fp8_unpack_exponents(s, c.shape[0], c.shape[1] // ref.FP8_BLOCK)) for c, s in (a, b))
-    return out.add_(va @ vb.T) if accumulate else out.copy_(va @ vb.T)
+        return _C().fp8_gemm_packed(a, b, (K + 127) // 128, out, accumulate)
+    return out.add_(a @ b.T) if accumulate else out.copy_(a @ b.T)
 
 
 def _as_matrix(x: torch.Tensor) -> torch.Tensor:
@@ -99,8 +95,12 @@ def quantize_fp8(x: torch.Tensor, *, square: bool = False, transpose: bool = Fal
         raise TypeError(f"bf16 or fp32 is wanted, got {x.dtype}")
     x = x.detach()
     x = x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
-    a, b = _quantize(x, not transpose, transpose, square)
-    return Fp8Blocks(*(b if transpose else a), x.shape[0] if transpose else x.shape[1])
+    if x.is_cuda:
+        codes, scales = _C().fp8_quantize(x, not transpose, transpose, square)[int(transpose)]
+    else:
+        codes, exps = ref.fp8_quantize(x.T if transpose else x, square)
+        scales = ref.fp8_pack_exponents(exps)
+    return Fp8Blocks(codes, scales, x.shape[0] if transpose else x.shape[1])
 
 
 def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, *, out_dtype: torch.dtype = torch.bfloat16,
@@ -121,7 +121,10 @@ def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, *, out_dtype: torch.dtype = torch.bfl
         raise ValueError(f"out has to be a row-major {(a.rows, b.rows)} matrix on {a.device}")
     elif out.dtype not in _TYPES or (accumulate and out.dtype != torch.float32):
         raise TypeError(f"out is {out.dtype}: bf16 or fp32 is wanted, fp32 to accumulate")
-    return _product((a.data, a.scales), (b.data, b.scales), out, accumulate)
+    if out.is_cuda:
+        return _C().fp8_gemm(a.data, a.scales, b.data, b.scales, out, accumulate)
+    value = a.dequantize() @ b.dequantize().T
+    return out.add_(value) if accumulate else out.copy_(value)
 
 
 class _LinearFp8(Function):
@@ -135,28 +138,29 @@ class _LinearFp8(Function):
         w2 = w if w.stride(1) == 1 or w.shape[1] == 1 else w.contiguous()
         xq, xt = _quantize(x2, True, need_w)
         wq, wt = _quantize(w2, True, need_x, True)
-        ctx.save_for_backward(w, *(xt or (None, None)), *(wt or (None, None)))
+        ctx.save_for_backward(w, xt, wt)
         ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
         y = torch.empty(x2.shape[0], w.shape[0], device=x.device, dtype=x.dtype)
-        return _product(xq, wq, y).view(*x.shape[:-1], w.shape[0])
+        return _product(xq, wq, w.shape[1], y).view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        w, xt, xts, wt, wts = ctx.saved_tensors
+        w, xt, wt = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad
         dy2 = _as_matrix(dy)
+        T, N = dy2.shape
         dyq, dyt = _quantize(dy2, need_x, need_w)
         dx = dw = None
         if need_x:
-            dx = torch.empty(dy2.shape[0], ctx.x_shape[-1], device=dy.device, dtype=ctx.x_dtype)
-            dx = _product(dyq, (wt, wts), dx).view(ctx.x_shape)
+            dx = torch.empty(T, ctx.x_shape[-1], device=dy.device, dtype=ctx.x_dtype)
+            dx = _product(dyq, wt, N, dx).view(ctx.x_shape)
         if need_w:
             mg = getattr(w, "main_grad", None)
             if mg is not None:
-                _product(dyt, (xt, xts), mg, True)
+                _product(dyt, xt, T, mg, True)
             else:
-                dw = _product(dyt, (xt, xts), torch.empty(w.shape, device=w.device, dtype=w.dtype))
+                dw = _product(dyt, xt, T, torch.empty(w.shape, device=w.device, dtype=w.dtype))
         return dx, dw
 
 
@@ -185,8 +189,11 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor | Fp8Blocks) -> torch.Tensor:
     if grad:
         return _LinearFp8.apply(x, w)
     x2 = _as_matrix(x)
-    if held and x.is_cuda and x2.shape[0] <= _C().FP8_FEW:
-        return _C().fp8_linear_few(x2, w.data, w.scales).view(*x.shape[:-1], N)
-    wq = (w.data, w.scales) if held else _quantize(w if w.stride(1) == 1 or K == 1 else w.contiguous(), square=True)[0]
-    y = torch.empty(x2.shape[0], N, device=x.device, dtype=x.dtype)
-    return _product(_quantize(x2)[0], wq, y).view(*x.shape[:-1], N)
+    if not held:
+        wq = _quantize(w if w.stride(1) == 1 or K == 1 else w.contiguous(), square=True)[0]
+        y = _product(_quantize(x2)[0], wq, K, torch.empty(x2.shape[0], N, device=x.device, dtype=x.dtype))
+    elif x.is_cuda:
+        y = _C().fp8_linear(x2, w.data, w.scales)
+    else:
+        y = matmul_fp8(quantize_fp8(x2), w, out_dtype=x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)

@@ -131,23 +131,27 @@ class AdamWMulti(Optimizer):
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWMulti.step() cannot be captured: learning rate and step number are launch arguments")
         for batch in self._batches:
-            grads = [p.grad for p in batch.params]
-            live = [i for i, g in enumerate(grads) if g is not None]
-            if not live:
-                continue
-            for i in live:
-                p, g, n = batch.params[i], grads[i], batch.slots[i].numel
-                if g.dtype is not batch.dtype or g.layout is not torch.strided or g.numel() != n or g.device != self.device:
-                    raise RuntimeError(f"the gradient of a {batch.dtype} parameter on {self.device} has to be a dense tensor of "
-                                       f"its type and size there, got {g.dtype} {tuple(g.shape)} on {g.device} ({g.layout})")
-                if p.dtype is not batch.dtype or p.numel() != n or p.device != self.device or not p.is_contiguous():
+            grads, live, dtype, device = [p.grad for p in batch.params], [], batch.dtype, self.device.index
+            for i, (s, g) in enumerate(zip(batch.slots, grads)):
+                if g is None:
+                    continue
+                live.append(i)
+                p, n = s.param, s.numel
+                if g.dtype is not dtype or g.layout is not torch.strided or g.numel() != n or (g.get_device() != device
+                                                                                               if g.is_cuda else device is not None):
+                    raise RuntimeError(f"the gradient of a {dtype} parameter on {self.device} has to be a dense tensor of its "
+                                       f"type and size there, got {g.dtype} {tuple(g.shape)} on {g.device} ({g.layout})")
+                if p.dtype is not dtype or p.numel() != n or not p.is_contiguous() or p.is_cuda is not g.is_cuda \
+                        or p.get_device() != g.get_device():
                     raise RuntimeError("a parameter was replaced by one of another type, size, device or layout")
                 if not g.is_contiguous():
                     grads[i] = g.contiguous()
+            if not live:
+                continue
             group = self.param_groups[batch.group]
             b1, b2 = group["betas"]
             lr = float(group["lr"])
-            steps = {batch.slots[i].step + 1 for i in live}     # one number, unless some had no gradient before
+            steps = {batch.slots[i].step + 1 for i in live}   # one number, unless some had no gradient before
             for t in sorted(steps):
                 now = live if len(steps) == 1 else [i for i in live if batch.slots[i].step + 1 == t]
                 hyper = dict(b1=b1, b2=b2, decay=1 - lr * group["weight_decay"], step_size=lr / (1 - b1 ** t),
