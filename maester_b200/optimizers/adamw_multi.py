@@ -10,6 +10,7 @@ Update rule and defaults: torch.optim.AdamW, as configured in maester/config.py:
 from __future__ import annotations
 
 import math
+import operator
 
 import numpy as np
 import torch
@@ -18,6 +19,9 @@ from torch.optim import Optimizer
 from maester_b200.ops import reference as ref
 
 _TYPES = (torch.float32, torch.bfloat16)
+# a step looks at every tensor: mapped over the lists, which takes half the time of a loop
+_grad, _dtype, _layout, _numel = map(operator.attrgetter, ("grad", "dtype", "layout", "numel"))
+_device, _contiguous, _address = torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 
 
 class _Slot:
@@ -131,52 +135,59 @@ class AdamWMulti(Optimizer):
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWMulti.step() cannot be captured: learning rate and step number are launch arguments")
         for batch in self._batches:
-            grads, live, dtype, device = [p.grad for p in batch.params], [], batch.dtype, self.device.index
-            for i, (s, g) in enumerate(zip(batch.slots, grads)):
-                if g is None:
+            slots, params, grads = batch.slots, batch.params, list(map(_grad, batch.params))
+            if any(g is None for g in grads):
+                live = [i for i, g in enumerate(grads) if g is not None]
+                if not live:
                     continue
-                live.append(i)
-                p, n = s.param, s.numel
-                if g.dtype is not dtype or g.layout is not torch.strided or g.numel() != n or (g.get_device() != device
-                                                                                               if g.is_cuda else device is not None):
-                    raise RuntimeError(f"the gradient of a {dtype} parameter on {self.device} has to be a dense tensor of its "
-                                       f"type and size there, got {g.dtype} {tuple(g.shape)} on {g.device} ({g.layout})")
-                if p.dtype is not dtype or p.numel() != n or not p.is_contiguous() or p.is_cuda is not g.is_cuda \
-                        or p.get_device() != g.get_device():
-                    raise RuntimeError("a parameter was replaced by one of another type, size, device or layout")
-                if not g.is_contiguous():
-                    grads[i] = g.contiguous()
-            if not live:
-                continue
+                slots, params, grads = ([x[i] for i in live] for x in (slots, params, grads))
+            self._check(batch, slots, params, grads)
+            if not all(map(_contiguous, grads)):
+                grads = [g.contiguous() for g in grads]
             group = self.param_groups[batch.group]
             b1, b2 = group["betas"]
             lr = float(group["lr"])
-            steps = {batch.slots[i].step + 1 for i in live}   # one number, unless some had no gradient before
-            for t in sorted(steps):
-                now = live if len(steps) == 1 else [i for i in live if batch.slots[i].step + 1 == t]
+            steps = {x.step for x in slots}     # one number, unless some had no gradient before
+            for t in sorted(steps, reverse=True):                 # (downwards: a slot that has moved on is not met again)
+                some = (slots, grads) if len(steps) == 1 else tuple(
+                    [y for x, y in zip(slots, z) if x.step == t] for z in (slots, grads))
+                t += 1
                 hyper = dict(b1=b1, b2=b2, decay=1 - lr * group["weight_decay"], step_size=lr / (1 - b1 ** t),
                              inv_root=1 / math.sqrt(1 - b2 ** t), eps=group["eps"])
-                (self._launch if self.device.type == "cuda" else self._plain)(batch, now, grads, hyper)
-                for i in now:
-                    batch.slots[i].step = t
+                (self._launch if self.device.type == "cuda" else self._plain)(batch, *some, hyper)
+                for x in some[0]:
+                    x.step = t
         return loss
 
-    def _launch(self, batch, now, grads, h) -> None:
+    def _check(self, batch, slots, params, grads) -> None:
+        """Parameters and gradients are what the tables say (a kernel gets nothing but their addresses)."""
+        dtype, device, sizes = batch.dtype, self.device.index if self.device.type == "cuda" else -1, list(map(_numel, slots))
+        if not (set(map(_dtype, grads)) == {dtype} and set(map(_layout, grads)) == {torch.strided}
+                and set(map(_device, grads)) == {device} and list(map(torch.Tensor.numel, grads)) == sizes):
+            g = next(g for g, n in zip(grads, sizes) if g.dtype is not dtype or g.layout is not torch.strided
+                     or g.get_device() != device or g.numel() != n)
+            raise RuntimeError(f"the gradient of a {dtype} parameter on {self.device} has to be a dense tensor of its type and "
+                               f"size there, got {g.dtype} {tuple(g.shape)} on {g.device} ({g.layout})")
+        if not (set(map(_dtype, params)) == {dtype} and set(map(_device, params)) == {device}
+                and list(map(torch.Tensor.numel, params)) == sizes and all(map(_contiguous, params))):
+            raise RuntimeError("a parameter was replaced by one of another type, size, device or layout")
+
+    def _launch(self, batch, slots, grads, h) -> None:
         from maester_b200.ops import cuda as C
-        table, slots = batch.table, batch.slots
-        if len(now) < len(slots):
-            table, slots, grads = table[now], [slots[i] for i in now], [grads[i] for i in now]
+        table = batch.table
+        if len(slots) < len(batch.slots):
+            table = np.array([(0, 0, 0, s.numel, s.offset, 0) for s in slots], dtype=np.int64)
         table[:, 0] = [s.param.data_ptr() for s in slots]
-        table[:, 1] = [g.data_ptr() for g in grads]
+        table[:, 1] = list(map(_address, grads))
         table[:, 2] = [0 if s.copy is None else s.copy.data_ptr() for s in slots]
         f = self._buffers
         C.adamw_multi(table, batch.dtype is torch.bfloat16, self.state_bits, f["exp_avg"], f.get("exp_avg_exp"),
                       f["exp_avg_root" if self.state_bits == 8 else "exp_avg_sq"], f.get("exp_avg_root_exp"),
                       (h["b1"], 1 - h["b1"], h["b2"], 1 - h["b2"], h["decay"], h["step_size"], h["inv_root"], h["eps"]))
 
-    def _plain(self, batch, now, grads, h) -> None:
-        for i in now:
-            s, p, g = batch.slots[i], batch.params[i], grads[i]
+    def _plain(self, batch, slots, grads, h) -> None:
+        for s, g in zip(slots, grads):
+            p = s.param
             m, v = self._moments(p)
             new, m, root, v = ref.adamw_multi_step(p.data.float().view(-1), g.float().reshape(-1), m, v, **h)
             p.copy_(new.view(p.shape))

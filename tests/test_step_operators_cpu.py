@@ -171,6 +171,22 @@ def test_32_bit_states_follow_torch_adamw():
             assert torch.allclose(p, q, rtol=0, atol=5 * (16 * 2.0 ** -24 * (1e-2 + p.abs().max().item())))
 
 
+def test_step_numbers_that_differ():
+    """Parameters that missed steps count their own: each is updated once by a step, whatever number it is at."""
+    a, b = _model(), _model()
+    oa, ob = AdamWMulti(a, state_bits=32, lr=1e-2), torch.optim.AdamW(b, lr=1e-2)
+    for s in range(5):
+        _grads(a, s)
+        _grads(b, s)
+        for i in range(s, len(a)):   # after step s parameters 0 .. s - 1 have been updated
+            a[i].grad = b[i].grad = None
+        oa.step()
+        ob.step()
+        assert [x.step for x in oa._slots.values()] == [max(0, s - i) for i in range(len(a))]
+        for p, q in zip(a, b):
+            assert torch.allclose(p, q, rtol=0, atol=5 * (16 * 2.0 ** -24 * (1e-2 + p.abs().max().item())))
+
+
 def test_8_bit_states_stay_near_32_bit_ones():
     """A code is off by at most 2^-4 of its value (or half the smallest step of its block) before each update; an element's
     update therefore stays within a fraction of the learning rate of the exact one."""
