@@ -156,9 +156,10 @@ struct Sums {
 };
 constexpr float HUGE_LOGIT = 1e30f, ZFAR = -1500.f;      // 2^-1500 is 0
 __device__ __forceinline__ bool plain(float m) { return fabsf(m) < HUGE_LOGIT; }
+__device__ __forceinline__ float base(float m, float k) { return __fmul_rn(m, k); }   // (never contracted: it is one number)
 // base(from) - base(to), at least ZFAR; `from` <= `to`, `to` finite or +inf, `from` may be -inf
 __device__ __forceinline__ float base_step(float from, float to, float k) {
-  const float d = plain(from) && plain(to) ? from * k - to * k : (from - to) * k;
+  const float d = plain(from) && plain(to) ? __fsub_rn(base(from, k), base(to, k)) : (from - to) * k;
   return fmaxf(d, ZFAR);
 }
 // the sums of `a` on the base of m >= a.m.  (t + s d: every old z moves by d.)
@@ -199,7 +200,7 @@ __device__ __forceinline__ void add_values(Sums& a, const Vec<T> (&v)[U], float 
   const float2 k2 = make_float2(k, k);
   if (plain(m) && (!ENT || (Vec<T>::PACKED && low >= Vec<T>::LOWEST))) {
     const uint32_t low2 = Vec<T>::both(low);
-    const float2 nb = make_float2(-(m * k), -(m * k));
+    const float2 nb = make_float2(-base(m, k), -base(m, k));
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -211,7 +212,7 @@ __device__ __forceinline__ void add_values(Sums& a, const Vec<T> (&v)[U], float 
       }
   } else {
     const bool p = plain(m);
-    const float2 nm = p ? make_float2(0.f, 0.f) : make_float2(-m, -m), nb = p ? make_float2(-(m * k), -(m * k)) : make_float2(0.f, 0.f);
+    const float2 nm = p ? make_float2(0.f, 0.f) : make_float2(-m, -m), nb = p ? make_float2(-base(m, k), -base(m, k)) : make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
       const float v = edge_v = to_f(q.row[edge_at]);
       if (v != -INFINITY) {
         a.m = v == v ? v : 0.f;
-        const float z = plain(a.m) ? fmaf(v, k, -(a.m * k)) : (v - a.m) * k, e = ex2(z);
+        const float z = plain(a.m) ? fmaf(v, k, -base(a.m, k)) : (v - a.m) * k, e = ex2(z);
         a.s = e;
         a.t = e * z;
       }
@@ -569,12 +570,12 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
     else if (at < blocks) part = block_parts[at];
     a = merge_lanes<WARPS>(part, k);
     // (log s on the base of m: what k m lost in its rounding is taken out)
-    const float base = a.m * k, log_s = logf(a.s) - (plain(a.m) ? fmaf(a.m, k, -base) * LN2 : 0.f);
+    const float log_s = logf(a.s) - (plain(a.m) ? fmaf(a.m, k, -base(a.m, k)) * LN2 : 0.f);
     if (tid == 0) {
-      const float h = logf(a.s) - a.t / a.s * LN2;
+      const float mean = a.t / a.s, h = logf(a.s) - mean * LN2;     // mean: of z under p
       if (p.tokens) p.logprob[row] = (at_token - a.m) * scale - log_s;
       if (ENT && p.entropy) p.entropy[row] = h;
-      if (p.stats) p.stats[row] = make_float4(a.m, log_s, h, 0.f);
+      if (p.stats) p.stats[row] = make_float4(a.m, 1.f / a.s, mean, 0.f);
     }
     if (TOP && tid < top) {
       const u64 e = best[tid];
@@ -586,13 +587,14 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
 
 // Gradient: reads the logits once more and writes as much.  A block owns `per` vectors of a row (16 bytes of output); where
 // rows of x and dx do not share their 16-byte boundaries it goes value by value, neighbours in neighbouring lanes.
+// With z and s as above p = 2^z / s and log p + H = (z - mean z) ln 2: neither needs a logarithm.
 struct RowGrad {
-  float m, k, log2_s, c0, c1, hot;
-  // p * (c0 + c1 log2 p): c1 carries the entropy's part
+  float m, k, nb, mean, c0, c1, hot;      // z = k (x - m) + nb, with m = 0 and nb = -base where that does not overflow
+  // 2^z (c0 + c1 (z - mean)): both carry -scale / s, c1 the entropy's part
   template <bool ENT>
   __device__ __forceinline__ float at(float x) const {
-    const float l = fmaf(x - m, k, -log2_s), p = ex2(l);
-    return ENT ? p * fmaf(fmaxf(l, -1e4f), c1, c0) : p * c0;
+    const float z = fmaf(x - m, k, nb), e = ex2(z);
+    return ENT ? e * fmaf(fmaxf(z, ZFAR) - mean, c1, c0) : e * c0;
   }
 };
 template <typename G>
@@ -635,7 +637,9 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
   const float gl = g_lp ? g_lp[row] : 0.f, ge = ENT ? g_ent[row] : 0.f;
   float all = gl;
   for (int a = 0; a < top; ++a) all += g_top[row * top + a];
-  const RowGrad f{r.x, scale * LOG2E, r.y * LOG2E, -scale * (all + ge * r.z), -scale * ge * LN2, gl * scale};
+  const float k = scale * LOG2E, per_s = -scale * r.y;
+  const bool p = plain(r.x);
+  const RowGrad f{p ? 0.f : r.x, k, p ? -base(r.x, k) : 0.f, r.z, per_s * all, per_s * ge * LN2, gl * scale};
   auto one = [&](int j) { return f.at<ENT>(to_f(xr[j])) + (j == tok ? f.hot : 0.f); };
   for (int i0 = v0; i0 < v1; i0 += THREADS * U) {
     Vec<T> in[U][L];
