@@ -29,11 +29,12 @@ constexpr long long IGNORE = -100;
 constexpr int MAX_TOP = 64;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float FAR = 1000.f;      // exp(-1000) is 0 in fp32: distances are cut there so that a weight of 0 never meets infinity
-constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int THREADS = 256;       // of a block of the backward pass
 constexpr int CAP = 96;            // entries of a warp's list: more than MAX_TOP and a vector
 constexpr int TURN = 4;            // vectors of a thread's turn
 constexpr int STAGES = 2;          // turns in flight
-constexpr int RESIDENT = 4;        // blocks of an SM (64 registers a thread, 55 KiB a block)
+constexpr int ON_SM = 1024;        // threads of an SM (64 registers each)
+constexpr int CELLS = 1024;        // of a row part, each with a maximum of its own
 constexpr int MAX_CLUSTER = 8;
 typedef unsigned long long u64;
 
@@ -231,20 +232,23 @@ __device__ __forceinline__ void add_values(Sums& a, const Vec<T> (&v)[U], float 
   if (ENT) a.t += t.x + t.y;
 }
 
-// ---- lists of candidates
+// ---- lists of candidates (they lie where the copies lay)
+template <int TH>
 struct Lists {
+  static constexpr int WARPS = TH / 32;
   u64 entry[WARPS][CAP];
   u64 merged[WARPS * CAP];   // survivors of this block
   u64 threshold;                 // an entry below it is not among the best
-  uint32_t maxima[THREADS / 2];  // of groups of 2 or 4 threads (as ordered whole numbers, 0: none)
-  uint16_t queue[THREADS];       // threads that reach the threshold
+  uint32_t maxima[128];          // of 64 or 128 groups of threads (as ordered whole numbers)
+  uint16_t queue[CELLS];   // cells that reach the threshold
   int queued;
   int count[WARPS];
   int survivors;
 };
 
 // Cut a warp's list of n entries (n >= top) down to its best `top`, best first; their last one becomes the threshold.
-__device__ __noinline__ void cut_list(Lists& l, int warp, int lane, int n, int top) {
+template <int TH>
+__device__ __noinline__ void cut_list(Lists<TH>& l, int warp, int lane, int n, int top) {
   static_assert(CAP % 32 == 0 && CAP >= MAX_TOP + 16, "");
   u64 mine[CAP / 32];
   int rank[CAP / 32];
@@ -291,8 +295,8 @@ __device__ __forceinline__ uint32_t top_of_maxima(const uint32_t* maxima, int la
 
 // Values above the threshold go into the warp's list (n entries, returned).  Every lane brings a vector whose first value has
 // index j0 (valid: there is one).  The whole warp calls this together and looks at one vector at a time, a value per lane.
-template <typename T>
-__device__ __forceinline__ int offer(Lists& l, const Vec<T>& v, bool valid, uint32_t j0, int n, int warp, int lane, int top) {
+template <typename T, int TH>
+__device__ __forceinline__ int offer(Lists<TH>& l, const Vec<T>& v, bool valid, uint32_t j0, int n, int warp, int lane, int top) {
   constexpr int N = Vec<T>::N;
   u64 thr = *const_cast<volatile u64*>(&l.threshold);
   // the best entry that the vector can hold: its maximum at its first index
@@ -323,10 +327,11 @@ __device__ __forceinline__ int offer(Lists& l, const Vec<T>& v, bool valid, uint
 }
 
 // Best `top` entries of the block, best first, into out (missing ones 0).  All threads call this; a barrier is inside.
-__device__ __forceinline__ void block_best(Lists& l, u64* out, int top, int tid) {
+template <int TH>
+__device__ __forceinline__ void block_best(Lists<TH>& l, u64* out, int top, int tid) {
   __syncthreads();
   const u64 thr = l.threshold;
-  for (int i = tid; i < WARPS * CAP; i += THREADS) {
+  for (int i = tid; i < l.WARPS * CAP; i += TH) {
     const int w = i / CAP, j = i % CAP;
     if (j < l.count[w]) {
       const u64 e = l.entry[w][j];
@@ -336,7 +341,7 @@ __device__ __forceinline__ void block_best(Lists& l, u64* out, int top, int tid)
   if (tid < top) out[tid] = 0;
   __syncthreads();
   const int n = l.survivors;
-  for (int i = tid; i < n; i += THREADS) {
+  for (int i = tid; i < n; i += TH) {
     const u64 e = l.merged[i];
     int rank = 0;
 #pragma unroll 8
@@ -344,7 +349,6 @@ __device__ __forceinline__ void block_best(Lists& l, u64* out, int top, int tid)
     if (rank < top) out[rank] = e;
   }
   __syncthreads();
-
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -392,16 +396,18 @@ struct FwdArgs {
   int* status;
 };
 
-template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T* __restrict__ x, const FwdArgs p) {
-  constexpr int N = Vec<T>::N, U = TURN;
+template <typename T, bool ENT, bool TOP, int TH>
+__global__ void __launch_bounds__(TH, ON_SM / TH) logprobs_fwd_kernel(const T* __restrict__ x, const FwdArgs p) {
+  constexpr int N = Vec<T>::N, U = TURN, WARPS = TH / 32, PARTS = CELLS / TH;
   __shared__ Sums parts[WARPS];
   __shared__ Sums block_parts[MAX_CLUSTER];          // first block: one of each block of the cluster
   __shared__ u64 block_best_of[TOP ? MAX_CLUSTER * MAX_TOP : 1];
   __shared__ u64 best[TOP ? MAX_TOP : 1];
   extern __shared__ __align__(16) uint8_t dynamic[];
-  uint4* slots = reinterpret_cast<uint4*>(dynamic);  // [STAGES][U][THREADS]
-  Lists& l = *reinterpret_cast<Lists*>(dynamic + STAGES * U * THREADS * 16);
+  uint4* slots = reinterpret_cast<uint4*>(dynamic);  // [STAGES][U][TH]
+  Lists<TH>& l = *reinterpret_cast<Lists<TH>*>(dynamic);     // ... after the last of them has been read
+  static_assert(sizeof(Lists<TH>) <= STAGES * U * TH * 16, "");
+  __shared__ uint16_t cells[TOP ? CELLS : 1];   // upper half of (the largest value as an ordered whole number)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.V, blocks = p.blocks, top = p.top;
   const int block = blocks > 1 ? static_cast<int>(cluster_rank()) : 0;
   const long long row = blockIdx.x / blocks;
@@ -424,17 +430,16 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
     return;
   }
   if (blocks > 1) cluster_arrive();   // (waited for before the first store into another block: it has started by then)
-  if (TOP && tid == 0) l.survivors = l.queued = 0;
   const Part<T> q(x + row * p.ld, V, blocks, block);
   const T* from = q.row + q.head;
   int copied = q.v0, into = 0;
   auto copy_turn = [&]() {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int at = copied + u * THREADS + tid;
-      if (at < q.v1) copy16(&slots[(into * U + u) * THREADS + tid], from + static_cast<long long>(at) * N);
+      const int at = copied + u * TH + tid;
+      if (at < q.v1) copy16(&slots[(into * U + u) * TH + tid], from + static_cast<long long>(at) * N);
     }
-    copied += THREADS * U;
+    copied += TH * U;
     into = into + 1 == STAGES ? 0 : into + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -461,17 +466,28 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
       }
     }
   }
-  float most = edge_v;    // largest value of this thread; NaN if there is one
+  const int turns = (q.v1 - q.v0 + TH * U - 1) / (TH * U), part = max(1, (turns + PARTS - 1) / PARTS);   // turns of a cell
+  float most = edge_v;    // largest value of the cell; NaN if there is one
+  uint32_t highest = 0;   // of the thread's cells
+  int cell = tid, left = part;
+  auto end_cell = [&]() {
+    const uint32_t key = order_of(most);
+    cells[cell] = static_cast<uint16_t>(key >> 16);
+    highest = max(highest, key);
+    cell += TH;
+    most = -INFINITY;
+    left = part;
+  };
   int stage = 0;
-  for (int i0 = q.v0; i0 < q.v1; i0 += THREADS * U) {
+  for (int i0 = q.v0; i0 < q.v1; i0 += TH * U) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     Vec<T> v[U];
     float cm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint4 w = slots[(stage * U + u) * THREADS + tid];
+      const uint4 w = slots[(stage * U + u) * TH + tid];
       v[u].w[0] = w.x; v[u].w[1] = w.y; v[u].w[2] = w.z; v[u].w[3] = w.w;
-      if (i0 + u * THREADS + tid >= q.v1) {   // nothing there: -inf, no weight
+      if (i0 + u * TH + tid >= q.v1) {   // nothing there: -inf, no weight
         const uint32_t none = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
         v[u].w[0] = v[u].w[1] = v[u].w[2] = v[u].w[3] = none;
       }
@@ -479,23 +495,32 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
     copy_turn();          // into the slots that were just read
-    if (TOP) most = max_nan(most, cm);
+    if (TOP) {
+      most = max_nan(most, cm);
+      if (--left == 0) end_cell();
+    }
     add_values<T, U, ENT>(a, v, cm, k, far);
   }
   a = merge_lanes<32>(a, k);
   if (lane == 0) parts[warp] = a;
   if (TOP) {
-    const uint32_t key = q.v0 + tid < q.v1 || has_edge ? order_of(most) : 0u;
-    // groups of four threads where `top` is at most half their number, else of two: the fewer, the shorter the search, and
-    // only threads that reach the threshold themselves are looked at again
-    uint32_t group = max(key, __shfl_xor_sync(~0u, key, 1));
-    if (top <= 32) group = max(group, __shfl_xor_sync(~0u, group, 2));
-    if (!(tid & (top <= 32 ? 3 : 1))) l.maxima[top <= 32 ? tid >> 2 : tid >> 1] = group;
+    if (left != part || cell == tid) end_cell();
+    // 64 groups of threads where `top` is at most half their number, else 128: the fewer, the shorter the search, and only
+    // cells that reach the threshold themselves are looked at again
+    const int in_group = TH / (top <= 32 ? 64 : 128);
+    uint32_t group = highest;
+    if (in_group >= 2) group = max(group, __shfl_xor_sync(~0u, group, 1));
+    if (in_group >= 4) group = max(group, __shfl_xor_sync(~0u, group, 2));
+    __syncthreads();       // (the copies have been read: the lists take their place)
+    if (tid % in_group == 0) l.maxima[tid / in_group] = group;
+    if (tid == 0) l.survivors = l.queued = 0;
     __syncthreads();
     const uint32_t reached = top <= 32 ? top_of_maxima<2>(l.maxima, lane, top) : top_of_maxima<4>(l.maxima, lane, top);
     const u64 thr = reached ? (static_cast<u64>(reached) << 32) - 1 : 0;   // (every entry of that value is above it)
     if (tid == 0) l.threshold = thr;
-    if (key && key > static_cast<uint32_t>(thr >> 32)) l.queue[atomicAdd(&l.queued, 1)] = static_cast<uint16_t>(tid);
+    if (highest >= reached)
+      for (int c = tid; c < cell; c += TH)
+        if (cells[c] >= reached >> 16) l.queue[atomicAdd(&l.queued, 1)] = static_cast<uint16_t>(c);
     __syncthreads();
     int listed = 0;
     if (warp == 0) {   // the ragged ends: at most 14 values
@@ -504,21 +529,21 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
       if (e > thr) l.entry[0][__popc(kept & ((1u << lane) - 1u))] = e;
       listed = __popc(kept);
     }
-    const int turns = (q.v1 - q.v0 + THREADS - 1) / THREADS, items = l.queued * turns;   // (at most the block's vectors and 255)
-    for (int i0 = warp * 32; i0 < items; i0 += THREADS * 2) {
+    const int of_cell = part * U, items = l.queued * of_cell;   // vectors (at most the block's and the ends of its cells)
+    for (int i0 = lane * WARPS + warp; i0 - lane * WARPS < items; i0 += TH * 2) {   // (neighbours to different warps)
       Vec<T> v[2];
       uint32_t j0[2];
       bool valid[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int item = i0 + u * THREADS + lane, w = item / turns;
-        const int at = item < items ? q.v0 + l.queue[w] + (item - w * turns) * THREADS : q.v1;
+        const int item = i0 + u * TH, w = item / of_cell, c = item < items ? l.queue[w] : 0;
+        const int at = item < items ? q.v0 + (c / TH * of_cell + item - w * of_cell) * TH + c % TH : q.v1;
         valid[u] = at < q.v1;
         j0[u] = static_cast<uint32_t>(q.head + at * N);
         if (valid[u]) v[u] = load_vec(q.row + j0[u]);
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) listed = offer<T>(l, v[u], valid[u], j0[u], listed, warp, lane, top);
+      for (int u = 0; u < 2; ++u) listed = offer<T, TH>(l, v[u], valid[u], j0[u], listed, warp, lane, top);
     }
     if (lane == 0) l.count[warp] = listed;
     block_best(l, best, top, tid);
@@ -544,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) logprobs_fwd_kernel(const T
     if (block) return;
     if (TOP) {
       const int n = blocks * top;
-      for (int i = tid; i < n; i += THREADS) {
+      for (int i = tid; i < n; i += TH) {
         // its place in its own list, and what is greater in the others (each is sorted, best first)
         const u64 e = block_best_of[i];
         int rank = i % top;
@@ -688,8 +713,8 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
 
 // Blocks of a row: the split with the fewest waves times the length of one.  A block costs its vectors and about 1500 more (its
 // start, the reductions, the alternatives), a cluster's barrier some 500.
-int blocks_per_row(int rows, int V, int elem) {
-  const long long slots = static_cast<long long>(RESIDENT) * mbh::sm_count(), vectors = static_cast<long long>(V) * elem / 16;
+int blocks_per_row(int rows, int V, int elem, bool& small) {
+  const long long sms = mbh::sm_count(), slots = ON_SM / 256 * sms, vectors = static_cast<long long>(V) * elem / 16;
   int best = 1;
   long long least = 0;
   for (int b = 1; b <= MAX_CLUSTER; b *= 2) {
@@ -700,16 +725,18 @@ int blocks_per_row(int rows, int V, int elem) {
       best = b;
     }
   }
-  return best;
+  const long long of_small = ON_SM / 128 * sms, cost = (rows + of_small - 1) / of_small * (2 * vectors + 1500);
+  small = cost < least;
+  return small ? 1 : best;
 }
 
-template <typename T, bool ENT, bool TOP>
+template <typename T, bool ENT, bool TOP, int TH>
 int launch_fwd(const void* x, const FwdArgs& p, cudaStream_t stream) {
-  constexpr int smem = STAGES * TURN * THREADS * 16 + (TOP ? static_cast<int>(sizeof(Lists)) : 0);
-  MB_SET_MAX_SMEM_ONCE((logprobs_fwd_kernel<T, ENT, TOP>), smem);
+  constexpr int smem = STAGES * TURN * TH * 16;
+  MB_SET_MAX_SMEM_ONCE((logprobs_fwd_kernel<T, ENT, TOP, TH>), smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.rows * p.blocks, 1, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.blockDim = dim3(TH, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -719,14 +746,20 @@ int launch_fwd(const void* x, const FwdArgs& p, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.blocks > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, ENT, TOP>, static_cast<const T*>(x), p);
+  cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, ENT, TOP, TH>, static_cast<const T*>(x), p);
   return mbh::check_launch("logprobs_fwd");
 }
-template <typename T>
+template <typename T, int TH>
 int fwd(const void* x, const FwdArgs& p, cudaStream_t stream) {
   const bool ent = p.entropy || p.stats;   // (the entropy's gradient needs the entropy)
-  if (p.top) return ent ? launch_fwd<T, true, true>(x, p, stream) : launch_fwd<T, false, true>(x, p, stream);
-  return ent ? launch_fwd<T, true, false>(x, p, stream) : launch_fwd<T, false, false>(x, p, stream);
+  if (p.top) return ent ? launch_fwd<T, true, true, TH>(x, p, stream) : launch_fwd<T, false, true, TH>(x, p, stream);
+  return ent ? launch_fwd<T, true, false, TH>(x, p, stream) : launch_fwd<T, false, false, TH>(x, p, stream);
+}
+template <typename T>
+int fwd(const void* x, FwdArgs& p, cudaStream_t stream) {
+  bool small;
+  p.blocks = blocks_per_row(p.rows, p.V, sizeof(T), small);
+  return small ? fwd<T, 128>(x, p, stream) : fwd<T, 256>(x, p, stream);
 }
 
 }  // namespace
@@ -741,7 +774,7 @@ extern "C" int mb_logprobs_fwd(const void* x, const long long* tokens, int type,
   if (type < T_BF16 || type > T_F32) return -3;
   int* status = mbh::status().dev;
   if (!status) return -4;
-  const FwdArgs p{tokens, rows, V, ld, scale, blocks_per_row(rows, V, type == T_F32 ? 4 : 2), logprob, entropy, top, top_lp, top_id,
+  FwdArgs p{tokens, rows, V, ld, scale, 1, logprob, entropy, top, top_lp, top_id,
                   static_cast<float4*>(stats), status};
   return type == T_BF16 ? fwd<__nv_bfloat16>(x, p, stream) : type == T_F16 ? fwd<__half>(x, p, stream) : fwd<float>(x, p, stream);
 }

@@ -105,6 +105,22 @@ def test_orders_and_masks(kind, rows, V):
         _check_fwd(ops.token_logprobs(xs, tokens, scale=scale, entropy=True, top=min(40, V)), xs, tokens, scale, min(40, V))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,V", [(700, 6), (700, 100), (800, 4099), (1200, 16003), (601, 32000)])
+def test_rows_that_share_an_sm(rows, V, dtype):
+    """More rows than blocks of 256 threads fit on the GPU at once: blocks are smaller then.  Random rows, and one whose
+    best values lie next to each other, one that ascends, one that is constant, one without a finite value but the last."""
+    x = _logits(rows, V, dtype, 1)
+    x[3, V // 2:V // 2 + 70] = 50.0
+    x[4] = torch.arange(V, device="cuda") / V
+    x[5] = -2.5
+    x[6, :-1] = -math.inf
+    tokens = torch.randint(0, V, (rows,), device="cuda")
+    tokens[1], tokens[6] = -100, V - 1
+    for top in sorted({0, 1, min(20, V), min(33, V), min(64, V)}):
+        _check_fwd(ops.token_logprobs(x, tokens, scale=0.9, entropy=True, top=top), x, tokens, 0.9, top)
+
+
 def test_rows_without_a_distribution():
     x = torch.zeros(5, 3000, device="cuda")
     x[0] = -math.inf
