@@ -30,7 +30,7 @@ constexpr int MAX_TOP = 64;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float FAR = 1000.f;      // exp(-1000) is 0 in fp32: distances are cut there so that a weight of 0 never meets infinity
 constexpr int THREADS = 256;       // of a block of the backward pass
-constexpr int CAP = 96;            // entries of a warp's list: more than MAX_TOP and a vector
+constexpr int CAP = 96;            // entries of a warp's list: MAX_TOP and one of each lane
 constexpr int TURN = 4;            // vectors of a thread's turn
 constexpr int STAGES = 2;          // turns in flight
 constexpr int ON_SM = 1024;        // threads of an SM (64 registers each)
@@ -239,7 +239,7 @@ struct Lists {
   u64 entry[WARPS][CAP];
   u64 merged[WARPS * CAP];   // survivors of this block
   u64 threshold;                 // an entry below it is not among the best
-  uint32_t maxima[128];          // of 64 or 128 groups of threads (as ordered whole numbers)
+  alignas(16) uint32_t maxima[128];          // of 64 or 128 groups of threads (as ordered whole numbers)
   uint16_t queue[CELLS];   // cells that reach the threshold
   int queued;
   int count[WARPS];
@@ -249,7 +249,7 @@ struct Lists {
 // Cut a warp's list of n entries (n >= top) down to its best `top`, best first; their last one becomes the threshold.
 template <int TH>
 __device__ __noinline__ void cut_list(Lists<TH>& l, int warp, int lane, int n, int top) {
-  static_assert(CAP % 32 == 0 && CAP >= MAX_TOP + 16, "");
+  static_assert(CAP % 32 == 0 && CAP >= MAX_TOP + 32, "");
   u64 mine[CAP / 32];
   int rank[CAP / 32];
 #pragma unroll
@@ -272,81 +272,77 @@ __device__ __noinline__ void cut_list(Lists<TH>& l, int warp, int lane, int n, i
   __syncwarp();
 }
 
-// Largest key, as far as its upper half goes, that at least `top` of 32 G maxima reach (0: fewer have a value); two bits a step.
-template <int G>
-__device__ __forceinline__ uint32_t top_of_maxima(const uint32_t* maxima, int lane, int top) {
-  uint32_t key[G], t = 0;
-#pragma unroll
-  for (int i = 0; i < G; ++i) key[i] = maxima[i * 32 + lane];
-  auto reach = [&](uint32_t c) {
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < G; ++i) n += __popc(__ballot_sync(~0u, key[i] >= c));
-    return n >= top;
-  };
-#pragma unroll
-  for (int bit = 30; bit >= 16; bit -= 2) {
-    const uint32_t c1 = t | (1u << bit), c2 = t | (2u << bit), c3 = t | (3u << bit);
-    const bool r1 = reach(c1), r2 = reach(c2), r3 = reach(c3);
-    t = r3 ? c3 : r2 ? c2 : r1 ? c1 : t;
+// The top-th largest of G keys, of which this thread (and GROUP - 1 neighbours that share the work) holds `mine`, becomes the
+// threshold: its upper half, as the lowest entry with it.  Every key is compared with every other, G / GROUP comparisons a
+// thread; the lower half of a key is its place, so that all differ.
+template <int G, int TH>
+__device__ __forceinline__ void set_threshold(Lists<TH>& l, uint32_t mine, int tid, int top) {
+  constexpr int GROUP = TH / G, PER = G / GROUP;
+  const int from = tid % GROUP * PER;
+  int rank = 0;
+#pragma unroll 4
+  for (int i = 0; i < PER; i += 4) {
+    const uint4 k = *reinterpret_cast<const uint4*>(&l.maxima[from + i]);
+    rank += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
   }
-  return t;
+#pragma unroll
+  for (int o = GROUP / 2; o; o >>= 1) rank += __shfl_xor_sync(~0u, rank, o);
+  if (rank == top - 1 && tid % GROUP == 0) l.threshold = static_cast<u64>(mine & 0xffff0000u) << 32;
 }
 
-// Values above the threshold go into the warp's list (n entries, returned).  Every lane brings a vector whose first value has
-// index j0 (valid: there is one).  The whole warp calls this together and looks at one vector at a time, a value per lane.
+// Entries of at least the threshold go into the warp's list (n entries, returned).  Every lane brings a vector whose first value
+// has index j0 (valid: there is one).  The whole warp calls this together.
 template <typename T, int TH>
 __device__ __forceinline__ int offer(Lists<TH>& l, const Vec<T>& v, bool valid, uint32_t j0, int n, int warp, int lane, int top) {
-  constexpr int N = Vec<T>::N;
   u64 thr = *const_cast<volatile u64*>(&l.threshold);
-  // the best entry that the vector can hold: its maximum at its first index
-  const u64 most = valid ? entry_of(v.top(), j0) : 0;
-  for (uint32_t h = __ballot_sync(~0u, most > thr); h; h &= h - 1) {
-    const int from = __ffs(h) - 1;
-    if (__shfl_sync(~0u, most, from) <= thr) continue;    // (a cut has raised the threshold)
-    uint32_t w[4];
+  float least = value_of(static_cast<uint32_t>(thr >> 32));      // (may be NaN: then all are looked at)
+  if (!__any_sync(~0u, valid && !(v.top() < least))) return n;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __shfl_sync(~0u, v.w[i], from);
-    const uint32_t first = __shfl_sync(~0u, j0, from);
-    const int i = lane & (N - 1), word = N == 8 ? i >> 1 : i;
-    Vec<T> mine;
-    mine.w[0] = word == 0 ? w[0] : word == 1 ? w[1] : word == 2 ? w[2] : w[3];
-    const u64 e = entry_of(N == 8 && (i & 1) ? mine.at(1) : mine.at(0), first + i);
-    const bool keep = lane < N && e > thr;
-    const uint32_t kept = __ballot_sync(~0u, keep);
-    if (keep) l.entry[warp][n + __popc(kept & ((1u << lane) - 1u))] = e;
-    n += __popc(kept);
-    if (n > CAP - N) {
+  for (int i = 0; i < Vec<T>::N; ++i) {
+    if (!__any_sync(~0u, valid && !(v.at(i) < least))) continue;
+    const u64 e = valid ? entry_of(v.at(i), j0 + i) : 0;
+    uint32_t kept = __ballot_sync(~0u, e >= thr);
+    if (n + __popc(kept) > CAP) {
       __syncwarp();
       cut_list(l, warp, lane, n, top);
       n = top;
       thr = *const_cast<volatile u64*>(&l.threshold);
+      least = value_of(static_cast<uint32_t>(thr >> 32));
+      kept = __ballot_sync(~0u, e >= thr);
     }
+    if (kept >> lane & 1) l.entry[warp][n + __popc(kept & ((1u << lane) - 1u))] = e;
+    n += __popc(kept);
   }
   return n;
 }
 
-// Best `top` entries of the block, best first, into out (missing ones 0).  All threads call this; a barrier is inside.
-template <int TH>
-__device__ __forceinline__ void block_best(Lists<TH>& l, u64* out, int top, int tid) {
-  __syncthreads();
-  const u64 thr = l.threshold;
-  for (int i = tid; i < l.WARPS * CAP; i += TH) {
-    const int w = i / CAP, j = i % CAP;
-    if (j < l.count[w]) {
-      const u64 e = l.entry[w][j];
-      if (e >= thr) l.merged[atomicAdd(&l.survivors, 1)] = e;   // (the entry that set the threshold is among the best)
-    }
+// Best `top` of the entries get(0 .. n - 1), of which 0 is none, best first, into out (missing ones 0).  All threads call this
+// with l.survivors = 0; barriers are inside, and one at the end.
+template <int TH, typename Get>
+__device__ __forceinline__ void best_of(Lists<TH>& l, int n, Get get, u64* out, int top, int tid) {
+  const int lane = tid & 31;
+  for (int i0 = 0; i0 < n; i0 += TH) {
+    const u64 e = i0 + tid < n ? get(i0 + tid) : 0;
+    const uint32_t kept = __ballot_sync(~0u, e != 0);
+    if (!kept) continue;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&l.survivors, __popc(kept));
+    at = __shfl_sync(~0u, at, 0);
+    if (e) l.merged[at + __popc(kept & ((1u << lane) - 1u))] = e;
   }
   if (tid < top) out[tid] = 0;
   __syncthreads();
-  const int n = l.survivors;
-  for (int i = tid; i < n; i += TH) {
-    const u64 e = l.merged[i];
+  const int m = l.survivors;
+  // four lanes an entry, each against a quarter of the others
+  for (int i0 = tid / 32 * 8; i0 < m; i0 += TH / 4) {
+    const int i = i0 + lane / 4;
+    const u64 e = i < m ? l.merged[i] : 0;
     int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) rank += l.merged[j] > e;
-    if (rank < top) out[rank] = e;
+#pragma unroll 4
+    for (int j = lane & 3; j < m; j += 4) rank += l.merged[j] > e;
+    rank += __shfl_xor_sync(~0u, rank, 1);
+    rank += __shfl_xor_sync(~0u, rank, 2);
+    if (e && !(lane & 3) && rank < top) out[rank] = e;
   }
   __syncthreads();
 }
@@ -512,21 +508,30 @@ __global__ void __launch_bounds__(TH, ON_SM / TH) logprobs_fwd_kernel(const T* _
     if (in_group >= 2) group = max(group, __shfl_xor_sync(~0u, group, 1));
     if (in_group >= 4) group = max(group, __shfl_xor_sync(~0u, group, 2));
     __syncthreads();       // (the copies have been read: the lists take their place)
+    group = (group & 0xffff0000u) | (TH - tid / in_group);
     if (tid % in_group == 0) l.maxima[tid / in_group] = group;
     if (tid == 0) l.survivors = l.queued = 0;
     __syncthreads();
-    const uint32_t reached = top <= 32 ? top_of_maxima<2>(l.maxima, lane, top) : top_of_maxima<4>(l.maxima, lane, top);
-    const u64 thr = reached ? (static_cast<u64>(reached) << 32) - 1 : 0;   // (every entry of that value is above it)
-    if (tid == 0) l.threshold = thr;
-    if (highest >= reached)
-      for (int c = tid; c < cell; c += TH)
-        if (cells[c] >= reached >> 16) l.queue[atomicAdd(&l.queued, 1)] = static_cast<uint16_t>(c);
+    if (top <= 32) set_threshold<64>(l, group, tid, top);
+    else set_threshold<128>(l, group, tid, top);
+    __syncthreads();
+    const u64 thr = l.threshold;
+    const uint32_t reached = static_cast<uint32_t>(thr >> 32);
+    if (__any_sync(~0u, highest >= reached))
+      for (int c = tid; c < cell; c += TH) {      // (every thread has as many cells)
+        const bool take = cells[c] >= reached >> 16;
+        const uint32_t kept = __ballot_sync(~0u, take);
+        int at = 0;
+        if (lane == 0 && kept) at = atomicAdd(&l.queued, __popc(kept));
+        at = __shfl_sync(~0u, at, 0) + __popc(kept & ((1u << lane) - 1u));
+        if (take) l.queue[at] = static_cast<uint16_t>(c);
+      }
     __syncthreads();
     int listed = 0;
     if (warp == 0) {   // the ragged ends: at most 14 values
       const u64 e = has_edge ? entry_of(edge_v, edge_at) : 0;
-      const uint32_t kept = __ballot_sync(~0u, e > thr);
-      if (e > thr) l.entry[0][__popc(kept & ((1u << lane) - 1u))] = e;
+      const uint32_t kept = __ballot_sync(~0u, has_edge && e >= thr);
+      if (kept >> lane & 1) l.entry[0][__popc(kept & ((1u << lane) - 1u))] = e;
       listed = __popc(kept);
     }
     const int of_cell = part * U, items = l.queued * of_cell;   // vectors (at most the block's and the ends of its cells)
@@ -546,7 +551,12 @@ __global__ void __launch_bounds__(TH, ON_SM / TH) logprobs_fwd_kernel(const T* _
       for (int u = 0; u < 2; ++u) listed = offer<T, TH>(l, v[u], valid[u], j0[u], listed, warp, lane, top);
     }
     if (lane == 0) l.count[warp] = listed;
-    block_best(l, best, top, tid);
+    __syncthreads();
+    const u64 least = l.threshold;       // (the entry that set it is among the best)
+    best_of(l, WARPS * CAP, [&](int i) {
+      const u64 e = i % CAP < l.count[i / CAP] ? l.entry[i / CAP][i % CAP] : 0;
+      return e >= least ? e : 0;
+    }, best, top, tid);
   } else {
     __syncthreads();
   }
@@ -561,6 +571,7 @@ __global__ void __launch_bounds__(TH, ON_SM / TH) logprobs_fwd_kernel(const T* _
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a.t) : "memory");
       }
     }
+    if (TOP && tid == 0) l.survivors = 0;
     if (TOP && tid < top)
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_block(&block_best_of[block * top + tid], 0)), "l"(best[tid])
                    : "memory");
@@ -568,24 +579,14 @@ __global__ void __launch_bounds__(TH, ON_SM / TH) logprobs_fwd_kernel(const T* _
     cluster_wait();
     if (block) return;
     if (TOP) {
-      const int n = blocks * top;
-      for (int i = tid; i < n; i += TH) {
-        // its place in its own list, and what is greater in the others (each is sorted, best first)
+      // every list holds `share` entries of at least the lowest of their share-th ones: together at least `top`
+      const int share = (top + blocks - 1) / blocks;
+      u64 least = ~0ull;
+      for (int b = 0; b < blocks; ++b) least = min(least, block_best_of[b * top + share - 1]);
+      best_of(l, blocks * top, [&](int i) {
         const u64 e = block_best_of[i];
-        int rank = i % top;
-        for (int b = 0; b < blocks && rank < top; ++b) {
-          if (b == i / top) continue;
-          const u64* list = block_best_of + b * top;
-          int lo = 0, hi = top;
-          while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (list[mid] > e) lo = mid + 1; else hi = mid;
-          }
-          rank += lo;
-        }
-        if (e && rank < top) best[rank] = e;
-      }
-      __syncthreads();
+        return e >= least ? e : 0;
+      }, best, top, tid);
     }
   }
   if (warp < (TOP ? (top + 31) / 32 : 1)) {
