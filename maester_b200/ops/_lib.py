@@ -163,6 +163,8 @@ def _declare(l: ctypes.CDLL) -> None:
         "mb_logprobs_fwd": [_P, _P, _I, _I, _I, _L, _F, _P, _P, _I, _P, _P, _P, _P],
         "mb_logprobs_bwd": [_P, _P, _I, _I, _I, _L, _F, _P, _P, _P, _I, _P, _P, _P, _I, _L, _P],
         "mb_fp8_quantize": [_P, _I, _I, _I, _L, _I, _P, _P, _P, _P, _P],
+        "mb_fp8_linear_fwd": [_P, _I, _L, _P, _I, _L, _I, _I, _I, _P, _P, _P, _P, _P],
+        "mb_fp8_linear_bwd": [_P, _I, _L, _I, _I, _I, _P, _P, _P, _P, _P, _L, _I, _P],
         "mb_fp8_linear": [_P, _I, _L, _I, _I, _P, _P, _P, _I, _L, _P, _L, _P],
         "mb_fp8_gemm": [_P, _P, _P, _P, _P, _I, _I, _I, _L, _L, _L, _I, _P],
         "mb_peer_copy": [_P, _P, _L, _P],

@@ -798,30 +798,42 @@ def _fp8_bytes(rows: int, blocks: int) -> int:
     return rows * blocks * 128 + (rows + 127) // 128 * ((blocks + 3) // 4) * 512
 
 
-def fp8_quantize_packed(x: torch.Tensor, rows: bool = True, cols: bool = False, square: bool = False):
-    """As ``fp8_quantize``, with codes and exponents of an orientation in one uint8 buffer (or None)."""
-    R, C = x.shape
-    rb, cb = (R + 127) // 128, (C + 127) // 128
-    q = torch.empty(_fp8_bytes(R, cb), device=x.device, dtype=torch.uint8) if rows else None
-    qt = torch.empty(_fp8_bytes(C, rb), device=x.device, dtype=torch.uint8) if cols else None
-    p, pt = (q.data_ptr() if rows else 0), (qt.data_ptr() if cols else 0)
+def fp8_linear_fwd(x: torch.Tensor, w: torch.Tensor, keep_x: bool, keep_w: bool):
+    """(``Q(x) @ Q(w).T``, packed codes of ``x.T`` | None, of ``w.T`` | None) of [M, K] and [N, K] with unit column stride."""
+    (M, K), (N, Kw) = x.shape, w.shape
+    assert K == Kw and x.device == w.device
+    kb, dev, u8, empty = (K + 127) // 128, x.device, torch.uint8, torch.empty
+    work = empty(_fp8_bytes(M, kb) + _fp8_bytes(N, kb), device=dev, dtype=u8)
+    x_t = empty(_fp8_bytes(K, (M + 127) // 128), device=dev, dtype=u8) if keep_x else None
+    w_t = empty(_fp8_bytes(K, (N + 127) // 128), device=dev, dtype=u8) if keep_w else None
+    y = empty(M, N, device=dev, dtype=x.dtype)
     with on_device(x):
-        _ck(_lib.lib().mb_fp8_quantize(x.data_ptr(), _LOGITS_TYPE[x.dtype], R, C, x.stride(0),
-                                       FP8_ROWS * rows + FP8_COLS * cols + FP8_SQUARE * square, p, p + R * cb * 128,
-                                       pt, pt + C * rb * 128, _stream_of(x)), "fp8_quantize")
-    return q, qt
+        _ck(_lib.lib().mb_fp8_linear_fwd(x.data_ptr(), _LOGITS_TYPE[x.dtype], x.stride(0), w.data_ptr(), _LOGITS_TYPE[w.dtype],
+                                         w.stride(0), M, K, N, work.data_ptr(), _ptr(x_t), _ptr(w_t), y.data_ptr(), _stream_of(x)),
+            "fp8_linear_fwd")
+    return y, x_t, w_t
 
 
-def fp8_gemm_packed(a: torch.Tensor, b: torch.Tensor, blocks: int, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
-    """``out (+)= A @ B.T`` of packed buffers with ``blocks`` blocks of the contraction."""
-    M, N = out.shape
-    Kp = blocks * 128
-    assert a.numel() == _fp8_bytes(M, blocks) and b.numel() == _fp8_bytes(N, blocks) and (out.stride(1) == 1 or N == 1)
-    pa, pb = a.data_ptr(), b.data_ptr()
-    with on_device(out):
-        _ck(_lib.lib().mb_fp8_gemm(pa, pa + M * Kp, pb, pb + N * Kp, out.data_ptr(), M, N, blocks, Kp, Kp, out.stride(0),
-                                   FP8_OUT_F32_ACC if accumulate else FP8_OUT[out.dtype], _stream_of(out)), "fp8_gemm")
-    return out
+def fp8_linear_bwd(dy: torch.Tensor, K: int, x_t: torch.Tensor | None, w_t: torch.Tensor | None, dw: torch.Tensor | None,
+                   accumulate: bool):
+    """dx [M, K] | None (with ``w_t``) of ``dy`` [M, N]; with ``x_t`` the weight's gradient goes into ``dw`` (or is added to it,
+    fp32 then)."""
+    M, N = dy.shape
+    nb, mb = (N + 127) // 128, (M + 127) // 128
+    work = torch.empty((0 if w_t is None else _fp8_bytes(M, nb)) + (0 if x_t is None else _fp8_bytes(N, mb)), device=dy.device,
+                       dtype=torch.uint8)
+    dx, ld, out = None, 0, 0
+    if w_t is not None:
+        assert w_t.numel() == _fp8_bytes(K, nb)
+        dx = torch.empty(M, K, device=dy.device, dtype=dy.dtype)
+    if x_t is not None:
+        assert x_t.numel() == _fp8_bytes(K, mb) and dw.shape == (N, K) and (dw.stride(1) == 1 or K == 1) and dw.device == dy.device
+        assert not accumulate or dw.dtype == torch.float32
+        ld, out = dw.stride(0), FP8_OUT_F32_ACC if accumulate else FP8_OUT[dw.dtype]
+    with on_device(dy):
+        _ck(_lib.lib().mb_fp8_linear_bwd(dy.data_ptr(), _LOGITS_TYPE[dy.dtype], dy.stride(0), M, K, N, work.data_ptr(), _ptr(w_t),
+                                         _ptr(x_t), _ptr(dx), _ptr(dw), ld, out, _stream_of(dy)), "fp8_linear_bwd")
+    return dx
 
 
 FP8_FEW = 8     # tokens that take the kernel for a decoding step

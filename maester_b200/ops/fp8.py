@@ -66,19 +66,27 @@ class Fp8Blocks:
         return ref.fp8_dequantize(self.data, self.exponents())[:, :self.cols].to(dtype)
 
 
-def _quantize(x: torch.Tensor, rows: bool = True, cols: bool = False, square: bool = False):
-    """(x | None, x.T | None) quantised, as ``_product`` takes them, from a matrix with unit column stride: on the GPU one
-    buffer of codes and exponents each."""
+def _quantized(x: torch.Tensor, square: bool = False) -> torch.Tensor:
+    """On the CPU: what the codes of a matrix (blocks along its rows) stand for."""
+    return ref.fp8_dequantize(*ref.fp8_quantize(x, square))[:, :x.shape[1]]
+
+
+def _forward(x: torch.Tensor, w: torch.Tensor, keep_x: bool, keep_w: bool):
+    """(y, x^T | None, w^T | None) with the transposes in the form that ``_backward`` takes."""
     if x.is_cuda:
-        return _C().fp8_quantize_packed(x, rows, cols, square)
-    return tuple(ref.fp8_dequantize(*ref.fp8_quantize(t, square))[:, :t.shape[1]] if want else None for want, t in ((rows, x), (cols, x.T)))
+        return _C().fp8_linear_fwd(x, w, keep_x, keep_w)
+    y = (_quantized(x) @ _quantized(w, True).T).to(x.dtype)
+    return y, _quantized(x.T) if keep_x else None, _quantized(w.T, True) if keep_w else None
 
 
-def _product(a, b, K: int, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
-    """``out (+)= A @ B.T`` of two results of ``_quantize`` over a contraction of K values."""
-    if out.is_cuda:
-        return _C().fp8_gemm_packed(a, b, (K + 127) // 128, out, accumulate)
-    return out.add_(a @ b.T) if accumulate else out.copy_(a @ b.T)
+def _backward(dy: torch.Tensor, K: int, x_t, w_t, dw: torch.Tensor | None, accumulate: bool) -> torch.Tensor | None:
+    """dx | None; the weight's gradient goes into ``dw``."""
+    if dy.is_cuda:
+        return _C().fp8_linear_bwd(dy, K, x_t, w_t, dw, accumulate)
+    if x_t is not None:
+        value = _quantized(dy.T) @ x_t.T
+        dw.add_(value) if accumulate else dw.copy_(value)
+    return None if w_t is None else (_quantized(dy) @ w_t.T).to(dy.dtype)
 
 
 def _as_matrix(x: torch.Tensor) -> torch.Tensor:
@@ -136,32 +144,21 @@ class _LinearFp8(Function):
         need_x, need_w = ctx.needs_input_grad
         x2 = _as_matrix(x)
         w2 = w if w.stride(1) == 1 or w.shape[1] == 1 else w.contiguous()
-        xq, xt = _quantize(x2, True, need_w)
-        wq, wt = _quantize(w2, True, need_x, True)
+        y, xt, wt = _forward(x2, w2, need_w, need_x)
         ctx.save_for_backward(w, xt, wt)
-        ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
-        y = torch.empty(x2.shape[0], w.shape[0], device=x.device, dtype=x.dtype)
-        return _product(xq, wq, w.shape[1], y).view(*x.shape[:-1], w.shape[0])
+        ctx.x_shape = x.shape
+        return y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         w, xt, wt = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad
-        dy2 = _as_matrix(dy)
-        T, N = dy2.shape
-        dyq, dyt = _quantize(dy2, need_x, need_w)
-        dx = dw = None
-        if need_x:
-            dx = torch.empty(T, ctx.x_shape[-1], device=dy.device, dtype=ctx.x_dtype)
-            dx = _product(dyq, wt, N, dx).view(ctx.x_shape)
-        if need_w:
+        dw = mg = None
+        if xt is not None:
             mg = getattr(w, "main_grad", None)
-            if mg is not None:
-                _product(dyt, xt, T, mg, True)
-            else:
-                dw = _product(dyt, xt, T, torch.empty(w.shape, device=w.device, dtype=w.dtype))
-        return dx, dw
+            dw = torch.empty(w.shape, device=w.device, dtype=w.dtype) if mg is None else mg
+        dx = _backward(_as_matrix(dy), w.shape[1], xt, wt, dw, mg is not None)
+        return None if dx is None else dx.view(ctx.x_shape), None if mg is not None else dw
 
 
 def linear_fp8(x: torch.Tensor, w: torch.Tensor | Fp8Blocks) -> torch.Tensor:
@@ -190,8 +187,7 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor | Fp8Blocks) -> torch.Tensor:
         return _LinearFp8.apply(x, w)
     x2 = _as_matrix(x)
     if not held:
-        wq = _quantize(w if w.stride(1) == 1 or K == 1 else w.contiguous(), square=True)[0]
-        y = _product(_quantize(x2)[0], wq, K, torch.empty(x2.shape[0], N, device=x.device, dtype=x.dtype))
+        y = _forward(x2, w if w.stride(1) == 1 or K == 1 else w.contiguous(), False, False)[0]
     elif x.is_cuda:
         y = _C().fp8_linear(x2, w.data, w.scales)
     else:
