@@ -150,17 +150,19 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 
 // Running maximum m of x, sum s of 2^z and sum t of z 2^z with z = k x - base(m), k = scale log2(e).  base(m) is k m as rounded:
-// one fused operation gives z, and the difference to k m is taken out of log s at the end.  Where k m could overflow
-// (logits of 1e30 and more, such as the lowest finite value as a mask) z = k (x - m), the base is k m itself.
+// one fused operation gives z, and the difference to k m (at most 2) is taken out of log s at the end.  Where |k m| is 2^26 or
+// more, or overflows (rows of the lowest finite value as a mask), z = k (x - m): the base is k m itself.
 struct Sums {
   float m, s, t;
 };
-constexpr float HUGE_LOGIT = 1e30f, ZFAR = -1500.f;      // 2^-1500 is 0
-__device__ __forceinline__ bool plain(float m) { return fabsf(m) < HUGE_LOGIT; }
+constexpr float ZFAR = -1500.f;      // 2^-1500 is 0
 __device__ __forceinline__ float base(float m, float k) { return __fmul_rn(m, k); }   // (never contracted: it is one number)
+__device__ __forceinline__ bool plain(float m, float k) { return fabsf(base(m, k)) < 67108864.f; }
+__device__ __forceinline__ float lost(float m, float k) { return plain(m, k) ? fmaf(m, k, -base(m, k)) : 0.f; }
 // base(from) - base(to), at least ZFAR; `from` <= `to`, `to` finite or +inf, `from` may be -inf
 __device__ __forceinline__ float base_step(float from, float to, float k) {
-  const float d = plain(from) && plain(to) ? __fsub_rn(base(from, k), base(to, k)) : (from - to) * k;
+  const float d = plain(from, k) && plain(to, k) ? __fsub_rn(base(from, k), base(to, k))
+                                                 : (from - to) * k + (lost(to, k) - lost(from, k));
   return fmaxf(d, ZFAR);
 }
 // the sums of `a` on the base of m >= a.m.  (t + s d: every old z moves by d.)
@@ -199,7 +201,7 @@ __device__ __forceinline__ void add_values(Sums& a, const Vec<T> (&v)[U], float 
   const float m = a.m, low = m - fmaxf(far, 0.02f * fabsf(m));
   float2 s = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
   const float2 k2 = make_float2(k, k);
-  if (plain(m) && (!ENT || (Vec<T>::PACKED && low >= Vec<T>::LOWEST))) {
+  if (plain(m, k) && (!ENT || (Vec<T>::PACKED && low >= Vec<T>::LOWEST))) {
     const uint32_t low2 = Vec<T>::both(low);
     const float2 nb = make_float2(-base(m, k), -base(m, k));
 #pragma unroll
@@ -212,7 +214,7 @@ __device__ __forceinline__ void add_values(Sums& a, const Vec<T> (&v)[U], float 
         if (ENT) t = fma2(e, z, t);
       }
   } else {
-    const bool p = plain(m);
+    const bool p = plain(m, k);
     const float2 nm = p ? make_float2(0.f, 0.f) : make_float2(-m, -m), nb = p ? make_float2(-base(m, k), -base(m, k)) : make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -456,7 +458,7 @@ __global__ void __launch_bounds__(TH, ON_SM / TH) logprobs_fwd_kernel(const T* _
       const float v = edge_v = to_f(q.row[edge_at]);
       if (v != -INFINITY) {
         a.m = v == v ? v : 0.f;
-        const float z = plain(a.m) ? fmaf(v, k, -base(a.m, k)) : (v - a.m) * k, e = ex2(z);
+        const float z = plain(a.m, k) ? fmaf(v, k, -base(a.m, k)) : (v - a.m) * k, e = ex2(z);
         a.s = e;
         a.t = e * z;
       }
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(TH, ON_SM / TH) logprobs_fwd_kernel(const T* _
     else if (at < blocks) part = block_parts[at];
     a = merge_lanes<WARPS>(part, k);
     // (log s on the base of m: what k m lost in its rounding is taken out)
-    const float log_s = logf(a.s) - (plain(a.m) ? fmaf(a.m, k, -base(a.m, k)) * LN2 : 0.f);
+    const float log_s = logf(a.s) - lost(a.m, k) * LN2;
     if (tid == 0) {
       const float mean = a.t / a.s, h = logf(a.s) - mean * LN2;     // mean: of z under p
       if (p.tokens) p.logprob[row] = (at_token - a.m) * scale - log_s;
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(TH, ON_SM / TH) logprobs_fwd_kernel(const T* _
 // rows of x and dx do not share their 16-byte boundaries it goes value by value, neighbours in neighbouring lanes.
 // With z and s as above p = 2^z / s and log p + H = (z - mean z) ln 2: neither needs a logarithm.
 struct RowGrad {
-  float m, k, nb, mean, c0, c1, hot;      // z = k (x - m) + nb, with m = 0 and nb = -base where that does not overflow
+  float m, k, nb, mean, c0, c1, hot;      // z = k (x - m) + nb, with m = 0 and nb = -base where the base is small enough
   // 2^z (c0 + c1 (z - mean)): both carry -scale / s, c1 the entropy's part
   template <bool ENT>
   __device__ __forceinline__ float at(float x) const {
@@ -664,7 +666,7 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
   float all = gl;
   for (int a = 0; a < top; ++a) all += g_top[row * top + a];
   const float k = scale * LOG2E, per_s = -scale * r.y;
-  const bool p = plain(r.x);
+  const bool p = plain(r.x, k);
   const RowGrad f{p ? 0.f : r.x, k, p ? -base(r.x, k) : 0.f, r.z, per_s * all, per_s * ge * LN2, gl * scale};
   auto one = [&](int j) { return f.at<ENT>(to_f(xr[j])) + (j == tok ? f.hot : 0.f); };
   for (int i0 = v0; i0 < v1; i0 += THREADS * U) {

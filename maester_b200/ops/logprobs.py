@@ -28,8 +28,8 @@ class TokenLogprobs(NamedTuple):
 
 
 def _check(tokens, lead, device, V, scale, entropy, top) -> None:
-    if not (isinstance(scale, (int, float)) and math.isfinite(scale) and scale > 0):
-        raise ValueError(f"the logit scale has to be a positive number, got {scale!r}")
+    if not (isinstance(scale, (int, float)) and 1e-8 <= scale <= 1e8):   # (logits up to 1e30 times it are fp32 numbers)
+        raise ValueError(f"the logit scale has to be a number in [1e-8, 1e8], got {scale!r}")
     if not (isinstance(top, int) and 0 <= top <= min(MAX_TOP, V)):
         raise ValueError(f"top has to be a whole number in [0, {min(MAX_TOP, V)}], got {top!r}")
     if tokens is None:
@@ -78,8 +78,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
 
     All results are fp32 whatever the type of the logits (bf16, fp16, fp32; rows may have any pitch).  A row whose token is
     -100 is skipped: log-probability and entropy 0, alternatives -inf with id -1, no gradient.  A -inf logit (or one whose
-    distance from the row's maximum is beyond fp32) has probability 0; a row without a finite logit, or with NaN or +inf, has no distribution: its numbers are NaN, its alternatives are
-    still in order (NaN above +inf).  A token id outside [0, V) gives NaN and a device status error
+    distance from the row's maximum is beyond fp32) has probability 0; a row without a finite logit, or with NaN or +inf, has
+    no distribution: its numbers are NaN, its alternatives are still in order (NaN above +inf).  A token id outside [0, V) gives NaN and a device status error
     (``ops.cuda.check_status``); on the CPU it raises.  Gradients flow to the logits from log-probabilities, entropies and
     the alternatives' log-probabilities.  The first call on a device has to run outside a stream capture."""
     if logits.dim() < 1 or not logits.is_floating_point():

@@ -121,6 +121,50 @@ def test_rows_that_share_an_sm(rows, V, dtype):
         _check_fwd(ops.token_logprobs(x, tokens, scale=0.9, entropy=True, top=top), x, tokens, 0.9, top)
 
 
+@pytest.mark.parametrize("scale,size", [(1e8, 1e-7), (1e8, 9e29), (1e-8, 1e9), (1.0, 9e29), (1.0, 3e38)])
+def test_scales_and_sizes_at_the_ends(scale, size):
+    """The largest logits times the largest scale, up to the ends of fp32: small distances, or one value that has it all."""
+    x = torch.linspace(-1, 1, 2000, device="cuda")[None].repeat(2, 1) * size
+    x[1] = x[1].flip(0)
+    tokens = torch.tensor([1999, 3], device="cuda")
+    got = ops.token_logprobs(x, tokens, scale=scale, entropy=True, top=4)
+    z = x.double() * scale
+    logp = torch.log_softmax(z - z.amax(1, keepdim=True), 1)
+    want = logp.gather(1, tokens[:, None])[:, 0]
+    far = want < -3e38      # beyond fp32
+    assert (got.logprobs[far] == -math.inf).all()
+    assert ((got.logprobs.double() - want).abs() <= _err(2000) + 4 * want.abs() * U)[~far].all()
+    ent = -(logp.exp() * logp).nan_to_num(0.0).sum(1)
+    assert ((got.entropy.double() - ent).abs() <= _err(2000) * (2 + math.log(2000))).all()
+    assert torch.equal(got.top_tokens, _order(x, 4))
+
+
+@pytest.mark.parametrize("scale,size", [(0.1, 2.0 ** 27), (0.1, 2.0 ** 29), (0.1, 2.0 ** 30), (0.05, -2.0 ** 30), (1e-3, 2.0 ** 36),
+                                        (1.0, 2.0 ** 25), (1.0, -2.0 ** 26), (1.0, 2.0 ** 40)])
+def test_close_logits_far_from_zero(scale, size):
+    """Neighbouring fp32 numbers around `size`, the largest ones last or first: what a product with the scale rounds away is
+    larger than their distances.  The gradient's tolerance is that of ``test_gradient``'s probabilities."""
+    V = 4000
+    step = abs(size) * 2.0 ** -23
+    x = (size + (torch.arange(V, device="cuda", dtype=torch.float64) // 571) * step).float()[None].repeat(2, 1)
+    x[:, 100:2000] = size / 4 if size > 0 else size * 4
+    x[1] = x[1].flip(0)
+    x.requires_grad_()
+    tokens = torch.tensor([V - 1, 1], device="cuda")
+    got = ops.token_logprobs(x, tokens, scale=scale, entropy=True, top=10)
+    with torch.no_grad():
+        _check_fwd(got, x, tokens, scale, 10)
+        logp, h = _exact(x, tokens, scale)
+    dx, = torch.autograd.grad(got.logprobs.sum() + got.entropy.sum(), x)
+    p = logp.exp()
+    one = (torch.arange(V, device="cuda")[None] == tokens[:, None]).double()
+    lp = torch.where(p > 0, logp, 0.0)
+    want = scale * (one - p - p * (lp + h[:, None]))
+    # (a probability below 2^-126, e^-87, is no normal fp32 number and may be taken for 0: here they go down to e^-91)
+    room = p * (2 + lp.abs() + h[:, None]) + one
+    assert ((dx.double() - want).abs() <= 4 * scale * (_err(V) + 3 * lp.abs() * U) * room + scale * room * (p < 2.0 ** -126)).all()
+
+
 def test_rows_without_a_distribution():
     x = torch.zeros(5, 3000, device="cuda")
     x[0] = -math.inf

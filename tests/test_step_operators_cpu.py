@@ -59,6 +59,12 @@ def test_logprobs_refusals(kw, error):
         ops.linear_logprobs(torch.randn(4, 6), torch.randn(8, 6), **kw)
 
 
+@pytest.mark.parametrize("scale", [1e-9, 1e9, math.inf, 10 ** 400, "1", None])
+def test_logprobs_refuse_a_scale_that_fp32_cannot_carry(scale):
+    with pytest.raises(ValueError, match="scale"):
+        ops.token_logprobs(torch.randn(2, 8), entropy=True, scale=scale)
+
+
 def test_logprobs_refuse_more_alternatives_than_the_limit():
     with pytest.raises(ValueError, match="64"):
         ops.token_logprobs(torch.randn(2, 100), top=65)
