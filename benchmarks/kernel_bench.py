@@ -2,7 +2,8 @@
 
 ``op``: ``gemm`` (forward / dgrad / wgrad layouts of the Gemma-3 4B projections, 1-CTA and CTA-pair
 kernels next to ``torch.matmul``), ``attention`` (forward and backward for head sizes 256 and 128,
-causal and sliding-window), ``elementwise`` (RMSNorm, GeGLU, AdamW), ``grouped`` (MoE grouped GEMM).
+causal and sliding-window), ``elementwise`` (RMSNorm, GeGLU, AdamW), ``grouped`` (MoE grouped GEMM), ``logprobs`` (token
+log-probabilities, alternatives, gradient), ``fp8`` (quantisation, product, few tokens), ``adamw8`` (AdamW over many tensors).
 Timing is by CUDA events after warm-up; every iteration's operands exceed the L2 capacity.
 ``--small`` runs one launch per kernel on a case of a few hundred MB, the size meant for a
 profiler capture.  Fractions are of the peaks in ``MEASURED_PEAKS.json`` at the repository root
@@ -234,15 +235,87 @@ def bench_ce(iters: int, small: bool) -> None:
     C.check_status()
 
 
+def bench_logprobs(iters: int, small: bool) -> None:
+    """Token log-probabilities, entropies and alternatives, and the gradient: one read, or one read and one write, of the logits."""
+    _, bw_peak = _peaks()
+    shapes = [(4096, 32000)] if small else [(16, 262144), (4096, 128256), (8192, 32000)]
+    warm = 0 if small else 3
+    for R, V in shapes:
+        x = (torch.randn(R, V, device="cuda") * 2).bfloat16()
+        tokens = torch.randint(0, V, (R,), device="cuda")
+        nb = 2 * R * V
+        for ent, top in ((False, 0), (True, 0), (True, 5), (True, 20), (True, 64)):
+            t = timeit(lambda: C.logprobs_fwd(x, tokens, 1.0, ent, top, False), iters, warm)
+            print(f"logprobs [{R} x {V}] entropy {int(ent)} alternatives {top:2d}: {t * 1e3:.1f} us {nb / t / 1e6:.0f} GB/s "
+                  f"({nb / t / 1e6 / bw_peak:.2f} of measured)")
+        st = C.logprobs_fwd(x, tokens, 1.0, True, 0, True)[4]
+        g = torch.randn(R, device="cuda")
+        t = timeit(lambda: C.logprobs_bwd(x, tokens, 1.0, st, g, g, None, None), iters, warm)
+        print(f"logprobs [{R} x {V}] gradient with entropy: {t * 1e3:.1f} us {2 * nb / t / 1e6:.0f} GB/s "
+              f"({2 * nb / t / 1e6 / bw_peak:.2f} of measured)")
+    C.check_status()
+
+
+def bench_fp8(iters: int, small: bool) -> None:
+    """Block-scaled 8-bit linear layers: the quantisation passes, the product, and a few tokens against a laid-out weight."""
+    from maester_b200 import ops
+    tf_peak, bw_peak = _peaks()
+    warm = 0 if small else 3
+    M, K = (8192, 4096) if small else (16384, 4096)
+    x = torch.randn(M, K, device="cuda", dtype=torch.bfloat16)
+    for name, mode, out in (("rows", (True, False, False), 1), ("rows and columns", (True, True, False), 2),
+                            ("tiles, both", (True, True, True), 2)):
+        t = timeit(lambda: C.fp8_quantize(x, *mode), iters, warm)
+        nb = M * K * (2 + out)
+        print(f"fp8 quantise {name:17s} [{M} x {K}]: {t * 1e3:.1f} us {nb / t / 1e6:.0f} GB/s ({nb / t / 1e6 / bw_peak:.2f} of measured)")
+    for M, N, K in [(8192, 4096, 4096)] if small else [(16384, 4096, 4096), (16384, 20480, 2560), (16384, 2560, 10240)]:
+        a = ops.quantize_fp8(torch.randn(M, K, device="cuda", dtype=torch.bfloat16))
+        b = ops.quantize_fp8(torch.randn(N, K, device="cuda", dtype=torch.bfloat16) * 0.02, square=True)
+        out = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+        t = timeit(lambda: C.fp8_gemm(a.data, a.scales, b.data, b.scales, out), iters, warm)
+        fl = 2 * M * N * K
+        print(f"fp8 product [{M} x {N} x {K}]: {t:.3f} ms {fl / t / 1e9:6.0f} TF ({fl / t / 1e9 / tf_peak:.2f} of measured bf16)")
+    N, K = 14336, 4096
+    weights = [ops.quantize_fp8(torch.randn(N, K, device="cuda", dtype=torch.bfloat16), square=True) for _ in range(1 if small else 8)]
+    for M in (1, 4, 8, 16, 64):
+        x = torch.randn(M, K, device="cuda", dtype=torch.bfloat16)
+        t = timeit(lambda: [C.fp8_linear(x, w.data, w.scales) for w in weights], iters, warm) / len(weights)
+        print(f"fp8 {M:2d} tokens x [{N} x {K}], quantised in the call: {t * 1e3:.1f} us {N * K / t / 1e6:.0f} GB/s "
+              f"({N * K / t / 1e6 / bw_peak:.2f} of measured)")
+    C.check_status()
+
+
+def bench_adamw8(iters: int, small: bool) -> None:
+    """AdamW over many tensors, states in 8 and in 32 bits."""
+    from maester_b200.optimizers import AdamWMulti
+    _, bw_peak = _peaks()
+    n = 4 if small else 24
+    for dtype, copy in ((torch.float32, True), (torch.bfloat16, False)):
+        for bits in (8, 32):
+            params = [torch.nn.Parameter(torch.randn(4096, 4096, device="cuda").to(dtype)) for _ in range(n)]
+            for p in params:
+                p.grad = torch.randn_like(p)
+            opt = AdamWMulti(params, lr=1e-3, state_bits=bits)
+            if copy:
+                opt.attach_copies({p: torch.empty_like(p, dtype=torch.bfloat16) for p in params})
+            t = timeit(opt.step, iters, 0 if small else 3)
+            per = 3 * params[0].element_size() + 2 * copy + (4 * 257 / 256 if bits == 8 else 16)
+            nb = per * sum(p.numel() for p in params)
+            print(f"AdamW {n} x [4096 x 4096] {dtype} states {bits:2d} bits copy {int(copy)}: {t * 1e3:.1f} us {nb / t / 1e6:.0f} GB/s "
+                  f"({nb / t / 1e6 / bw_peak:.2f} of measured)")
+            del opt, params
+    C.check_status()
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("op", choices=["gemm", "attention", "elementwise", "grouped", "moe", "ce", "all"])
+    ap.add_argument("op", choices=["gemm", "attention", "elementwise", "grouped", "moe", "ce", "logprobs", "fp8", "adamw8", "all"])
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--small", action="store_true", help="one cold launch per kernel on a small case")
     a = ap.parse_args()
     iters = 1 if a.small else a.iters
     table = {"gemm": bench_gemm, "attention": bench_attention, "elementwise": bench_elementwise, "grouped": bench_grouped,
-             "moe": bench_moe, "ce": bench_ce}
+             "moe": bench_moe, "ce": bench_ce, "logprobs": bench_logprobs, "fp8": bench_fp8, "adamw8": bench_adamw8}
     for name, fn in table.items():
         if a.op in (name, "all"):
             fn(iters, a.small)
