@@ -9,6 +9,11 @@
 // tile as one block), of its transpose (blocks along a column), or of both.  A thread holds 8 x 8 values: maxima along rows
 // meet within 16 lanes, maxima along columns through shared memory, and the transposed codes go through a swizzled 16 KiB
 // tile so that both outputs leave as whole 128-byte lines.
+//
+// Measured (16384 x 4096 bf16): codes of x 38 us (5290 GB/s of 6540), of x and its transpose 56 us (4760), with one scale a tile
+// 49 us (5450).  The integer pipe is busy 65 to 75 % of the time (packed maxima, shifts of 16-bit values into fp32, packing of
+// codes), and only 4 blocks an SM fit its registers, so neither it nor memory is full; at 6 MB (5003 x 2560, 800 blocks on 592
+// places) the second wave costs as much as the first: 15 us.
 #include "fp8_common.cuh"
 #include "host_common.cuh"
 

@@ -2,10 +2,16 @@
 // tokens: a decoding step, bound by reading the weight's codes once (14336 x 4096: 9 us at the copy rate).
 //
 // Everything else is kept off their way: no staging, no tensor memory, no barrier but one at the end.  A warp takes 32 rows of w
-// and every 4th, 8th or 16th block of the contraction (as many warps share them), with the next block on its way.  The matrix instruction (16 x 8 x 32) does not care
-// in which order the contraction comes, as long as both operands agree: the 16 neighbouring bytes that a lane reads are its
-// values of two instructions, of w and of x alike, so neither operand is ever rearranged.  The warps' sums meet in shared memory
-// and are added in order.
+// and every 4th, 8th or 16th block of the contraction (as many warps share them), with the next block on its way.  The matrix
+// instruction (16 x 8 x 32) does not care in which order the contraction comes, as long as both operands agree: the 16
+// neighbouring bytes that a lane reads are its values of two instructions, of w and of x alike, so neither operand is ever
+// rearranged.  The warps' sums meet in shared memory and are added in order.
+//
+// Measured with the quantiser, launches from a graph over 400 MB of weights: 4 tokens x 14336 x 4096 15.5 us (a kernel that only
+// reads the codes: 10.7), 1 x 4096 x 4096 7.3 us, 1 x 2560 x 10240 10.5 us; the tcgen05 kernel for few rows of fp8_gemm.cu took
+// 19.5, 11.1 and 22.6: at this size a contraction's depth is too short for its pipeline to fill.  Above eight tokens a second
+// set of columns would double the instructions, and that kernel takes over (16 tokens: 23 us).  Called from the host one after
+// the other a call takes 19 us, which is the host's.
 //
 // The tokens are quantised by the kernel of fp8_blocks.cu (doing it here instead, once for every 32 rows of w, took longer than
 // the weight: 18.6 us).  This kernel starts while that one runs (programmatic launch): what it reads of w was there before

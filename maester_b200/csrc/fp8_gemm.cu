@@ -17,6 +17,11 @@
 //
 // Warp 0: TMA; warp 1: MMA issue (even CTA); warps 2-5: epilogue.  All waits are bounded; both CTAs always reach the cluster
 // barriers.
+//
+// Measured: 16384 x 4096 x 4096 0.211 to 0.216 ms (2550 to 2600 TFLOP/s, 1.55 of the 16-bit rate of 1641), 16384 x 20480 x 2560
+// 2390, 16384 x 2560 x 10240 2530.  Bound by power: the tensor pipe is active 81 % of the time at 1.56 GHz, and zeros as
+// operands run at 3180.  The copies of the exponents cost 5 % there (3350 without them), the scaling itself as much again (3520
+// for the plain 8-bit instruction); issuing the copies in the middle of the previous group was slower (the commit waits for them).
 #include "gemm_common.cuh"
 #include "host_common.cuh"
 #include "sm100_pair.cuh"
@@ -535,6 +540,19 @@ int make_scales_tmap(CUtensorMap* m, const void* base, uint64_t row_tiles, uint6
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
 }
 
+// Which kernel takes less time, in ns, as fitted to 336 problems of 12 to 777 rows, 256 to 20480 columns and 333 to 10240 deep
+// (errors 7 and 10 %; the choice costs 0.2 % over the faster one on average).  A wave of 256 x 256 tiles costs its depth, and
+// rows that are not on 16-byte boundaries their single stores; a wave of the small tiles its depth, its rows, and the meeting of
+// its parts.  Examples (us, 256 x 256 tiles and small ones): 24 x 4096 x 4096 16.8 and 9.9, 64 x 20480 x 2560 21.3 and 16.9,
+// 64 x 14336 x 4096 17.7 and 20.2, 256 x 4096 x 4096 17.6 and 20.2, 333 x 777 x 1100 14.5 and 11.4, 512 x 4608 x 512 7.9 and 10.7.
+bool few_is_faster(long long tiles, long long units, int n, int split, int kblocks, int groups, bool vec) {
+  const long long sms = mbh::sm_count(), big_waves = (tiles + sms / 2 - 1) / (sms / 2);
+  const long long big = 4800 + big_waves * (1600 + 350ll * kblocks + (vec ? 0 : 4200));
+  const long long ctas = units * split, waves = (ctas + 2 * sms - 1) / (2 * sms), depth = min(kblocks, (groups + split - 1) / split * 4);
+  const long long of_few = 3200 + waves * (77 * n + 400 * depth + depth * n * (ctas > sms ? 2 : 1) * 57 / 100 + (split > 1 ? 138 * n / split : 0));
+  return of_few < big;
+}
+
 }  // namespace
 
 // a: [M, 128 kblocks] codes with row pitch lda and exponents sa, b: [N, 128 kblocks] likewise; out: 0 bf16, 1 fp32, 2 fp32 +=
@@ -559,11 +577,13 @@ extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const v
   if (tiles > 0x7fffffffll / 2) return -3;
   CUtensorMap ta, tb, tsa, tsb;
   const uint64_t cols = static_cast<uint64_t>(kblocks) * 128, groups = (kblocks + 3) / 4;
-  // Tiles of 256 x 256 need some 37 of them (half the pairs) to be worth their size; below that, and for few rows, 128 x 64 tiles
-  // with a split contraction put more SMs to work.
   const int row_tiles = (N + few::ROWS - 1) / few::ROWS;
   const int n = M <= 16 ? 16 : M <= 32 ? 32 : 64, m_tiles = (M + n - 1) / n;
-  const bool few_rows = (M <= few::MAX_N || tiles < mbh::sm_count() / 4) && m_tiles <= 65535;
+  // CTAs of a tile: two an SM altogether at the most, whole groups of four k-blocks each
+  const long long units = static_cast<long long>(row_tiles) * m_tiles;
+  int split = static_cast<int>(min(2 * mbh::sm_count() / units, static_cast<long long>(few::MAX_SPLIT)));
+  split = static_cast<int>(min(static_cast<uint64_t>(max(split, 1)), groups));
+  const bool few_rows = m_tiles <= 65535 && few_is_faster(tiles, units, n, split, kblocks, static_cast<int>(groups), p.vec);
   int e = make_codes_tmap(&ta, a, cols, M, lda, few_rows ? n : BM);
   if (!e) e = make_codes_tmap(&tb, b, cols, N, ldb, BNH);
   if (!e) e = make_scales_tmap(&tsa, sa, (M + 127) / 128, groups, 1);
@@ -573,11 +593,6 @@ extern "C" int mb_fp8_gemm(const void* a, const void* sa, const void* b, const v
     few::FewParams fp;
     fp.p = p;
     fp.n = n;
-    // CTAs of a tile: two an SM altogether at the most
-    const long long units = static_cast<long long>(row_tiles) * m_tiles;
-    int split = static_cast<int>(2 * mbh::sm_count() / units);
-    split = split < 1 ? 1 : split > few::MAX_SPLIT ? few::MAX_SPLIT : split;
-    if (split > static_cast<int>(groups)) split = static_cast<int>(groups);
     fp.split = split;
     const int smem = few::smem_bytes(n);
     MB_SET_MAX_SMEM_ONCE(few::fp8_gemm_few_kernel, 113 * 1024);

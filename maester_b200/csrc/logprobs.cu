@@ -6,18 +6,29 @@
 // Statistics are 32-bit whatever the type of the logits.  -inf logits have probability 0 and gradient 0; a row without a
 // finite logit, or with NaN or +inf, has no distribution and comes out as NaN.
 //
-// Forward: one pass over the logits.  A row belongs to one block of 256 threads, or to a cluster of 2, 4 or 8 of them when
-// rows are few (their results meet in the first block's shared memory).  Every thread copies its own next vectors into its own
-// slots of shared memory (cp.async), STAGES turns ahead: no thread waits for another's copy, and four blocks an SM keep 128 KiB
-// on the way while one of them puts a row's results together.  (Resident blocks that take row after row, with copies across
-// the ends of rows, were slower: SMs differ in their distance to memory, and a fixed share of the rows leaves the fast ones
-// idle at the end; 176 against 163 us for 4099 x 128256 bf16.)  A thread keeps its own running (max, sum, weighted sum) and
-// takes the maximum of 32 values first, so the sums are rescaled once for 32.
-// The alternatives need the threads' maxima only: at least `top` values reach the top-th largest of the 256, and hardly more
-// do, so the second look goes to the values of some `top` threads (a 256th of the row each, mostly still in L2).  What
-// reaches that threshold goes into short lists, one a warp; a full list is cut down to its best `top`, which raises the
-// threshold for the whole block.  Entries are (ordered value, inverted index), all different: equal values come out by the
-// lowest index, whatever the order of the work.
+// Forward: one pass over the logits, bound by reading them.  A row belongs to one block of 256 threads, or to a cluster of 2, 4
+// or 8 of them when rows are few (their results meet in the first block's shared memory), or to a block of 128 threads when
+// rows are many and short: what a block does after its last vector does not overlap with its own copies, and smaller blocks
+// leave more neighbours that go on.  Every thread copies its own next vectors into its own slots of shared memory (cp.async),
+// STAGES turns ahead: no thread waits for another's copy, and 128 KiB an SM are on the way while a block puts a row's results
+// together (three turns ahead: no faster; five blocks an SM: slower by a twentieth, the registers spill).  Resident blocks that
+// take row after row, with copies across the ends of rows, were slower: SMs differ in their distance to memory, and a fixed
+// share of the rows leaves the fast ones idle at the end; 176 against 163 us for 4099 x 128256 bf16.
+// A thread keeps its own running (max, sum, weighted sum) and takes the maximum of 32 values first, so the sums are rescaled
+// once for 32; two fp32 operations an instruction.
+//
+// Alternatives: 1024 cells (a quarter or an eighth of a thread's turns) keep their maxima.  At least `top` values reach the
+// top-th largest of 64 or 128 groups of threads, and hardly more do, so the second look goes to some `top` cells (a thousandth
+// of the row each, mostly still in L2).  What reaches that threshold goes into short lists, one a warp; a full list is cut down
+// to its best `top`, which raises the threshold for the whole block.  Entries are (ordered value, inverted index), all
+// different: equal values come out by the lowest index, whatever the order of the work.  With one maximum a thread the second
+// look was four times as long: 240 against 202 us for 4099 x 128256 bf16, 20 alternatives; a threshold found bit by bit and
+// lists filled by one vector a warp at a time cost 370 - 243 us of it at 64.
+//
+// Measured (bf16, copy rate of the same GPU: 6540 GB/s): 4096 x 128256 162 us without entropy (6470 GB/s), 179 with, 194 with 5
+// alternatives, 204 with 20, 245 with 64; 8192 x 32000 92, 100, 126, 135, 200; 16 x 262144, where a launch and a row's chain of
+// steps count, 10 to 17.  The entropy costs its instructions (two more of some nine for two values), the alternatives the
+// steps after the last vector, some 9000 cycles of a row.  Gradient: 330 us for 4096 x 128256 (6370 GB/s).
 #include "host_common.cuh"
 #include "sm100.cuh"
 #include <cuda_fp16.h>
@@ -714,8 +725,10 @@ logprobs_bwd_kernel(const T* __restrict__ x, const long long* __restrict__ token
   }
 }
 
-// Blocks of a row: the split with the fewest waves times the length of one.  A block costs its vectors and about 1500 more (its
-// start, the reductions, the alternatives), a cluster's barrier some 500.
+// Blocks of a row, and whether they are the small ones: the split with the fewest waves times the length of one.  A block costs
+// its vectors and about 1500 more (its start, the reductions, the alternatives), a cluster's barrier some 500; small blocks run
+// at half the speed, twice as many at a time.  (8192 x 32000 bf16, 5 alternatives: 126 us with small blocks, 160 with large ones;
+// 4099 x 128256: 211 and 200; 2048 x 50257: 54 and 62.)
 int blocks_per_row(int rows, int V, int elem, bool& small) {
   const long long sms = mbh::sm_count(), slots = ON_SM / 256 * sms, vectors = static_cast<long long>(V) * elem / 16;
   int best = 1;
