@@ -79,9 +79,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     All results are fp32 whatever the type of the logits (bf16, fp16, fp32; rows may have any pitch).  A row whose token is
     -100 is skipped: log-probability and entropy 0, alternatives -inf with id -1, no gradient.  A -inf logit (or one whose
     distance from the row's maximum is beyond fp32) has probability 0; a row without a finite logit, or with NaN or +inf, has
-    no distribution: its numbers are NaN, its alternatives are still in order (NaN above +inf).  A token id outside [0, V) gives NaN and a device status error
-    (``ops.cuda.check_status``); on the CPU it raises.  Gradients flow to the logits from log-probabilities, entropies and
-    the alternatives' log-probabilities.  The first call on a device has to run outside a stream capture."""
+    no distribution: its numbers are NaN, its alternatives are still in order (NaN above +inf).  A token id outside [0, V)
+    gives NaN and a device status error (``ops.cuda.check_status``); on the CPU it raises.  ``scale`` is a number in
+    [1e-8, 1e8].  Gradients flow to the logits from log-probabilities, entropies and the alternatives' log-probabilities.
+    The first call on a device has to run outside a stream capture."""
     if logits.dim() < 1 or not logits.is_floating_point():
         raise TypeError("logits have to be a floating-point tensor with a vocabulary dimension")
     V, lead = logits.shape[-1], logits.shape[:-1]
