@@ -714,6 +714,12 @@ def _stream_of(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+def _fit(*sizes: int) -> None:
+    """Sizes that travel as C ints."""
+    if max(sizes) > 0x7fffffff - 65536:
+        raise ValueError(f"a matrix of {' x '.join(map(str, sizes))}: rows and columns have to be below 2^31 - 2^16")
+
+
 def on_device(t: torch.Tensor):
     """Context in which ``t``'s device is the current one (its current stream takes the launches)."""
     return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
@@ -725,6 +731,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 def logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor | None, scale: float, entropy: bool, top: int, stats: bool):
     """Rows of ``logits`` [R, V] -> (logprobs | None, entropy | None, top_logprobs | None, top_tokens | None, stats | None)."""
     R, V = logits.shape
+    _fit(R, V)
     dev, f32, empty = logits.device, torch.float32, torch.empty
     lp = empty(R, device=dev, dtype=f32) if tokens is not None else None
     ent = empty(R, device=dev, dtype=f32) if entropy else None
@@ -743,6 +750,7 @@ def logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor | None, scale: float
                  g_top: torch.Tensor | None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of the logits; ``out`` (optional, row-major) may be bf16 beside fp32 logits."""
     R, V = logits.shape
+    _fit(R, V)
     if out is None:   # rows that lie as the logits' rows do: both are then aligned alike
         pitch = logits.stride(0) if V <= logits.stride(0) < 2 * V else V
         out = torch.empty(R, pitch, device=logits.device, dtype=logits.dtype)
@@ -771,6 +779,7 @@ def _fp8_buffers(rows: int, cols: int, device):
 def fp8_quantize(x: torch.Tensor, rows: bool = True, cols: bool = False, square: bool = False):
     """((codes, scales) of ``x`` | None, (codes, scales) of ``x.T`` | None) from one pass over ``x`` [R, C]."""
     R, C = x.shape
+    _fit(R, C)
     q, sq = _fp8_buffers(R, C, x.device) if rows else (None, None)
     qt, sqt = _fp8_buffers(C, R, x.device) if cols else (None, None)
     mode = FP8_ROWS * rows + FP8_COLS * cols + FP8_SQUARE * square
@@ -784,6 +793,7 @@ def fp8_gemm(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tenso
              accumulate: bool = False) -> torch.Tensor:
     """``out (+)= A @ B.T`` of codes [M, Kp] and [N, Kp] with packed exponents; ``out`` row-major bf16 or fp32."""
     M, N = a.shape[0], b.shape[0]
+    _fit(M, N)
     assert a.shape[1] == b.shape[1] and a.shape[1] % 128 == 0 and out.shape == (M, N) and out.stride(1) == 1
     assert not accumulate or out.dtype == torch.float32
     with on_device(out):
@@ -802,6 +812,7 @@ def fp8_linear_fwd(x: torch.Tensor, w: torch.Tensor, keep_x: bool, keep_w: bool)
     """(``Q(x) @ Q(w).T``, packed codes of ``x.T`` | None, of ``w.T`` | None) of [M, K] and [N, K] with unit column stride."""
     (M, K), (N, Kw) = x.shape, w.shape
     assert K == Kw and x.device == w.device
+    _fit(M, K, N)
     kb, dev, u8, empty = (K + 127) // 128, x.device, torch.uint8, torch.empty
     work = empty(_fp8_bytes(M, kb) + _fp8_bytes(N, kb), device=dev, dtype=u8)
     x_t = empty(_fp8_bytes(K, (M + 127) // 128), device=dev, dtype=u8) if keep_x else None
@@ -819,6 +830,7 @@ def fp8_linear_bwd(dy: torch.Tensor, K: int, x_t: torch.Tensor | None, w_t: torc
     """dx [M, K] | None (with ``w_t``) of ``dy`` [M, N]; with ``x_t`` the weight's gradient goes into ``dw`` (or is added to it,
     fp32 then)."""
     M, N = dy.shape
+    _fit(M, N)
     nb, mb = (N + 127) // 128, (M + 127) // 128
     work = torch.empty((0 if w_t is None else _fp8_bytes(M, nb)) + (0 if x_t is None else _fp8_bytes(N, mb)), device=dy.device,
                        dtype=torch.uint8)
@@ -843,6 +855,7 @@ def fp8_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> to
     """``Q(x) @ W.T`` for ``x`` [M, K] of unit column stride and a weight's codes [N, Kp]."""
     M, K = x.shape
     N, Kp = codes.shape
+    _fit(M, N, K)
     y = torch.empty(M, N, device=x.device, dtype=x.dtype)
     work = torch.empty(_fp8_bytes(M, Kp // 128), device=x.device, dtype=torch.uint8)   # codes and exponents of x
     with on_device(x):

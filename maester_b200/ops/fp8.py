@@ -125,7 +125,8 @@ def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, *, out_dtype: torch.dtype = torch.bfl
         if out_dtype not in _TYPES:
             raise TypeError(f"bf16 or fp32 output is wanted, got {out_dtype}")
         out = torch.empty(a.rows, b.rows, device=a.device, dtype=out_dtype)
-    elif tuple(out.shape) != (a.rows, b.rows) or out.device != a.device or (out.stride(1) != 1 and out.shape[1] > 1):
+    elif tuple(out.shape) != (a.rows, b.rows) or out.device != a.device or (out.stride(1) != 1 and out.shape[1] > 1) or (
+            out.stride(0) < out.shape[1] and out.shape[0] > 1):
         raise ValueError(f"out has to be a row-major {(a.rows, b.rows)} matrix on {a.device}")
     elif out.dtype not in _TYPES or (accumulate and out.dtype != torch.float32):
         raise TypeError(f"out is {out.dtype}: bf16 or fp32 is wanted, fp32 to accumulate")

@@ -79,6 +79,9 @@ class AdamWMulti(Optimizer):
             self._slots[p] = slot = _Slot(p, total, p.numel())
             batch.slots.append(slot)
             total += -(-p.numel() // ref.STATE_BLOCK) * ref.STATE_BLOCK
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in every if p.numel())
+        if any(a[1] > b[0] > 0 for a, b in zip(spans, spans[1:])):
+            raise ValueError("two parameters share memory, or one is given twice: a step would update it twice at a time")
         if state_bits == 8:
             blocks = total // ref.STATE_BLOCK
             code = lambda: torch.zeros(total, device=self.device, dtype=torch.float8_e4m3fn)
@@ -97,6 +100,9 @@ class AdamWMulti(Optimizer):
         if self._sealed:
             raise RuntimeError("the state buffers are laid out once: give every parameter to the constructor")
         super().add_param_group(group)
+
+    def __getstate__(self):
+        raise TypeError("AdamWMulti cannot be copied or pickled as an object: use state_dict()")
 
     def state_buffers(self) -> dict[str, torch.Tensor]:
         """The flat state buffers themselves: ``exp_avg``, ``exp_avg_root`` (codes) with ``exp_avg_exp``,

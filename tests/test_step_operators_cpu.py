@@ -1,4 +1,5 @@
 """Token log-probabilities, 8-bit linear layers and AdamW over many tensors on the CPU: definitions, refusals, checkpoints."""
+import copy
 import math
 
 import pytest
@@ -57,6 +58,13 @@ def test_logprobs_refusals(kw, error):
     with pytest.raises(error):
         kw = {("logit_scale" if k == "scale" else k): v for k, v in kw.items()}
         ops.linear_logprobs(torch.randn(4, 6), torch.randn(8, 6), **kw)
+
+
+def test_sizes_that_no_kernel_counts():
+    from maester_b200.ops import cuda as C
+    C._fit(5, 2 ** 31 - 2 ** 16 - 1)
+    with pytest.raises(ValueError, match="below"):
+        C._fit(5, 2 ** 31)
 
 
 @pytest.mark.parametrize("scale", [1e-9, 1e9, math.inf, 10 ** 400, "1", None])
@@ -144,6 +152,7 @@ def test_fp8_refusals():
                        (lambda: ops.matmul_fp8(h, h, out=torch.zeros(8, 8, dtype=torch.bfloat16), accumulate=True), TypeError),
                        (lambda: ops.matmul_fp8(h, h, out=torch.zeros(8, 9)), ValueError),
                        (lambda: ops.matmul_fp8(h, h, out=torch.zeros(8, 16)[:, ::2]), ValueError),
+                       (lambda: ops.matmul_fp8(h, h, out=torch.zeros(1, 8).expand(8, 8)), ValueError),
                        (lambda: ops.Fp8Blocks(h.data, h.scales, 129), ValueError),
                        (lambda: ops.Fp8Blocks(h.data[:, :64], h.scales, 64), TypeError),
                        (lambda: ops.Fp8Blocks(h.data, h.scales[:, :, :16], 64), ValueError),
@@ -298,6 +307,16 @@ def test_adamw_multi_refusals():
                        (lambda: AdamWMulti([p]).load_param_state(p, {"exp_avg": torch.zeros(3)}), ValueError)):
         with pytest.raises(error):
             bad()
+    flat = torch.zeros(20)
+    twice = (flat[:12], flat[11:]), (flat, flat), (flat.view(4, 5), flat)
+    for pair in twice:
+        with pytest.raises(ValueError, match="share memory"):
+            AdamWMulti([torch.nn.Parameter(x) for x in pair])
+    with pytest.warns(UserWarning, match="duplicate"), pytest.raises(ValueError, match="twice"):
+        AdamWMulti([p, p])
+    AdamWMulti([torch.nn.Parameter(x) for x in (flat[:10], flat[10:], flat[:0])])
+    with pytest.raises(TypeError, match="state_dict"):
+        copy.deepcopy(AdamWMulti([p]))
     opt = AdamWMulti([p])
     p.grad = torch.zeros(4, 4).to_sparse()
     with pytest.raises(RuntimeError, match="dense"):
