@@ -21,7 +21,8 @@
 // Measured: 16384 x 4096 x 4096 0.211 to 0.216 ms (2550 to 2600 TFLOP/s, 1.55 of the 16-bit rate of 1641), 16384 x 20480 x 2560
 // 2390, 16384 x 2560 x 10240 2530.  Bound by power: the tensor pipe is active 81 % of the time at 1.56 GHz, and zeros as
 // operands run at 3180.  The copies of the exponents cost 5 % there (3350 without them), the scaling itself as much again (3520
-// for the plain 8-bit instruction); issuing the copies in the middle of the previous group was slower (the commit waits for them).
+// for the plain 8-bit instruction); issuing the copies in the middle of the previous group was slower (the commit waits for them),
+// and so was writing the exponents with four more warps (tcgen05.st, a commit more every four k-blocks: 242 us and more).
 #include "gemm_common.cuh"
 #include "host_common.cuh"
 #include "sm100_pair.cuh"
