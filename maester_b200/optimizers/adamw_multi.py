@@ -20,8 +20,9 @@ from maester_b200.ops import reference as ref
 
 _TYPES = (torch.float32, torch.bfloat16)
 # a step looks at every tensor: mapped over the lists, which takes half the time of a loop
-_grad, _dtype, _layout, _numel = map(operator.attrgetter, ("grad", "dtype", "layout", "numel"))
-_device, _contiguous, _address = torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+_grad, _dtype = map(operator.attrgetter, ("grad", "dtype"))
+_device, _numel, _contiguous, _address = (torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.is_contiguous,
+                                          torch.Tensor.data_ptr)
 
 
 class _Slot:
@@ -34,7 +35,7 @@ class _Slot:
 
 
 class _Batch:
-    __slots__ = ("group", "dtype", "slots", "params", "table")
+    __slots__ = ("group", "dtype", "slots", "params", "sizes", "copies", "table")
 
     def __init__(self, group: int, dtype: torch.dtype):
         self.group, self.dtype, self.slots = group, dtype, []
@@ -91,7 +92,7 @@ class AdamWMulti(Optimizer):
         else:
             self._buffers = {k: torch.zeros(total, device=self.device) for k in ("exp_avg", "exp_avg_sq")}
         for b in self._batches:
-            b.params = [s.param for s in b.slots]
+            b.params, b.sizes, b.copies = [s.param for s in b.slots], [s.numel for s in b.slots], False
             b.table = np.array([(0, 0, 0, s.numel, s.offset, 0) for s in b.slots], dtype=np.int64)
         self.writes_lowp = False    # the sharding runtime's 16-bit parameters are written by step()
         self._sealed = True
@@ -120,6 +121,8 @@ class AdamWMulti(Optimizer):
                                  f"many on {self.device}")
         for p, c in copies.items():
             self._slots[p].copy = c
+        for b in self._batches:
+            b.copies = any(x.copy is not None for x in b.slots)
 
     def attach_sharding(self, sharded) -> None:
         """Write the sharding runtime's 16-bit shard with the update (called by the optimizer builder)."""
@@ -141,14 +144,13 @@ class AdamWMulti(Optimizer):
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWMulti.step() cannot be captured: learning rate and step number are launch arguments")
         for batch in self._batches:
-            slots, params, grads = batch.slots, batch.params, list(map(_grad, batch.params))
+            slots, params, sizes, grads = batch.slots, batch.params, batch.sizes, list(map(_grad, batch.params))
             if any(g is None for g in grads):
                 live = [i for i, g in enumerate(grads) if g is not None]
                 if not live:
                     continue
-                slots, params, grads = ([x[i] for i in live] for x in (slots, params, grads))
-            self._check(batch, slots, params, grads)
-            if not all(map(_contiguous, grads)):
+                slots, params, sizes, grads = ([x[i] for i in live] for x in (slots, params, sizes, grads))
+            if not self._check(batch.dtype, params, sizes, grads):
                 grads = [g.contiguous() for g in grads]
             group = self.param_groups[batch.group]
             b1, b2 = group["betas"]
@@ -165,27 +167,31 @@ class AdamWMulti(Optimizer):
                     x.step = t
         return loss
 
-    def _check(self, batch, slots, params, grads) -> None:
-        """Parameters and gradients are what the tables say (a kernel gets nothing but their addresses)."""
-        dtype, device, sizes = batch.dtype, self.device.index if self.device.type == "cuda" else -1, list(map(_numel, slots))
-        if not (set(map(_dtype, grads)) == {dtype} and set(map(_layout, grads)) == {torch.strided}
-                and set(map(_device, grads)) == {device} and list(map(torch.Tensor.numel, grads)) == sizes):
+    def _check(self, dtype, params, sizes, grads) -> bool:
+        """Parameters and gradients are what the tables say (a kernel gets nothing but their addresses).  Are the gradients
+        contiguous?"""
+        device = self.device.index if self.device.type == "cuda" else -1
+        contiguous = all(map(_contiguous, grads))       # (no sparse gradient is)
+        if not ((contiguous or all(g.layout is torch.strided for g in grads)) and set(map(_dtype, grads)) == {dtype}
+                and set(map(_device, grads)) == {device} and list(map(_numel, grads)) == sizes):
             g = next(g for g, n in zip(grads, sizes) if g.dtype is not dtype or g.layout is not torch.strided
                      or g.get_device() != device or g.numel() != n)
             raise RuntimeError(f"the gradient of a {dtype} parameter on {self.device} has to be a dense tensor of its type and "
                                f"size there, got {g.dtype} {tuple(g.shape)} on {g.device} ({g.layout})")
         if not (set(map(_dtype, params)) == {dtype} and set(map(_device, params)) == {device}
-                and list(map(torch.Tensor.numel, params)) == sizes and all(map(_contiguous, params))):
+                and list(map(_numel, params)) == sizes and all(map(_contiguous, params))):
             raise RuntimeError("a parameter was replaced by one of another type, size, device or layout")
+        return contiguous
 
     def _launch(self, batch, slots, grads, h) -> None:
         from maester_b200.ops import cuda as C
         table = batch.table
         if len(slots) < len(batch.slots):
             table = np.array([(0, 0, 0, s.numel, s.offset, 0) for s in slots], dtype=np.int64)
-        table[:, 0] = [s.param.data_ptr() for s in slots]
+        table[:, 0] = list(map(_address, [s.param for s in slots]))
         table[:, 1] = list(map(_address, grads))
-        table[:, 2] = [0 if s.copy is None else s.copy.data_ptr() for s in slots]
+        if batch.copies:
+            table[:, 2] = [0 if s.copy is None else s.copy.data_ptr() for s in slots]
         f = self._buffers
         C.adamw_multi(table, batch.dtype is torch.bfloat16, self.state_bits, f["exp_avg"], f.get("exp_avg_exp"),
                       f["exp_avg_root" if self.state_bits == 8 else "exp_avg_sq"], f.get("exp_avg_root_exp"),

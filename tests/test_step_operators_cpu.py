@@ -318,9 +318,10 @@ def test_adamw_multi_refusals():
     with pytest.raises(TypeError, match="state_dict"):
         copy.deepcopy(AdamWMulti([p]))
     opt = AdamWMulti([p])
-    p.grad = torch.zeros(4, 4).to_sparse()
-    with pytest.raises(RuntimeError, match="dense"):
-        opt.step()
+    for sparse in (torch.zeros(4, 4).to_sparse(), torch.eye(4).to_sparse()):
+        p.grad = sparse
+        with pytest.raises(RuntimeError, match="dense"):
+            opt.step()
 
 
 # ---------------------------------------------------------------- together
