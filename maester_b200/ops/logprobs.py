@@ -44,6 +44,10 @@ def _check(tokens, lead, device, V, scale, entropy, top) -> None:
         raise ValueError(f"tokens are on {tokens.device}, the rows on {device}")
 
 
+def _dense_f32(g: torch.Tensor | None) -> torch.Tensor | None:
+    return g if g is None or (g.dtype is torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
+
+
 class _TokenLogprobs(Function):
     @staticmethod
     def forward(ctx, x, tokens, scale, entropy, top):
@@ -61,7 +65,7 @@ class _TokenLogprobs(Function):
         x, tokens, stats, top_id = ctx.saved_tensors
         if g_lp is None and g_ent is None and g_top is None:
             return None, None, None, None, None
-        g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_lp, g_ent, g_top)]
+        g = [_dense_f32(t) for t in (g_lp, g_ent, g_top)]
         return _C().logprobs_bwd(x, tokens, ctx.scale, stats, g[0], g[1], top_id, g[2]), None, None, None, None
 
 
@@ -92,7 +96,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     x = logits if logits.dim() == 2 else logits.reshape(math.prod(lead), V)
     t = None
     if tokens is not None:
-        t = tokens.reshape(-1)
+        t = tokens if len(lead) == 1 else tokens.reshape(-1)
         if t.dtype != torch.int64:
             t = t.to(torch.int64)
         if not t.is_contiguous():
@@ -138,7 +142,7 @@ class _LinearLogprobs(Function):
             return (None,) * 6
         M, D = h.shape
         V = w.shape[0]
-        g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_lp, g_ent, g_top)]
+        g = [_dense_f32(t) for t in (g_lp, g_ent, g_top)]
         # a row of dh is one product (fp32 sum over the whole vocabulary, rounded once, the same bits every time); dw adds
         # the chunks up in fp32
         dh = torch.empty(M, D, device=h.device, dtype=h.dtype) if ctx.needs_input_grad[0] else None
