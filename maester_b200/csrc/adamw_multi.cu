@@ -17,7 +17,7 @@
 //
 // Measured (24 tensors of 4096 x 4096; copy rate 6540 GB/s): fp32 parameters with a copy 1081 us with 8-bit states (6710 GB/s),
 // 1799 us with 32-bit ones (6710); bf16 parameters 769 us with 8-bit states (5240: the codes cost more instructions than the 10
-// bytes of a value cost time), 1339 us with 32-bit ones (6610).  Small tensors are the host's: 48 us for 20 of them.
+// bytes of a value cost time), 1339 us with 32-bit ones (6610).  Small tensors are the host's: 40 us for 20 of them.
 #include "fp8_common.cuh"
 #include "host_common.cuh"
 #include <math.h>

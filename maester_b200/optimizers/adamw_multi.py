@@ -26,16 +26,16 @@ _device, _numel, _contiguous, _address = (torch.Tensor.get_device, torch.Tensor.
 
 
 class _Slot:
-    """A parameter, where its states lie, and how many steps it has taken."""
+    """A parameter, its row in the batch's table, where its states lie, and how many steps it has taken."""
 
-    __slots__ = ("param", "offset", "numel", "step", "copy")
+    __slots__ = ("param", "row", "offset", "numel", "step", "copy")
 
-    def __init__(self, param, offset: int, numel: int):
-        self.param, self.offset, self.numel, self.step, self.copy = param, offset, numel, 0, None
+    def __init__(self, param, row: int, offset: int, numel: int):
+        self.param, self.row, self.offset, self.numel, self.step, self.copy = param, row, offset, numel, 0, None
 
 
 class _Batch:
-    __slots__ = ("group", "dtype", "slots", "params", "sizes", "copies", "table")
+    __slots__ = ("group", "dtype", "slots", "params", "sizes", "memory", "addresses", "table")
 
     def __init__(self, group: int, dtype: torch.dtype):
         self.group, self.dtype, self.slots = group, dtype, []
@@ -77,7 +77,7 @@ class AdamWMulti(Optimizer):
             if batch is None:
                 batch = _Batch(of[id(p)], p.dtype)
                 self._batches.append(batch)
-            self._slots[p] = slot = _Slot(p, total, p.numel())
+            self._slots[p] = slot = _Slot(p, len(batch.slots), total, p.numel())
             batch.slots.append(slot)
             total += -(-p.numel() // ref.STATE_BLOCK) * ref.STATE_BLOCK
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in every if p.numel())
@@ -92,8 +92,9 @@ class AdamWMulti(Optimizer):
         else:
             self._buffers = {k: torch.zeros(total, device=self.device) for k in ("exp_avg", "exp_avg_sq")}
         for b in self._batches:
-            b.params, b.sizes, b.copies = [s.param for s in b.slots], [s.numel for s in b.slots], False
+            b.params, b.sizes = [s.param for s in b.slots], [s.numel for s in b.slots]
             b.table = np.array([(0, 0, 0, s.numel, s.offset, 0) for s in b.slots], dtype=np.int64)
+            self._take_memory(b)
         self.writes_lowp = False    # the sharding runtime's 16-bit parameters are written by step()
         self._sealed = True
 
@@ -120,9 +121,9 @@ class AdamWMulti(Optimizer):
                 raise ValueError(f"the copy of a parameter of {p.numel()} elements has to be a contiguous bf16 tensor of as "
                                  f"many on {self.device}")
         for p, c in copies.items():
-            self._slots[p].copy = c
+            self._slots[p].copy = c.detach()        # (of its own: what happens to the caller's tensor leaves it where it is)
         for b in self._batches:
-            b.copies = any(x.copy is not None for x in b.slots)
+            b.table[:, 2] = [0 if x.copy is None else x.copy.data_ptr() for x in b.slots]
 
     def attach_sharding(self, sharded) -> None:
         """Write the sharding runtime's 16-bit shard with the update (called by the optimizer builder)."""
@@ -145,12 +146,15 @@ class AdamWMulti(Optimizer):
             raise RuntimeError("AdamWMulti.step() cannot be captured: learning rate and step number are launch arguments")
         for batch in self._batches:
             slots, params, sizes, grads = batch.slots, batch.params, batch.sizes, list(map(_grad, batch.params))
+            # parameters in the memory they were in are what they were: it is held, so nothing else can have its addresses
+            if list(map(_address, params)) != batch.addresses or not all(map(_contiguous, params)):
+                self._take_memory(batch)
             if any(g is None for g in grads):
                 live = [i for i, g in enumerate(grads) if g is not None]
                 if not live:
                     continue
-                slots, params, sizes, grads = ([x[i] for i in live] for x in (slots, params, sizes, grads))
-            if not self._check(batch.dtype, params, sizes, grads):
+                slots, sizes, grads = ([x[i] for i in live] for x in (slots, sizes, grads))
+            if not self._check(batch.dtype, sizes, grads):
                 grads = [g.contiguous() for g in grads]
             group = self.param_groups[batch.group]
             b1, b2 = group["betas"]
@@ -167,9 +171,18 @@ class AdamWMulti(Optimizer):
                     x.step = t
         return loss
 
-    def _check(self, dtype, params, sizes, grads) -> bool:
-        """Parameters and gradients are what the tables say (a kernel gets nothing but their addresses).  Are the gradients
-        contiguous?"""
+    def _take_memory(self, batch) -> None:
+        """Note where the parameters are and hold that memory."""
+        for p, n in zip(batch.params, batch.sizes):
+            if p.dtype is not batch.dtype or p.device != self.device or p.numel() != n or not p.is_contiguous() or (
+                    n and not p.data_ptr()):
+                raise RuntimeError("a parameter was replaced by one of another type, size, device or layout, or has no memory")
+        batch.memory = [p.detach() for p in batch.params]
+        batch.addresses = list(map(_address, batch.memory))
+        batch.table[:, 0] = batch.addresses
+
+    def _check(self, dtype, sizes, grads) -> bool:
+        """Gradients are what the table says (a kernel gets nothing but their addresses).  Are they contiguous?"""
         device = self.device.index if self.device.type == "cuda" else -1
         contiguous = all(map(_contiguous, grads))       # (no sparse gradient is)
         if not ((contiguous or all(g.layout is torch.strided for g in grads)) and set(map(_dtype, grads)) == {dtype}
@@ -178,20 +191,12 @@ class AdamWMulti(Optimizer):
                      or g.get_device() != device or g.numel() != n)
             raise RuntimeError(f"the gradient of a {dtype} parameter on {self.device} has to be a dense tensor of its type and "
                                f"size there, got {g.dtype} {tuple(g.shape)} on {g.device} ({g.layout})")
-        if not (set(map(_dtype, params)) == {dtype} and set(map(_device, params)) == {device}
-                and list(map(_numel, params)) == sizes and all(map(_contiguous, params))):
-            raise RuntimeError("a parameter was replaced by one of another type, size, device or layout")
         return contiguous
 
     def _launch(self, batch, slots, grads, h) -> None:
         from maester_b200.ops import cuda as C
-        table = batch.table
-        if len(slots) < len(batch.slots):
-            table = np.array([(0, 0, 0, s.numel, s.offset, 0) for s in slots], dtype=np.int64)
-        table[:, 0] = list(map(_address, [s.param for s in slots]))
+        table = batch.table if len(slots) == len(batch.slots) else batch.table[[s.row for s in slots]]
         table[:, 1] = list(map(_address, grads))
-        if batch.copies:
-            table[:, 2] = [0 if s.copy is None else s.copy.data_ptr() for s in slots]
         f = self._buffers
         C.adamw_multi(table, batch.dtype is torch.bfloat16, self.state_bits, f["exp_avg"], f.get("exp_avg_exp"),
                       f["exp_avg_root" if self.state_bits == 8 else "exp_avg_sq"], f.get("exp_avg_root_exp"),

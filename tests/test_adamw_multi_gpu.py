@@ -170,6 +170,36 @@ def test_strided_gradients_streams_and_capture():
             opt.step()
 
 
+def test_parameters_that_move():
+    """A parameter whose memory is replaced is updated where it is then; one that is no longer what it was is refused."""
+    a, b = _params([700, 33, 5000], torch.float32), _params([700, 33, 5000], torch.float32)
+    for p, q in zip(a, b):
+        q.data.copy_(p.data)
+    oa, ob = AdamWMulti(a, lr=0.1), AdamWMulti(b, lr=0.1)
+    for step in range(3):
+        _grads(a, step)
+        for p, q in zip(a, b):
+            q.grad = p.grad.clone()
+        old = a[1].data
+        if step == 1:
+            a[1].data = old.clone()
+            before = old.clone()
+        oa.step()
+        ob.step()
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+        if step == 1:
+            assert torch.equal(old, before)
+    good = a[2].data
+    for bad in (good.bfloat16(), good[:100].clone(), good.cpu(), torch.zeros(10000, device="cuda")[::2]):
+        a[2].grad = None
+        a[2].data = bad
+        with pytest.raises(RuntimeError, match="replaced"):
+            oa.step()
+    a[2].data = good
+    a[2].grad = torch.zeros(5000, device="cuda")
+    oa.step()
+
+
 def test_saved_and_loaded_on_the_gpu():
     a = _params([1000, 77], torch.float32)
     opt = AdamWMulti(a, lr=1e-2)
