@@ -23,6 +23,12 @@ _TYPES = (torch.float32, torch.bfloat16)
 _grad, _dtype = map(operator.attrgetter, ("grad", "dtype"))
 _device, _numel, _contiguous, _address = (torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.is_contiguous,
                                           torch.Tensor.data_ptr)
+_held_at, _held_bytes = torch.UntypedStorage.data_ptr, torch.UntypedStorage.nbytes
+
+
+def _missing(x: torch.Tensor) -> int:
+    """Bytes that a tensor's storage is short of what the tensor spans (a storage may have been resized under it)."""
+    return (x.storage_offset() + x.numel()) * x.element_size() - x.untyped_storage().nbytes() if x.numel() else 0
 
 
 class _Slot:
@@ -95,6 +101,7 @@ class AdamWMulti(Optimizer):
             b.params, b.sizes = [s.param for s in b.slots], [s.numel for s in b.slots]
             b.table = np.array([(0, 0, 0, s.numel, s.offset, 0) for s in b.slots], dtype=np.int64)
             self._take_memory(b)
+        self._copy_storages, self._copy_memory = [], []       # of the 16-bit copies: theirs once each, and where they were
         self.writes_lowp = False    # the sharding runtime's 16-bit parameters are written by step()
         self._sealed = True
 
@@ -113,7 +120,8 @@ class AdamWMulti(Optimizer):
         return dict(self._buffers)
 
     def attach_copies(self, copies: dict) -> None:
-        """{fp32 parameter: bf16 tensor of as many elements}: ``step()`` also writes the updated value there, rounded."""
+        """{fp32 parameter: bf16 tensor of as many elements}: ``step()`` also writes the updated value there, rounded.  A
+        copy whose memory has been freed (its storage resized to nothing) when ``step()`` is called is left out."""
         for p, c in copies.items():
             if p not in self._slots or p.dtype != torch.float32:
                 raise ValueError("a 16-bit copy belongs to an fp32 parameter of this optimizer")
@@ -121,9 +129,26 @@ class AdamWMulti(Optimizer):
                 raise ValueError(f"the copy of a parameter of {p.numel()} elements has to be a contiguous bf16 tensor of as "
                                  f"many on {self.device}")
         for p, c in copies.items():
-            self._slots[p].copy = c.detach()        # (of its own: what happens to the caller's tensor leaves it where it is)
+            self._slots[p].copy = c.detach()   # (of its own: the caller's tensor may change its shape or take another storage)
+        held = [x.copy.untyped_storage() for x in self._slots.values() if x.copy is not None]
+        self._copy_storages, self._copy_memory = list({s._cdata: s for s in held}.values()), None
+        self._find_copies()
+
+    def _find_copies(self) -> None:
+        """Note where the copies are.  Holding a tensor does not keep its storage from being resized: looked at in every step."""
+        now = list(map(_held_at, self._copy_storages)) + list(map(_held_bytes, self._copy_storages))
+        if now == self._copy_memory:
+            return
         for b in self._batches:
-            b.table[:, 2] = [0 if x.copy is None else x.copy.data_ptr() for x in b.slots]
+            at = []
+            for x in b.slots:
+                gone = x.copy is None or x.copy.untyped_storage().nbytes() == 0
+                if not gone and _missing(x.copy) > 0:
+                    raise RuntimeError(f"the storage of a 16-bit copy of {x.numel} elements has been resized to "
+                                       f"{x.copy.untyped_storage().nbytes()} bytes")
+                at.append(0 if gone else x.copy.data_ptr())
+            b.table[:, 2] = at
+        self._copy_memory = now
 
     def attach_sharding(self, sharded) -> None:
         """Write the sharding runtime's 16-bit shard with the update (called by the optimizer builder)."""
@@ -144,6 +169,7 @@ class AdamWMulti(Optimizer):
                 loss = closure()
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWMulti.step() cannot be captured: learning rate and step number are launch arguments")
+        self._find_copies()
         for batch in self._batches:
             slots, params, sizes, grads = batch.slots, batch.params, batch.sizes, list(map(_grad, batch.params))
             # parameters in the memory they were in are what they were: it is held, so nothing else can have its addresses
@@ -208,7 +234,7 @@ class AdamWMulti(Optimizer):
             m, v = self._moments(p)
             new, m, root, v = ref.adamw_multi_step(p.data.float().view(-1), g.float().reshape(-1), m, v, **h)
             p.copy_(new.view(p.shape))
-            if s.copy is not None:
+            if batch.table[s.row, 2]:
                 s.copy.view(-1).copy_(p.view(-1))
             self._store(p, m, root, v)
 
