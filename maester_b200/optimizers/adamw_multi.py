@@ -31,6 +31,12 @@ def _missing(x: torch.Tensor) -> int:
     return (x.storage_offset() + x.numel()) * x.element_size() - x.untyped_storage().nbytes() if x.numel() else 0
 
 
+def _overlap(tensors) -> bool:
+    """Do two of these contiguous tensors share memory?"""
+    spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in tensors if x.numel())
+    return any(a[1] > b[0] > 0 for a, b in zip(spans, spans[1:]))
+
+
 class _Slot:
     """A parameter, its row in the batch's table, where its states lie, and how many steps it has taken."""
 
@@ -41,7 +47,7 @@ class _Slot:
 
 
 class _Batch:
-    __slots__ = ("group", "dtype", "slots", "params", "sizes", "memory", "addresses", "table")
+    __slots__ = ("group", "dtype", "slots", "params", "sizes", "memory", "storages", "bytes", "addresses", "table")
 
     def __init__(self, group: int, dtype: torch.dtype):
         self.group, self.dtype, self.slots = group, dtype, []
@@ -86,8 +92,7 @@ class AdamWMulti(Optimizer):
             self._slots[p] = slot = _Slot(p, len(batch.slots), total, p.numel())
             batch.slots.append(slot)
             total += -(-p.numel() // ref.STATE_BLOCK) * ref.STATE_BLOCK
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in every if p.numel())
-        if any(a[1] > b[0] > 0 for a, b in zip(spans, spans[1:])):
+        if _overlap(every):
             raise ValueError("two parameters share memory, or one is given twice: a step would update it twice at a time")
         if state_bits == 8:
             blocks = total // ref.STATE_BLOCK
@@ -128,6 +133,9 @@ class AdamWMulti(Optimizer):
             if c.dtype != torch.bfloat16 or c.numel() != p.numel() or not c.is_contiguous() or c.device != self.device:
                 raise ValueError(f"the copy of a parameter of {p.numel()} elements has to be a contiguous bf16 tensor of as "
                                  f"many on {self.device}")
+        after = {p: x.copy for p, x in self._slots.items() if x.copy is not None} | copies
+        if _overlap([*self._slots, *after.values()]):
+            raise ValueError("16-bit copies share memory, with one another or with a parameter")
         for p, c in copies.items():
             self._slots[p].copy = c.detach()   # (of its own: the caller's tensor may change its shape or take another storage)
         held = [x.copy.untyped_storage() for x in self._slots.values() if x.copy is not None]
@@ -169,12 +177,11 @@ class AdamWMulti(Optimizer):
                 loss = closure()
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWMulti.step() cannot be captured: learning rate and step number are launch arguments")
+        self._find_parameters()
         self._find_copies()
+        work = []                                   # (everything is looked at before anything runs)
         for batch in self._batches:
-            slots, params, sizes, grads = batch.slots, batch.params, batch.sizes, list(map(_grad, batch.params))
-            # parameters in the memory they were in are what they were: it is held, so nothing else can have its addresses
-            if list(map(_address, params)) != batch.addresses or not all(map(_contiguous, params)):
-                self._take_memory(batch)
+            slots, sizes, grads = batch.slots, batch.sizes, list(map(_grad, batch.params))
             if any(g is None for g in grads):
                 live = [i for i, g in enumerate(grads) if g is not None]
                 if not live:
@@ -182,6 +189,8 @@ class AdamWMulti(Optimizer):
                 slots, sizes, grads = ([x[i] for i in live] for x in (slots, sizes, grads))
             if not self._check(batch.dtype, sizes, grads):
                 grads = [g.contiguous() for g in grads]
+            work.append((batch, slots, grads))
+        for batch, slots, grads in work:
             group = self.param_groups[batch.group]
             b1, b2 = group["betas"]
             lr = float(group["lr"])
@@ -197,13 +206,30 @@ class AdamWMulti(Optimizer):
                     x.step = t
         return loss
 
+    def _find_parameters(self) -> None:
+        """Parameters of the size and type they had, in the memory they were in, are what they were: that memory is held, so
+        nothing else can have its addresses."""
+        if all(list(map(_address, b.params)) == b.addresses and list(map(_numel, b.params)) == b.sizes
+               and all(map(_contiguous, b.params)) and set(map(_dtype, b.params)) == {b.dtype}
+               and list(map(_held_bytes, b.storages)) == b.bytes for b in self._batches):
+            return
+        for b in self._batches:
+            self._take_memory(b)
+        if _overlap([*self._slots, *(x.copy for x in self._slots.values() if x.copy is not None)]):
+            for b in self._batches:
+                b.addresses = None                  # (looked at again in the next step)
+            raise RuntimeError("two parameters, or a parameter and a copy, share memory: a step would update it twice at a time")
+
     def _take_memory(self, batch) -> None:
         """Note where the parameters are and hold that memory."""
+        batch.addresses = None
         for p, n in zip(batch.params, batch.sizes):
             if p.dtype is not batch.dtype or p.device != self.device or p.numel() != n or not p.is_contiguous() or (
-                    n and not p.data_ptr()):
+                    n and not p.data_ptr()) or _missing(p) > 0:
                 raise RuntimeError("a parameter was replaced by one of another type, size, device or layout, or has no memory")
         batch.memory = [p.detach() for p in batch.params]
+        batch.storages = list({s._cdata: s for s in (m.untyped_storage() for m in batch.memory)}.values())
+        batch.bytes = list(map(_held_bytes, batch.storages))
         batch.addresses = list(map(_address, batch.memory))
         batch.table[:, 0] = batch.addresses
 
