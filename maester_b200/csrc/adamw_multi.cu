@@ -8,6 +8,14 @@
 // second moment needs (e4m3 then spans 2^34 of v inside a block), and a root that is not zero never becomes zero: the
 // smallest code stands in, so m / r stays bounded where a block holds very different gradients.
 //
+// A moving average changes by a few percent a step, or by a thousandth, and neighbouring codes are 6 to 12 percent apart: rounded
+// to nearest it would stand still (the second moment never decays at b2 >= 0.95, and hardly grows at 0.999).  So a value becomes
+// one of its two neighbouring codes lo < hi, at random, and its expectation stays what it was: m the upper one with probability
+// (m - lo) / (hi - lo), the root with (v - lo^2) / (hi^2 - lo^2), which keeps the expectation of v (that of r would add the
+// variance of every rounding to v).  A parameter's first step rounds to nearest: nothing has gone before it that a rounding could
+// hold fast, and the error is half as large where the bias correction weighs it most.  The random numbers are a hash of the step
+// number and the value's place, so that runs repeat.
+//
 // The moments are rounded to 32 bits operation by operation (no contraction), in the order written above: the codes do not
 // depend on what the compiler fuses.  The root is a reciprocal root with one Newton step, whose remainder is exact (the rounded
 // root but for one value in a million); the quotient m / (...) is off by two steps of its own at most, a fraction of a step of p.
@@ -49,6 +57,8 @@ struct Table {
 };
 struct Hyper {
   float b1, omb1, b2, omb2, decay, step, inv_root, eps;
+  uint32_t key;    // stands for the step number in the noise of the codes' rounding
+  int noisy;       // 0: codes are rounded to nearest
   float one;   // 1, unknown to the compiler: a packed product and sum would be contracted, and ties between two codes go the
 };             // other way then; a fused operation with it is a plain sum
 
@@ -120,6 +130,65 @@ __device__ __forceinline__ void store_all(float* p, const float2 (&a)[4]) {
 __device__ __forceinline__ void store_all(__nv_bfloat16* p, const float2 (&a)[4]) {
   __stcs(reinterpret_cast<uint4*>(p), make_uint4(mb::pack_bf16(a[0].x, a[0].y), mb::pack_bf16(a[1].x, a[1].y),
                                                  mb::pack_bf16(a[2].x, a[2].y), mb::pack_bf16(a[3].x, a[3].y)));
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// ---- noise: 32 random bits for each of the 8 values of a lane, a hash of their group's place and a linear congruence after it.
+// The upper 23 bits round the root, the lower 20 the first moment (what they share weighs 2^-13 and less in the root's).
+__device__ __forceinline__ uint32_t first_noise(uint32_t group, uint32_t key) {
+  uint32_t x = group * 0x9E3779B9u + key;
+  x = (x ^ (x >> 16)) * 0xB7E15163u;
+  x = (x ^ (x >> 15)) * 0x6A09E667u;
+  return x ^ (x >> 16);
+}
+__device__ __forceinline__ uint32_t next_noise(uint32_t x) { return x * 0x6A09E667u + 0xBB67AE85u; }
+__device__ __forceinline__ uint32_t bits_of(uint32_t x) { return x ^ (x >> 16); }
+__device__ __forceinline__ float one_plus(uint32_t bits) { return __uint_as_float(0x3f800000u | (bits >> 9)); }
+
+constexpr float NORMAL = 0.015625f;   // 2^-6: below it codes keep the distance 2^-9
+// the largest code that is at most a in [0, 448], after `add` units of 2^-20 of a code's last place; its distance to the next
+__device__ __forceinline__ float code_below(float a, uint32_t add, float& gap) {
+  const float low = a < NORMAL ? NORMAL : 0.f;
+  const uint32_t z = (__float_as_uint(__fadd_rn(a, low)) + add) & 0xfff00000u;
+  gap = __uint_as_float(z & 0x7f800000u) * 0.125f;
+  return __uint_as_float(z) - low;
+}
+// m / 2^k, and the root y of w (both in their units), as one of the two neighbouring codes; NaN stays
+__device__ __forceinline__ float round_noisy(float y, uint32_t bits) {
+  float gap;
+  const float r = copysignf(code_below(fabsf(y), bits & 0xfffffu, gap), y);
+  return y == y ? r : y;
+}
+__device__ __forceinline__ float round_root_noisy(float y, float w, uint32_t bits, float one) {
+  float gap;
+  const float lo = code_below(y, 0u, gap), q = gap * (2.f * lo + gap);            // hi^2 - lo^2: exact, as all is here but u q
+  const float t = __fmaf_rn(__fmul_rn(one_plus(bits), q), one, fmaf(lo, lo, -q));   // lo^2 + u q
+  float r = w > t ? lo + gap : lo;
+  if (y > 0.f) r = fmaxf(r, 0.001953125f);
+  return y == y ? r : y;
+}
+// the same for eight values that are no smaller than NORMAL
+__device__ __forceinline__ void round_all(float2 (&m)[4], float2 (&r)[4], const float2 (&w)[4], uint32_t x, float one) {
+  const float2 one2 = make_float2(one, one), two = make_float2(2.f, 2.f);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t a = bits_of(x), b = bits_of(x = next_noise(x));
+    x = next_noise(x);
+    m[j].x = __uint_as_float((__float_as_uint(m[j].x) + (a & 0xfffffu)) & 0xfff00000u);
+    m[j].y = __uint_as_float((__float_as_uint(m[j].y) + (b & 0xfffffu)) & 0xfff00000u);
+    const uint32_t lx = __float_as_uint(r[j].x) & 0xfff00000u, ly = __float_as_uint(r[j].y) & 0xfff00000u;
+    const float2 lo = make_float2(__uint_as_float(lx), __uint_as_float(ly));
+    const float2 gap = mul2(make_float2(__uint_as_float(lx & 0x7f800000u), __uint_as_float(ly & 0x7f800000u)), 0.125f);
+    const float2 q = mul2(gap, fma2(lo, two, gap));
+    const float2 t = fma2(mul2(make_float2(one_plus(a), one_plus(b)), q), one2, fma2(lo, lo, make_float2(-q.x, -q.y)));
+    const float2 hi = fma2(lo, one2, gap);
+    r[j] = make_float2(w[j].x > t.x ? hi.x : lo.x, w[j].y > t.y ? hi.y : lo.y);
+  }
 }
 
 struct States {
@@ -201,14 +270,18 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
       v[j] = mul2(r, r);
     }
   }
-  float am = 0.f, av = 0.f, least = INFINITY;     // over what is not NaN
+  float am = 0.f, av = 0.f;                       // NaN if there is one
+  float least = INFINITY, least_m = INFINITY;     // over what is not NaN
   const float2 one = make_float2(h.one, h.one);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     m[j] = fma2(mul2(m[j], h.b1), one, mul2(d[j], h.omb1));
     v[j] = fma2(mul2(v[j], h.b2), one, mul2(mul2(d[j], d[j]), h.omb2));
-    if (EIGHT) am = fmaxf(fmaxf(am, fabsf(m[j].x)), fabsf(m[j].y));
-    av = fmaxf(fmaxf(av, v[j].x), v[j].y);
+    if (EIGHT) {
+      am = max_nan(max_nan(am, fabsf(m[j].x)), fabsf(m[j].y));
+      least_m = fminf(fminf(least_m, fabsf(m[j].x)), fabsf(m[j].y));
+    }
+    av = max_nan(max_nan(av, v[j].x), v[j].y);
     least = fminf(fminf(least, v[j].x), v[j].y);
   }
   if (!EIGHT) {
@@ -220,6 +293,9 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
       store_some(st.v32 + s0 + e, n - e, v);
     }
   }
+  float2 w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = v[j];
   if (least >= ROOT_FROM && av < ROOT_TO) {      // v becomes its root (NaN stays)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = root2(v[j]);
@@ -245,7 +321,8 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
     uint32_t bm = __float_as_uint(am), br = __float_as_uint(av);
     bm = __reduce_max_sync(~0u, bm);
     br = __reduce_max_sync(~0u, br);
-    if (bm >= 0x7f800000u || br >= 0x7f800000u) {   // an infinity: it becomes the NaN code and sets no scale
+    const bool odd = bm >= 0x7f800000u || br >= 0x7f800000u;
+    if (odd) {               // an infinity becomes the NaN code; neither it nor NaN sets a scale
       bm = br = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -271,8 +348,25 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
       m[j] = mul2(m[j], im);
       v[j] = mul2(v[j], ir);
     }
-    // a lane whose smallest root is at least the smallest code has nothing to lift (the margin covers the roots' roundings)
-    if (!(least * (ir * ir) >= 3.9e-6f)) {
+    if (h.noisy) {
+      const uint32_t x = first_noise(static_cast<uint32_t>((s0 >> 3) + lane), h.key);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = mul2(w[j], ir * ir);
+      // (a whole warp goes one way; the margin over 2^-12 covers the roots' roundings)
+      if (!__any_sync(~0u, odd || !(least * (ir * ir) >= 2.45e-4f && least_m * im >= NORMAL))) {
+        round_all(m, v, w, x, h.one);
+      } else {
+        uint32_t y = x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a = bits_of(y), b = bits_of(y = next_noise(y));
+          y = next_noise(y);
+          m[j] = make_float2(round_noisy(m[j].x, a), round_noisy(m[j].y, b));
+          v[j] = make_float2(round_root_noisy(v[j].x, w[j].x, a, h.one), round_root_noisy(v[j].y, w[j].y, b, h.one));
+        }
+      }
+    } else if (!(least * (ir * ir) >= 3.9e-6f)) {
+      // (a lane whose smallest root is at least the smallest code has nothing to lift; the margin covers the roots' roundings)
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = make_float2(floored(v[j].x), floored(v[j].y));
     }
@@ -362,14 +456,17 @@ int launch(const Tensor* rows, int& at, int count, bool bf16, bool eight, const 
 
 // tensors: host array of `count` rows (struct Tensor above), all of one type: 32-bit (p_bf16 = 0) or bf16 values with
 // gradients of the same type.  bits 8: m, m_exp, r, r_exp; bits 32: m, r hold fp32 moments and the exponents are null.
-// hyper: 8 host floats in the order of struct Hyper.
+// hyper: 8 host floats in the order of struct Hyper.  key: 32 bits that stand for the step number in the noise of the codes'
+// rounding; negative: they are rounded to nearest.
 extern "C" int mb_adamw_multi(const void* tensors, int count, int p_bf16, int bits, void* m, void* m_exp, void* r,
-                              void* r_exp, const float* hyper, cudaStream_t stream) {
+                              void* r_exp, const float* hyper, long long key, cudaStream_t stream) {
   if (count < 0 || (bits != 8 && bits != 32)) return -3;
   const Tensor* rows = static_cast<const Tensor*>(tensors);
   Hyper h;
   h.b1 = hyper[0]; h.omb1 = hyper[1]; h.b2 = hyper[2]; h.omb2 = hyper[3];
   h.decay = hyper[4]; h.step = hyper[5]; h.inv_root = hyper[6]; h.eps = hyper[7];
+  h.key = static_cast<uint32_t>(key);
+  h.noisy = key >= 0;
   h.one = 1.f;
   const States st{static_cast<uint8_t*>(m), static_cast<uint8_t*>(m_exp), static_cast<uint8_t*>(r), static_cast<uint8_t*>(r_exp),
                   static_cast<float*>(m), static_cast<float*>(r)};

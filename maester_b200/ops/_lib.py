@@ -159,7 +159,7 @@ def _declare(l: ctypes.CDLL) -> None:
         "mb_ce_grad": [_P, _P, _P, _I, _P, _P, _L, _I, _L, _L, _I, _I, _P],
         "mb_expect_scalar": [_P, _F, _P],
         "mb_adamw": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _F, _F, _F, _F, _F, _F, _I, _P],
-        "mb_adamw_multi": [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P],
+        "mb_adamw_multi": [_P, _I, _I, _I, _P, _P, _P, _P, _P, _L, _P],
         "mb_logprobs_fwd": [_P, _P, _I, _I, _I, _L, _F, _P, _P, _I, _P, _P, _P, _P],
         "mb_logprobs_bwd": [_P, _P, _I, _I, _I, _L, _F, _P, _P, _P, _I, _P, _P, _P, _I, _L, _P],
         "mb_fp8_quantize": [_P, _I, _I, _I, _L, _I, _P, _P, _P, _P, _P],

@@ -869,10 +869,11 @@ ADAMW_ROW = 48   # bytes of one row of the tensor table: p, g, copy, n, off (8 b
 
 
 def adamw_multi(table, bf16: bool, bits: int, m: torch.Tensor, m_exp: torch.Tensor | None, r: torch.Tensor,
-                r_exp: torch.Tensor | None, hyper: tuple) -> None:
-    """``table``: int64 numpy array [n, 6] of (parameter, gradient, copy, elements, state offset, 0)."""
+                r_exp: torch.Tensor | None, hyper: tuple, noise_key: int = -1) -> None:
+    """``table``: int64 numpy array [n, 6] of (parameter, gradient, copy, elements, state offset, 0); ``noise_key``
+    (``reference.state_noise_key``): 8-bit codes are rounded stochastically, -1: to nearest."""
     assert table.flags.c_contiguous and table.itemsize * table.shape[1] == ADAMW_ROW
     h = (ctypes.c_float * 8)(*hyper)
     with on_device(m):
         _ck(_lib.lib().mb_adamw_multi(table.ctypes.data, table.shape[0], int(bf16), bits, m.data_ptr(), _ptr(m_exp),
-                                      r.data_ptr(), _ptr(r_exp), h, _stream_of(m)), "adamw_multi")
+                                      r.data_ptr(), _ptr(r_exp), h, noise_key, _stream_of(m)), "adamw_multi")

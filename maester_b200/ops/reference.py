@@ -276,13 +276,71 @@ STATE_BLOCK = 256        # values of an optimizer state that share a scale
 STATE_MIN_EXP, ROOT_MIN_EXP = -117, -54   # (the square of the smallest root code is still a normal number)
 
 
-def state_encode(x: torch.Tensor, root: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+def _mix32(x: int) -> int:
+    for shift, factor in ((16, 0x9E3779B9), (15, 0xB7E15163), (16, 1)):    # (digits of the golden ratio and of e)
+        x = (x ^ (x >> shift)) * factor & 0xFFFFFFFF
+    return x
+
+
+def state_noise_key(step: int) -> int:
+    """32 bits that stand for a step number."""
+    return _mix32(_mix32(step & 0xFFFFFFFF) + 0x6A09E667 & 0xFFFFFFFF)
+
+
+def state_noise(step: int, first: int, n: int, device=None) -> torch.Tensor:
+    """32 random bits (int64) for values ``first`` .. ``first + n - 1`` of the flat states in a step: a hash of the step and
+    of the value's group of 8, and a linear congruence along the group."""
+    m32 = 0xFFFFFFFF
+    i = torch.arange(first, first + n, dtype=torch.int64, device=device)
+    x = (i >> 3) * 0x9E3779B9 + state_noise_key(step) & m32
+    for shift, factor in ((16, 0xB7E15163), (15, 0x6A09E667), (16, 1)):
+        x = (x ^ (x >> shift)) * factor & m32
+    out = x
+    for j in range(1, 8):
+        x = x * 0x6A09E667 + 0xBB67AE85 & m32
+        out = torch.where(i & 7 == j, x, out)
+    return out ^ (out >> 16)
+
+
+def _code_below(a: torch.Tensor, add) -> tuple[torch.Tensor, torch.Tensor]:
+    """(the largest code that is at most ``a`` in [0, 448], the distance to the next one); with ``add`` in [0, 2^20) the bits
+    below a code's last place are added up first, in units of 2^-20 of that distance."""
+    low = torch.where(a < 2.0 ** -6, torch.full_like(a, 2.0 ** -6), torch.zeros_like(a))     # below it codes keep one distance
+    z = ((a + low).view(torch.int32) + add) & -(1 << 20)
+    z, gap = z.view(torch.float32), (z & 0x7F800000).view(torch.float32) * 0.125
+    return z - low, gap
+
+
+def state_round(y: torch.Tensor, noise: torch.Tensor) -> torch.Tensor:
+    """Values in [-448, 448] rounded to one of their two neighbouring codes, so that the expectation is the value."""
+    a, _ = _code_below(y.abs(), (noise & 0xFFFFF).to(torch.int32))
+    return torch.where(y.isnan(), y, torch.copysign(a, y))
+
+
+def state_round_root(y: torch.Tensor, w: torch.Tensor, noise: torch.Tensor) -> torch.Tensor:
+    """The root ``y`` of ``w`` rounded to one of its two neighbouring codes, so that the expectation of its SQUARE is ``w``;
+    what is not zero does not become zero."""
+    lo, gap = _code_below(y, 0)
+    u1 = ((noise >> 9).to(torch.int32) | 0x3F800000).view(torch.float32)        # 1 + u
+    q = gap * (2 * lo + gap)                                                      # hi^2 - lo^2
+    out = torch.where(w > u1 * q + (lo * lo - q), lo + gap, lo)
+    out = torch.where(y > 0, out.clamp_min(E4M3_TINY), out)
+    return torch.where(y.isnan(), y, out)
+
+
+def state_encode(x: torch.Tensor, root: bool = False, noise: torch.Tensor | None = None,
+                 square: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes and biased block exponents of a flat state whose length is a multiple of 256; ``root``: a value that is not
-    zero does not become zero."""
+    zero does not become zero.  Rounded to nearest, or with ``noise`` (``state_noise``) to a neighbour whose expectation is
+    the value, for a root (of ``square``) in the squares.  What is a code already stays one."""
     b = x.view(-1, STATE_BLOCK)
     k = fp8_block_exponents(_finite_abs(b).amax(dim=1), ROOT_MIN_EXP if root else STATE_MIN_EXP)
     y = b * pow2(-k)[:, None]
-    if root:
+    if noise is not None:
+        y = torch.where(y.isinf(), torch.full_like(y, math.nan), y)
+        n = noise.view(-1, STATE_BLOCK)
+        y = state_round_root(y, square.view(-1, STATE_BLOCK) * pow2(-2 * k)[:, None], n) if root else state_round(y, n)
+    elif root:
         y = torch.where(y > 0, y.clamp_min(E4M3_TINY), y)
     return y.to(torch.float8_e4m3fn).view(-1), (k + 127).to(torch.uint8)
 

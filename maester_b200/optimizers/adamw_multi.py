@@ -2,7 +2,10 @@
 
 The parameters may lie anywhere (they need no common buffer) and be fp32 or bf16.  The moments of all of them live in flat
 buffers, every tensor's on a multiple of 256 values.  With 8 bits the first moment and the ROOT of the second are e4m3
-codes with one power-of-two scale for every 256 values: 2.008 bytes a parameter instead of 8.  Checkpoints hold the
+codes with one power-of-two scale for every 256 values: 2.008 bytes a parameter instead of 8.  An average that moves by
+less than half a code a step would stand still if it were rounded to nearest, so from a parameter's second step on a value
+becomes one of its two neighbouring codes at random, with itself (for the root, its square) as the expectation; the random
+numbers are a hash of the step number and the place, so a run repeats, also one that was saved and loaded.  Checkpoints hold the
 moments as fp32 ``exp_avg`` and ``exp_avg_sq``, the names and shapes that ``FusedAdamW`` and ``torch.optim.AdamW`` write, so
 a run may change between them; encoding what was decoded gives the same values, so saving and loading changes nothing.
 Update rule and defaults: torch.optim.AdamW, as configured in maester/config.py:147-154.
@@ -19,6 +22,7 @@ from torch.optim import Optimizer
 from maester_b200.ops import reference as ref
 
 _TYPES = (torch.float32, torch.bfloat16)
+NOISE_FROM = 2      # step number of a parameter from which its 8-bit codes are rounded stochastically
 # a step looks at every tensor: mapped over the lists, which takes half the time of a loop
 _grad, _dtype = map(operator.attrgetter, ("grad", "dtype"))
 _device, _numel, _contiguous, _address = (torch.Tensor.get_device, torch.Tensor.numel, torch.Tensor.is_contiguous,
@@ -249,10 +253,11 @@ class AdamWMulti(Optimizer):
         from maester_b200.ops import cuda as C
         table = batch.table if len(slots) == len(batch.slots) else batch.table[[s.row for s in slots]]
         table[:, 1] = list(map(_address, grads))
-        f = self._buffers
+        f, step = self._buffers, slots[0].step + 1
+        key = ref.state_noise_key(step) if self.state_bits == 8 and step >= NOISE_FROM else -1
         C.adamw_multi(table, batch.dtype is torch.bfloat16, self.state_bits, f["exp_avg"], f.get("exp_avg_exp"),
                       f["exp_avg_root" if self.state_bits == 8 else "exp_avg_sq"], f.get("exp_avg_root_exp"),
-                      (h["b1"], 1 - h["b1"], h["b2"], 1 - h["b2"], h["decay"], h["step_size"], h["inv_root"], h["eps"]))
+                      (h["b1"], 1 - h["b1"], h["b2"], 1 - h["b2"], h["decay"], h["step_size"], h["inv_root"], h["eps"]), key)
 
     def _plain(self, batch, slots, grads, h) -> None:
         for s, g in zip(slots, grads):
@@ -262,7 +267,7 @@ class AdamWMulti(Optimizer):
             p.copy_(new.view(p.shape))
             if batch.table[s.row, 2]:
                 s.copy.view(-1).copy_(p.view(-1))
-            self._store(p, m, root, v)
+            self._store(p, m, root, v, s.step + 1)
 
     # ---- states
     def _moments(self, p) -> tuple[torch.Tensor, torch.Tensor]:
@@ -276,7 +281,8 @@ class AdamWMulti(Optimizer):
         m, r = (ref.state_decode(f[k][off:end], f[k + "_exp"][blk])[:n] for k in ("exp_avg", "exp_avg_root"))
         return m, r * r
 
-    def _store(self, p, m=None, root=None, v=None) -> None:
+    def _store(self, p, m=None, root=None, v=None, step: int = 1) -> None:
+        """Take over moments: as they are, or as codes, rounded as in step number ``step``."""
         off, n = self._slots[p].offset, self._slots[p].numel
         f = self._buffers
         if n == 0:
@@ -291,9 +297,11 @@ class AdamWMulti(Optimizer):
         blk = slice(off // ref.STATE_BLOCK, end // ref.STATE_BLOCK)
         if root is None and v is not None:
             root = v.sqrt()
-        for k, x, is_root in (("exp_avg", m, False), ("exp_avg_root", root, True)):
+        noise = None if step < NOISE_FROM else ref.state_noise(step, off, end - off, self.device)
+        padded = lambda x: None if x is None else torch.nn.functional.pad(x, (0, end - off - n))
+        for k, x, square in (("exp_avg", m, None), ("exp_avg_root", root, v)):
             if x is not None:
-                codes, exps = ref.state_encode(torch.nn.functional.pad(x, (0, end - off - n)), is_root)
+                codes, exps = ref.state_encode(padded(x), square is not None, noise, padded(square))
                 f[k][off:end].copy_(codes)
                 f[k + "_exp"][blk].copy_(exps)
 
