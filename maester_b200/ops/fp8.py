@@ -17,6 +17,7 @@ import math
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from maester_b200.ops import reference as ref
 from maester_b200.ops.functional import _C
@@ -131,7 +132,9 @@ def matmul_fp8(a: Fp8Blocks, b: Fp8Blocks, *, out_dtype: torch.dtype = torch.bfl
     elif out.dtype not in _TYPES or (accumulate and out.dtype != torch.float32):
         raise TypeError(f"out is {out.dtype}: bf16 or fp32 is wanted, fp32 to accumulate")
     if out.is_cuda:
-        return _C().fp8_gemm(a.data, a.scales, b.data, b.scales, out, accumulate)
+        _C().fp8_gemm(a.data, a.scales, b.data, b.scales, out, accumulate)
+        increment_version(out)
+        return out
     value = a.dequantize() @ b.dequantize().T
     return out.add_(value) if accumulate else out.copy_(value)
 

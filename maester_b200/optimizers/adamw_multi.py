@@ -17,6 +17,7 @@ import operator
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 from torch.optim import Optimizer
 
 from maester_b200.ops import reference as ref
@@ -258,6 +259,10 @@ class AdamWMulti(Optimizer):
         C.adamw_multi(table, batch.dtype is torch.bfloat16, self.state_bits, f["exp_avg"], f.get("exp_avg_exp"),
                       f["exp_avg_root" if self.state_bits == 8 else "exp_avg_sq"], f.get("exp_avg_root_exp"),
                       (h["b1"], 1 - h["b1"], h["b2"], 1 - h["b2"], h["decay"], h["step_size"], h["inv_root"], h["eps"]), key)
+        # (a backward pass through a graph of before this step is an error, as after torch's own optimizers)
+        increment_version([x.param for x in slots])
+        if self._copy_storages:
+            increment_version([x.copy for x in slots if x.copy is not None])
 
     def _plain(self, batch, slots, grads, h) -> None:
         for s, g in zip(slots, grads):
