@@ -316,17 +316,18 @@ class AdamWMulti(Optimizer):
         return {"step": torch.tensor(float(self._slots[p].step)), "exp_avg": m.clone().view(p.shape),
                 "exp_avg_sq": v.clone().view(p.shape)}
 
+    @staticmethod
+    def _fits(p, state: dict) -> None:
+        for k in ("exp_avg", "exp_avg_sq"):
+            if k in state and state[k].numel() != p.numel():
+                raise ValueError(f"{k} of {state[k].numel()} elements for a parameter of {p.numel()}")
+
     @torch.no_grad()
     def load_param_state(self, p, state: dict) -> None:
         """Take over any of ``step``, ``exp_avg``, ``exp_avg_sq`` of one parameter."""
-        n = p.numel()
-        flat = {}
-        for k in ("exp_avg", "exp_avg_sq"):
-            if k in state:
-                x = state[k]
-                if x.numel() != n:
-                    raise ValueError(f"{k} of {x.numel()} elements for a parameter of {n}")
-                flat[k] = x.detach().to(device=self.device, dtype=torch.float32).reshape(-1)
+        self._fits(p, state)
+        flat = {k: state[k].detach().to(device=self.device, dtype=torch.float32).reshape(-1)
+                for k in ("exp_avg", "exp_avg_sq") if k in state}
         self._store(p, m=flat.get("exp_avg"), v=flat.get("exp_avg_sq"))
         if "step" in state:
             self._slots[p].step = int(state["step"])
@@ -337,7 +338,16 @@ class AdamWMulti(Optimizer):
         return sd
 
     def load_state_dict(self, state_dict: dict) -> None:
+        """Moments and step numbers become those of ``state_dict``; a parameter, or a part of its state, that is not in it
+        starts afresh."""
+        every = [p for g in self.param_groups for p in g["params"]]
+        states = [state_dict["state"].get(i, {}) for i in range(len(every))]
+        for p, state in zip(every, states):
+            self._fits(p, state)
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        for i, p in enumerate(p for g in self.param_groups for p in g["params"]):
-            if i in state_dict["state"]:
-                self.load_param_state(p, state_dict["state"][i])
+        for k, x in self._buffers.items():
+            x.view(torch.uint8).fill_(0 if not k.endswith("_exp") else
+                                      127 + (ref.ROOT_MIN_EXP if "root" in k else ref.STATE_MIN_EXP))
+        for p, state in zip(every, states):
+            self._slots[p].step = 0
+            self.load_param_state(p, state)
