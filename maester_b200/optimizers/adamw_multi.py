@@ -70,7 +70,10 @@ class AdamWMulti(Optimizer):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits has to be 8 or 32, got {state_bits!r}")
         self._sealed = False
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        # (the rest is what torch.optim.AdamW keeps in its groups: a checkpoint's reader asks for every key that it has itself)
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, amsgrad=False, maximize=False,
+                                      foreach=None, capturable=False, differentiable=False, fused=True,
+                                      decoupled_weight_decay=True))
         for g in self.param_groups:
             b1, b2 = g["betas"]
             if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and g["eps"] >= 0.0 and g["weight_decay"] >= 0.0 and g["lr"] >= 0.0):
@@ -182,6 +185,9 @@ class AdamWMulti(Optimizer):
                 loss = closure()
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamWMulti.step() cannot be captured: learning rate and step number are launch arguments")
+        for key in ("amsgrad", "maximize"):         # (another optimizer's settings may have been loaded)
+            if any(g.get(key) for g in self.param_groups):
+                raise RuntimeError(f"AdamWMulti has no {key}")
         self._find_parameters()
         self._find_copies()
         work = []                                   # (everything is looked at before anything runs)
