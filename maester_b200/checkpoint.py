@@ -84,8 +84,26 @@ def _as_dtensor(local: torch.Tensor, slot, sharded) -> torch.Tensor:
             return local
         placements = [Shard(0)]
     shape = slot.global_shape
+    if not _on_mesh_device(local, mesh):
+        return _as_host_piece(local, mesh, placements, shape)
     stride = torch.empty(shape, device="meta").stride()
     return DTensor.from_local(local, mesh, placements, run_check=False, shape=shape, stride=stride)
+
+
+def _on_mesh_device(local: torch.Tensor, mesh) -> bool:
+    return local.device.type == mesh.device_type
+
+
+def _as_host_piece(local: torch.Tensor, mesh, placements, shape) -> torch.Tensor:
+    """This rank's piece of a parameter's state that is held on the host (a DTensor over a GPU mesh would be a copy of it
+    there): the tensor itself, with DCP's checkpointable hooks that say where it belongs."""
+    from torch.distributed.tensor._utils import compute_local_shape_and_global_offset
+
+    sizes, offsets = compute_local_shape_and_global_offset(shape, mesh, placements)
+    piece = local.view(sizes)
+    t = _with_chunks(piece, {torch.Size(offsets): piece} if piece.numel() else {}, shape)
+    t._mb_rewrap = lambda new_local: _as_host_piece(new_local, mesh, placements, shape)
+    return t
 
 
 def row_pieces(slot, own_lo: int, own_hi: int) -> list[tuple[int, int, int]]:
@@ -106,22 +124,27 @@ def _as_row_pieces(local: torch.Tensor, slot, sharded) -> torch.Tensor:
     place in the whole tensor (the reference's row order), so that the checkpoint holds the tensor exactly as an
     unsharded model has it and any other layout can load it.  DTensor cannot describe this (one contiguous range per
     rank), so the tensor carries DCP's checkpointable hooks itself: one write / read item per piece."""
-    from torch.distributed.checkpoint.metadata import ChunkStorageMetadata, MetadataIndex, TensorProperties
-    from torch.distributed.checkpoint.planner import TensorWriteData, WriteItem, WriteItemType
-
     lo, hi = sharded._own_rows(slot)
     cols = tuple(slot.shape[1:])
     rows2d = local.reshape(-1, *cols)[: hi - lo] if hi > lo else local.reshape(-1, *cols)[:0]
-    pieces = row_pieces(slot, lo, hi)
-    size = slot.global_shape
     zeros = (0,) * len(cols)
-    t = rows2d.view(rows2d.shape)          # a fresh tensor object over the same memory to carry the hooks
-    chunks = [ChunkStorageMetadata(offsets=torch.Size((g0, *zeros)), sizes=torch.Size((n, *cols))) for _, g0, n in pieces]
-    views = {c.offsets: rows2d[l0: l0 + n] for c, (l0, _, n) in zip(chunks, pieces)}
+    views = {torch.Size((g0, *zeros)): rows2d[l0: l0 + n] for l0, g0, n in row_pieces(slot, lo, hi)}
+    t = _with_chunks(rows2d, views, slot.global_shape)
+    t._mb_rewrap = lambda new_local: _as_row_pieces(new_local, slot, sharded)   # after a dtype conversion
+    return t
+
+
+def _with_chunks(local: torch.Tensor, views: dict, size) -> torch.Tensor:
+    """``local`` with DCP's checkpointable hooks: ``views`` {offset in the whole tensor of ``size``: part of ``local``}."""
+    from torch.distributed.checkpoint.metadata import ChunkStorageMetadata, MetadataIndex, TensorProperties
+    from torch.distributed.checkpoint.planner import TensorWriteData, WriteItem, WriteItemType
+
+    t = local.view(local.shape)            # a fresh tensor object over the same memory to carry the hooks
+    chunks = [ChunkStorageMetadata(offsets=o, sizes=v.shape) for o, v in views.items()]
 
     def create_write_items(fqn, obj):
         return [WriteItem(index=MetadataIndex(fqn, c.offsets), type=WriteItemType.SHARD,
-                          tensor_data=TensorWriteData(chunk=c, properties=TensorProperties.create_from_tensor(rows2d),
+                          tensor_data=TensorWriteData(chunk=c, properties=TensorProperties.create_from_tensor(local),
                                                       size=size)) for c in chunks]
 
     def get_tensor_shard(index):
@@ -132,7 +155,6 @@ def _as_row_pieces(local: torch.Tensor, slot, sharded) -> torch.Tensor:
     t.__get_tensor_shard__ = get_tensor_shard
     # the load planner compares ``obj.size()`` with the stored (whole) size before it asks for the chunk list
     t.size = lambda *dim: size if not dim else size[dim[0]]
-    t._mb_rewrap = lambda new_local: _as_row_pieces(new_local, slot, sharded)   # after a dtype conversion
     return t
 
 

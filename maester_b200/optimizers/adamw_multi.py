@@ -317,10 +317,10 @@ class AdamWMulti(Optimizer):
                 f[k + "_exp"][blk].copy_(exps)
 
     def param_state(self, p) -> dict[str, torch.Tensor]:
-        """What a checkpoint holds of one parameter: ``step``, and fp32 ``exp_avg`` and ``exp_avg_sq`` of its shape."""
-        m, v = self._moments(p)
-        return {"step": torch.tensor(float(self._slots[p].step)), "exp_avg": m.clone().view(p.shape),
-                "exp_avg_sq": v.clone().view(p.shape)}
+        """What a checkpoint holds of one parameter: ``step``, and fp32 ``exp_avg`` and ``exp_avg_sq`` of its shape, on the
+        host (on the device those of all parameters would take four times the memory of 8-bit states)."""
+        m, v = (x.to("cpu", copy=True).view(p.shape) for x in self._moments(p))
+        return {"step": torch.tensor(float(self._slots[p].step)), "exp_avg": m, "exp_avg_sq": v}
 
     @staticmethod
     def _fits(p, state: dict) -> None:
