@@ -193,7 +193,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, scale: flo
     scored = torch.ones(x.shape[0], dtype=torch.bool, device=x.device) if tokens is None else tokens != IGNORE_INDEX
     if tokens is not None and bool((scored & ((tokens < 0) | (tokens >= V))).any()):
         raise ValueError(f"token ids have to be in [0, {V}) or {IGNORE_INDEX}")
-    logp = torch.log_softmax(x * scale, dim=-1)
+    if tokens is not None:     # (a row that is not scored may have no distribution: its gradient is 0 all the same)
+        x = torch.where(scored[:, None], x, torch.zeros_like(x))
+    m = x.detach().amax(dim=-1, keepdim=True)      # taken off before the scale: logits of the lowest value do not overflow
+    logp = torch.log_softmax((x - torch.where(m.isfinite(), m, torch.zeros_like(m))) * scale, dim=-1)
     lp = ent = top_lp = top_id = None
     if tokens is not None:
         at = torch.where(scored, tokens, torch.zeros_like(tokens))
