@@ -169,16 +169,78 @@ class _LinearLogprobs(Function):
         return dh, dw, None, None, None, None
 
 
+class _PlainLinearLogprobs(Function):
+    """The same off the native products' path (other types than bf16, odd widths, the CPU): logits are a plain product in 32
+    bits (64 where either operand has them), a chunk of rows at a time, formed again in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, h, w, tokens, scale, entropy, top):
+        ctx.wide = torch.float64 if torch.float64 in (h.dtype, w.dtype) else torch.float32
+        ctx.args = scale, entropy, top
+        ctx.save_for_backward(h, w, tokens)
+        wt = w.to(ctx.wide).T
+        parts = []
+        for r0, r1 in _chunks(h.shape[0], w.shape[0]):
+            t = None if tokens is None else tokens[r0:r1]
+            parts.append(_of_logits(_product(h[r0:r1].to(ctx.wide), wt), t, scale, entropy, top))
+        out = tuple(None if c[0] is None else c[0] if len(c) == 1 else torch.cat(c) for c in zip(*parts))
+        if out[3] is not None:
+            ctx.mark_non_differentiable(out[3])
+        ctx.set_materialize_grads(False)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        h, w, tokens = ctx.saved_tensors
+        grads = grads[:3]
+        if all(g is None for g in grads):
+            return (None,) * 6
+        ww = w.to(ctx.wide)
+        dh = torch.empty(h.shape, device=h.device, dtype=h.dtype) if ctx.needs_input_grad[0] else None
+        mg = getattr(w, "main_grad", None)
+        dw = None
+        if ctx.needs_input_grad[1]:
+            dw = mg if mg is not None else torch.zeros(w.shape, device=w.device, dtype=ctx.wide)
+        for r0, r1 in _chunks(h.shape[0], w.shape[0]):
+            hh = h[r0:r1].to(ctx.wide)
+            logits = _product(hh, ww.T).detach().requires_grad_(True)
+            with torch.enable_grad():
+                out = _of_logits(logits, None if tokens is None else tokens[r0:r1], *ctx.args)
+            some = [(o, g[r0:r1]) for o, g in zip(out[:3], grads) if g is not None]
+            dl, = torch.autograd.grad([o for o, _ in some], [logits], [g for _, g in some])
+            if dh is not None:
+                dh[r0:r1] = _product(dl, ww)
+            if dw is not None:
+                dw.add_(_product(dl.T, hh))
+        return dh, None if dw is None or mg is not None else dw.to(w.dtype), None, None, None, None
+
+
+def _product(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    with torch.autocast(a.device.type, enabled=False):      # (in the operands' own type)
+        return a @ b
+
+
+def _of_logits(logits, tokens, scale, entropy, top):
+    """(log-probabilities, entropies, alternatives', their ids) of a matrix of logits, by kernel where there is one."""
+    if logits.is_cuda and logits.dtype in _NATIVE:
+        return tuple(token_logprobs(logits, tokens, scale=scale, entropy=entropy, top=top))
+    return ref.token_logprobs(logits, tokens, scale, entropy, top)
+
+
 def _chunks(rows: int, V: int) -> list[tuple[int, int]]:
     step = max(128, CHUNK_BYTES // (4 * V) // 128 * 128)
-    return [(r0, min(rows, r0 + step)) for r0 in range(0, rows, step)]
+    return [(r0, min(rows, r0 + step)) for r0 in range(0, rows, step)] or [(0, 0)]
 
 
 def linear_logprobs(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor | None = None, *, logit_scale: float = 1.0,
                     entropy: bool = False, top: int = 0) -> TokenLogprobs:
     """``token_logprobs`` of the logits ``h @ w.T * logit_scale`` for hidden states ``h`` [..., D] and an output weight
     ``w`` [V, D], with gradients to both (into ``w.main_grad`` where there is one).  Logits are fp32 and live one chunk of
-    rows at a time."""
+    rows at a time, whatever the types of ``h`` and ``w``; bf16 with a width that 8 divides runs in the framework's own
+    products, the rest in plain ones (and 64-bit operands in 64 bits)."""
+    if not (h.is_floating_point() and w.is_floating_point()):
+        raise TypeError(f"hidden states and weight have to be floating-point tensors, got {h.dtype} and {w.dtype}")
     if h.dim() < 1 or w.dim() != 2 or h.shape[-1] != w.shape[1]:
         raise ValueError(f"hidden states {tuple(h.shape)} do not fit the weight {tuple(w.shape)}")
     if w.device != h.device:
@@ -194,8 +256,6 @@ def linear_logprobs(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor | Non
         h2, w2 = h2.contiguous(), w if w.is_contiguous() else w.contiguous()
         with _C().on_device(h2):
             out = _LinearLogprobs.apply(h2, w2, t, logit_scale, entropy, top)
-    elif h2.is_cuda and h2.dtype in _NATIVE:
-        return token_logprobs(ref.linear(h, w), tokens, scale=logit_scale, entropy=entropy, top=top)
     else:
-        out = ref.token_logprobs(ref.linear(h2, w), t, logit_scale, entropy, top)
+        out = _PlainLinearLogprobs.apply(h2, w, t, logit_scale, entropy, top)
     return _shaped(out, lead, top)
