@@ -794,11 +794,11 @@ def fp8_gemm(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tenso
     """``out (+)= A @ B.T`` of codes [M, Kp] and [N, Kp] with packed exponents; ``out`` row-major bf16 or fp32."""
     M, N = a.shape[0], b.shape[0]
     _fit(M, N)
-    assert a.shape[1] == b.shape[1] and a.shape[1] % 128 == 0 and out.shape == (M, N) and out.stride(1) == 1
+    assert a.shape[1] == b.shape[1] and a.shape[1] % 128 == 0 and out.shape == (M, N) and (out.stride(1) == 1 or N == 1)
     assert not accumulate or out.dtype == torch.float32
     with on_device(out):
         _ck(_lib.lib().mb_fp8_gemm(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), out.data_ptr(), M, N,
-                                   a.shape[1] // 128, a.stride(0), b.stride(0), out.stride(0),
+                                   a.shape[1] // 128, a.stride(0), b.stride(0), out.stride(0) if M > 1 else N,
                                    FP8_OUT_F32_ACC if accumulate else FP8_OUT[out.dtype], _stream_of(out)), "fp8_gemm")
     return out
 
