@@ -226,12 +226,13 @@ struct Patch<float> {
 
 template <typename T, int MODE>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 4 : MODE == (ROWS | COLS) ? 1 : 2)
-fp8_quantize_kernel(const T* __restrict__ src, int rows, int cols, long long ld, int vec, uint8_t* q, uint8_t* sq, uint8_t* qt,
-                    uint8_t* sqt) {
+fp8_quantize_kernel(const T* __restrict__ src, int rows, int cols, long long ld, int vec, uint32_t across, uint8_t* q, uint8_t* sq,
+                    uint8_t* qt, uint8_t* sqt) {
   __shared__ __align__(16) uint8_t tile[(MODE & COLS) ? B * B : 16];
   __shared__ __align__(16) uint32_t maxima[(MODE & COLS) ? 8 * 128 : 8];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (a kernel that was launched to start beside this one may)
-  const int rt = blockIdx.y, ct = blockIdx.x, tid = threadIdx.x;
+  const int rt = blockIdx.x / across, ct = blockIdx.x % across, tid = threadIdx.x;   // (tiles in one dimension: a second one
+  // ends at 65535 of them, 8.4 million rows)
   const int ctiles = (cols + B - 1) / B, rtiles = (rows + B - 1) / B;
   if (rt >= rtiles || ct >= ctiles) {  // past the matrix: only the padding of the exponent bytes
     if (tid < B) {
@@ -309,11 +310,11 @@ fp8_quantize_kernel(const T* __restrict__ src, int rows, int cols, long long ld,
 }
 
 template <typename T>
-int launch(int mode, dim3 grid, cudaStream_t stream, const void* x, int rows, int cols, long long ld, uint8_t* const* o) {
+int launch(int mode, uint32_t across, uint32_t grid, cudaStream_t stream, const void* x, int rows, int cols, long long ld, uint8_t* const* o) {
   const int vec = !(reinterpret_cast<uintptr_t>(x) & 15) && !((ld * static_cast<int>(sizeof(T))) & 15);
   const T* p = static_cast<const T*>(x);
   switch (mode) {
-#define CASE(m) case m: fp8_quantize_kernel<T, m><<<grid, THREADS, 0, stream>>>(p, rows, cols, ld, vec, o[0], o[1], o[2], o[3]); break
+#define CASE(m) case m: fp8_quantize_kernel<T, m><<<grid, THREADS, 0, stream>>>(p, rows, cols, ld, vec, across, o[0], o[1], o[2], o[3]); break
     CASE(ROWS);
     CASE(COLS);
     CASE(ROWS | COLS);
@@ -338,8 +339,8 @@ extern "C" int mb_fp8_quantize(const void* x, int type, int rows, int cols, long
   const int rt = (rows + B - 1) / B, ct = (cols + B - 1) / B;
   // the tiles past the end only write the padding of the exponent bytes
   const int gx = (mode & ROWS) ? (ct + 3) / 4 * 4 : ct, gy = (mode & COLS) ? (rt + 3) / 4 * 4 : rt;
-  if (gy > 65535) return -3;
+  if (static_cast<long long>(gx) * gy > 0x7fffffffll) return -3;
   uint8_t* o[4] = {static_cast<uint8_t*>(q), static_cast<uint8_t*>(sq), static_cast<uint8_t*>(qt), static_cast<uint8_t*>(sqt)};
-  return type == 0 ? launch<__nv_bfloat16>(mode, dim3(gx, gy), stream, x, rows, cols, ld, o)
-                   : launch<float>(mode, dim3(gx, gy), stream, x, rows, cols, ld, o);
+  return type == 0 ? launch<__nv_bfloat16>(mode, gx, gx * gy, stream, x, rows, cols, ld, o)
+                   : launch<float>(mode, gx, gx * gy, stream, x, rows, cols, ld, o);
 }

@@ -31,3 +31,16 @@ def test_results_of_one_column_or_row(M, N, dtype):
         assert (buf[:, 1:] == 7).all()
     if dtype == torch.float32:
         assert torch.equal(ops.matmul_fp8(a, b, out=out, accumulate=True), want + want)
+
+
+def test_more_rows_than_a_grid_dimension_counts():
+    n, at = 65535 * 128 + 257, 65534 * 128
+    x = torch.randn(n, 4, device="cuda")
+    q, part = ops.quantize_fp8(x), ops.quantize_fp8(x[at:])
+    assert torch.equal(q.data[at:].view(torch.uint8), part.data.view(torch.uint8))
+    assert torch.equal(q.scales[at // 128:], part.scales)
+    t, square = ops.quantize_fp8(x, transpose=True), ops.quantize_fp8(x, square=True)
+    assert torch.equal(t.data[:, at:].view(torch.uint8), ops.quantize_fp8(x[at:], transpose=True).data.view(torch.uint8))
+    assert torch.equal(square.scales[at // 128:], ops.quantize_fp8(x[at:], square=True).scales)
+    w = ops.quantize_fp8(torch.randn(8, 4, device="cuda"), square=True)
+    assert torch.equal(ops.linear_fp8(x, w)[at:], ops.linear_fp8(x[at:], w))
