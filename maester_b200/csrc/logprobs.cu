@@ -775,6 +775,7 @@ template <typename T>
 int fwd(const void* x, FwdArgs& p, cudaStream_t stream) {
   bool small;
   p.blocks = blocks_per_row(p.rows, p.V, sizeof(T), small);
+  if (static_cast<long long>(p.rows) * p.blocks > 0x7fffffffll) p.blocks = 1;
   return small ? fwd<T, 128>(x, p, stream) : fwd<T, 256>(x, p, stream);
 }
 
@@ -786,7 +787,7 @@ extern "C" int mb_logprobs_fwd(const void* x, const long long* tokens, int type,
                                float* logprob, float* entropy, int top, float* top_lp, long long* top_id, void* stats,
                                cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (V <= 0 || V > 0x7fffffff - 65536 || rows > 0x7fffffff / MAX_CLUSTER || top < 0 || top > MAX_TOP || top > V) return -3;
+  if (V <= 0 || V > 0x7fffffff - 65536 || top < 0 || top > MAX_TOP || top > V) return -3;
   if (type < T_BF16 || type > T_F32) return -3;
   int* status = mbh::status().dev;
   if (!status) return -4;
