@@ -6,7 +6,8 @@
 // instruction (16 x 8 x 32) does not care in which order the contraction comes, as long as both operands agree: the 16
 // neighbouring bytes that a lane reads are its values of two instructions, of w and of x alike, so neither operand is ever
 // rearranged.  The warps' sums meet in shared memory and are added in order.  The instruction cuts its sums off some 27 bits below
-// the largest term; a block's sum of 128 products is then added in rounded fp32 (8192 products of one sign: at most 4 units of 2^-24 off, 0.01 on average).
+// the largest term; a block's sum of 128 products is then added in rounded fp32 (8192 products of one sign: at most 4 units of
+// 2^-24 off, 0.01 on average).
 //
 // Measured with the quantiser, launches from a graph over 400 MB of weights: 4 tokens x 14336 x 4096 15.5 us (a kernel that only
 // reads the codes: 10.7), 1 x 4096 x 4096 7.3 us, 1 x 2560 x 10240 10.5 us; the tcgen05 kernel for few rows of fp8_gemm.cu took

@@ -3,8 +3,9 @@
 // With z = scale * x, m = max z, s = sum exp(z - m) and t = sum (z - m) exp(z - m):
 //   log p_j = (z_j - m) - log s,    H = log s - t / s   (every term of t has one sign: no cancellation)
 //   dx_j = scale * [ g (1[j = token] - p_j) - gH p_j (log p_j + H) + sum_a ga (1[j = alternative a] - p_j) ]
-// Statistics are 32-bit whatever the type of the logits.  -inf logits have probability 0 and gradient 0; a row without a
-// finite logit, or with NaN or +inf, has no distribution and comes out as NaN.
+// Statistics are 32-bit whatever the type of the logits.  -inf logits have probability 0 and the gradient 0, but for the own term
+// (g, ga) of the token and of alternatives; a row without a finite logit, or with NaN or +inf, has no distribution and comes out
+// as NaN.
 //
 // Forward: one pass over the logits, bound by reading them.  A row belongs to one block of 256 threads, or to a cluster of 2, 4
 // or 8 of them when rows are few (their results meet in the first block's shared memory), or to a block of 128 threads when

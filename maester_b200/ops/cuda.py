@@ -706,7 +706,6 @@ def moe_slot_dot(buf: torch.Tensor, slot_row: torch.Tensor, g: torch.Tensor, k: 
 
 # ------------------------------------------------------------------ token log-probabilities
 _LOGITS_TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-MAX_TOP = 64
 
 
 def _stream_of(t: torch.Tensor) -> int:
@@ -846,9 +845,6 @@ def fp8_linear_bwd(dy: torch.Tensor, K: int, x_t: torch.Tensor | None, w_t: torc
         _ck(_lib.lib().mb_fp8_linear_bwd(dy.data_ptr(), _LOGITS_TYPE[dy.dtype], dy.stride(0), M, K, N, work.data_ptr(), _ptr(w_t),
                                          _ptr(x_t), _ptr(dx), _ptr(dw), ld, out, _stream_of(dy)), "fp8_linear_bwd")
     return dx
-
-
-FP8_FEW = 8     # tokens that take the kernel for a decoding step
 
 
 def fp8_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:

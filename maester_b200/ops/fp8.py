@@ -9,8 +9,9 @@ the product that reads them, weights one for every 128 x 128 tile, so that a wei
 
 with sums in fp32, on the GPU those of its matrix units: 32 products at a time are added to a 32-bit sum, which is cut off, not
 rounded (so are products some 2^25 below the sum): 8192 products of one sign come out low by 4e-6 of their sum on average in
-the kernel for many rows, by 2e-7 in that for few, by nothing in that for up to eight tokens.  A NaN or an infinity becomes the NaN code (it reaches every output that reads it) and leaves its block's
-scale alone.  The reference project has no counterpart.
+the kernel for many rows, by 2e-7 in that for few, by nothing in that for up to eight tokens.  A NaN or an infinity becomes
+the NaN code (it reaches every output that reads it) and leaves its block's scale alone.  The reference project has no
+counterpart.
 """
 from __future__ import annotations
 
