@@ -11,10 +11,11 @@
 // A moving average changes by a few percent a step, or by a thousandth, and neighbouring codes are 6 to 12 percent apart: rounded
 // to nearest it would stand still (the second moment never decays at b2 >= 0.95, and hardly grows at 0.999).  So a value becomes
 // one of its two neighbouring codes lo < hi, at random, and its expectation stays what it was: m the upper one with probability
-// (m - lo) / (hi - lo), the root with (v - lo^2) / (hi^2 - lo^2), which keeps the expectation of v (that of r would add the
-// variance of every rounding to v).  A parameter's first step rounds to nearest: nothing has gone before it that a rounding could
-// hold fast, and the error is half as large where the bias correction weighs it most.  The random numbers are a hash of the step
-// number and the value's place, so that runs repeat.
+// (m - lo) / (hi - lo), the root r with (r^2 - lo^2) / (hi^2 - lo^2), which keeps the expectation of v (keeping that of r would
+// add the variance of every rounding to v).  (r^2 is v to 2^-23: holding v itself to the end costs 8 registers a thread, 3 % of the
+// time with fp32 and 8 % with bf16 parameters.)  A parameter's first step rounds to nearest: nothing has gone before it that a
+// rounding could hold fast, and the error is half as large where the bias correction weighs it most.  The random numbers are a
+// hash of the step number and the value's place, so that runs repeat.
 //
 // The moments are rounded to 32 bits operation by operation (no contraction), in the order written above: the codes do not
 // depend on what the compiler fuses.  The root is a reciprocal root with one Newton step, whose remainder is exact (the rounded
@@ -36,8 +37,8 @@ using namespace mbf8;
 
 constexpr int BLOCK = 256;    // values that share an exponent; one warp
 constexpr int WARP_BLOCKS = 4;                          // neighbouring blocks of a warp
-constexpr int CHUNK = 8 * WARP_BLOCKS * BLOCK;          // values of one thread block
-constexpr int THREADS = 256;
+constexpr int THREADS = 128;                            // (256: bf16 parameters 3 % slower)
+constexpr int CHUNK = THREADS / 32 * WARP_BLOCKS * BLOCK;   // values of one thread block
 constexpr int CAP_SMALL = 32, CAP_LARGE = 512;   // tensors of one launch: the table travels as a kernel argument of
 // 1.5 or 24 KiB (20 tensors: 10 us of the host's time with the small one, 14 with the large one)
 
@@ -158,22 +159,22 @@ __device__ __forceinline__ float code_below(float a, uint32_t add, float& gap) {
   gap = __uint_as_float(z & 0x7f800000u) * 0.125f;
   return __uint_as_float(z) - low;
 }
-// m / 2^k, and the root y of w (both in their units), as one of the two neighbouring codes; NaN stays
+// m / 2^k and a root / 2^k as one of the two neighbouring codes; NaN stays
 __device__ __forceinline__ float round_noisy(float y, uint32_t bits) {
   float gap;
   const float r = copysignf(code_below(fabsf(y), bits & 0xfffffu, gap), y);
   return y == y ? r : y;
 }
-__device__ __forceinline__ float round_root_noisy(float y, float w, uint32_t bits, float one) {
+__device__ __forceinline__ float round_root_noisy(float y, uint32_t bits, float one) {
   float gap;
   const float lo = code_below(y, 0u, gap), q = gap * (2.f * lo + gap);            // hi^2 - lo^2: exact, as all is here but u q
   const float t = __fmaf_rn(__fmul_rn(one_plus(bits), q), one, fmaf(lo, lo, -q));   // lo^2 + u q
-  float r = w > t ? lo + gap : lo;
+  float r = __fmul_rn(y, y) > t ? lo + gap : lo;
   if (y > 0.f) r = fmaxf(r, 0.001953125f);
   return y == y ? r : y;
 }
 // the same for eight values that are no smaller than NORMAL
-__device__ __forceinline__ void round_all(float2 (&m)[4], float2 (&r)[4], const float2 (&w)[4], uint32_t x, float one) {
+__device__ __forceinline__ void round_all(float2 (&m)[4], float2 (&r)[4], uint32_t x, float one) {
   const float2 one2 = make_float2(one, one), two = make_float2(2.f, 2.f);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -186,8 +187,8 @@ __device__ __forceinline__ void round_all(float2 (&m)[4], float2 (&r)[4], const 
     const float2 gap = mul2(make_float2(__uint_as_float(lx & 0x7f800000u), __uint_as_float(ly & 0x7f800000u)), 0.125f);
     const float2 q = mul2(gap, fma2(lo, two, gap));
     const float2 t = fma2(mul2(make_float2(one_plus(a), one_plus(b)), q), one2, fma2(lo, lo, make_float2(-q.x, -q.y)));
-    const float2 hi = fma2(lo, one2, gap);
-    r[j] = make_float2(w[j].x > t.x ? hi.x : lo.x, w[j].y > t.y ? hi.y : lo.y);
+    const float2 hi = fma2(lo, one2, gap), w = mul2(r[j], r[j]);
+    r[j] = make_float2(w.x > t.x ? hi.x : lo.x, w.y > t.y ? hi.y : lo.y);
   }
 }
 
@@ -271,16 +272,13 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
     }
   }
   float am = 0.f, av = 0.f;                       // NaN if there is one
-  float least = INFINITY, least_m = INFINITY;     // over what is not NaN
+  float least = INFINITY;                         // over what is not NaN
   const float2 one = make_float2(h.one, h.one);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     m[j] = fma2(mul2(m[j], h.b1), one, mul2(d[j], h.omb1));
     v[j] = fma2(mul2(v[j], h.b2), one, mul2(mul2(d[j], d[j]), h.omb2));
-    if (EIGHT) {
-      am = max_nan(max_nan(am, fabsf(m[j].x)), fabsf(m[j].y));
-      least_m = fminf(fminf(least_m, fabsf(m[j].x)), fabsf(m[j].y));
-    }
+    if (EIGHT) am = max_nan(max_nan(am, fabsf(m[j].x)), fabsf(m[j].y));
     av = max_nan(max_nan(av, v[j].x), v[j].y);
     least = fminf(fminf(least, v[j].x), v[j].y);
   }
@@ -293,9 +291,6 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
       store_some(st.v32 + s0 + e, n - e, v);
     }
   }
-  float2 w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = v[j];
   if (least >= ROOT_FROM && av < ROOT_TO) {      // v becomes its root (NaN stays)
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = root2(v[j]);
@@ -350,11 +345,14 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
     }
     if (h.noisy) {
       const uint32_t x = first_noise(static_cast<uint32_t>((s0 >> 3) + lane), h.key);
+      float small = INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = mul2(w[j], ir * ir);
+      for (int j = 0; j < 4; ++j) small = fminf(fminf(small, fabsf(m[j].x)), fabsf(m[j].y));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) small = fminf(fminf(small, v[j].x), v[j].y);
       // (a whole warp goes one way; the margin over 2^-12 covers the roots' roundings)
-      if (!__any_sync(~0u, odd || !(least * (ir * ir) >= 2.45e-4f && least_m * im >= NORMAL))) {
-        round_all(m, v, w, x, h.one);
+      if (!__any_sync(~0u, odd || !(small >= NORMAL))) {
+        round_all(m, v, x, h.one);
       } else {
         uint32_t y = x;
 #pragma unroll
@@ -362,7 +360,7 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
           const uint32_t a = bits_of(y), b = bits_of(y = next_noise(y));
           y = next_noise(y);
           m[j] = make_float2(round_noisy(m[j].x, a), round_noisy(m[j].y, b));
-          v[j] = make_float2(round_root_noisy(v[j].x, w[j].x, a, h.one), round_root_noisy(v[j].y, w[j].y, b, h.one));
+          v[j] = make_float2(round_root_noisy(v[j].x, a, h.one), round_root_noisy(v[j].y, b, h.one));
         }
       }
     } else if (!(least * (ir * ir) >= 3.9e-6f)) {
@@ -378,7 +376,7 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
 }
 
 template <typename P, bool EIGHT, int CAP>
-__global__ void __launch_bounds__(THREADS, 4)
+__global__ void __launch_bounds__(THREADS, 8)
 adamw_multi_kernel(const __grid_constant__ Table<CAP> tab, const Hyper h, const States st) {
   int lo = 0, hi = tab.count - 1;
   const int chunk = blockIdx.x;

@@ -320,29 +320,29 @@ def state_round(y: torch.Tensor, noise: torch.Tensor) -> torch.Tensor:
     return torch.where(y.isnan(), y, torch.copysign(a, y))
 
 
-def state_round_root(y: torch.Tensor, w: torch.Tensor, noise: torch.Tensor) -> torch.Tensor:
-    """The root ``y`` of ``w`` rounded to one of its two neighbouring codes, so that the expectation of its SQUARE is ``w``;
+def state_round_root(y: torch.Tensor, noise: torch.Tensor) -> torch.Tensor:
+    """Values in [0, 448] rounded to one of their two neighbouring codes, so that the expectation of the SQUARE is the value's;
     what is not zero does not become zero."""
     lo, gap = _code_below(y, 0)
     u1 = ((noise >> 9).to(torch.int32) | 0x3F800000).view(torch.float32)        # 1 + u
     q = gap * (2 * lo + gap)                                                      # hi^2 - lo^2
-    out = torch.where(w > u1 * q + (lo * lo - q), lo + gap, lo)
+    out = torch.where(y * y > u1 * q + (lo * lo - q), lo + gap, lo)
     out = torch.where(y > 0, out.clamp_min(E4M3_TINY), out)
     return torch.where(y.isnan(), y, out)
 
 
-def state_encode(x: torch.Tensor, root: bool = False, noise: torch.Tensor | None = None,
-                 square: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+def state_encode(x: torch.Tensor, root: bool = False,
+                 noise: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes and biased block exponents of a flat state whose length is a multiple of 256; ``root``: a value that is not
     zero does not become zero.  Rounded to nearest, or with ``noise`` (``state_noise``) to a neighbour whose expectation is
-    the value, for a root (of ``square``) in the squares.  What is a code already stays one."""
+    the value, for a root in the squares.  What is a code already stays one."""
     b = x.view(-1, STATE_BLOCK)
     k = fp8_block_exponents(_finite_abs(b).amax(dim=1), ROOT_MIN_EXP if root else STATE_MIN_EXP)
     y = b * pow2(-k)[:, None]
     if noise is not None:
         y = torch.where(y.isinf(), torch.full_like(y, math.nan), y)
         n = noise.view(-1, STATE_BLOCK)
-        y = state_round_root(y, square.view(-1, STATE_BLOCK) * pow2(-2 * k)[:, None], n) if root else state_round(y, n)
+        y = state_round_root(y, n) if root else state_round(y, n)
     elif root:
         y = torch.where(y > 0, y.clamp_min(E4M3_TINY), y)
     return y.to(torch.float8_e4m3fn).view(-1), (k + 127).to(torch.uint8)

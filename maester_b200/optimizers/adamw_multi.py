@@ -309,10 +309,9 @@ class AdamWMulti(Optimizer):
         if root is None and v is not None:
             root = v.sqrt()
         noise = None if step < NOISE_FROM else ref.state_noise(step, off, end - off, self.device)
-        padded = lambda x: None if x is None else torch.nn.functional.pad(x, (0, end - off - n))
-        for k, x, square in (("exp_avg", m, None), ("exp_avg_root", root, v)):
+        for k, x, is_root in (("exp_avg", m, False), ("exp_avg_root", root, True)):
             if x is not None:
-                codes, exps = ref.state_encode(padded(x), square is not None, noise, padded(square))
+                codes, exps = ref.state_encode(torch.nn.functional.pad(x, (0, end - off - n)), is_root, noise)
                 f[k][off:end].copy_(codes)
                 f[k + "_exp"][blk].copy_(exps)
 
