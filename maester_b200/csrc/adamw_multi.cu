@@ -24,9 +24,10 @@
 // The step moves 18 bytes a value with 8-bit states beside 32-bit parameters and their 16-bit copy (30 with 32-bit states) and
 // is bound by that.  A warp owns 256 consecutive values at a time, so a block's maximum is one warp reduction.
 //
-// Measured (24 tensors of 4096 x 4096; copy rate 6540 GB/s): fp32 parameters with a copy 1081 us with 8-bit states (6710 GB/s),
-// 1799 us with 32-bit ones (6710); bf16 parameters 769 us with 8-bit states (5240: the codes cost more instructions than the 10
-// bytes of a value cost time), 1339 us with 32-bit ones (6610).  Small tensors are the host's: 40 us for 20 of them.
+// Measured (24 tensors of 4096 x 4096; copy rate 6540 GB/s): fp32 parameters with a copy 1130 us with 8-bit states (6420 GB/s),
+// 1801 us with 32-bit ones (6710); bf16 parameters 856 us with 8-bit states (4710: the codes cost more instructions than the 10
+// bytes of a value cost time), 1341 us with 32-bit ones (6610).  Of the 8-bit times the noise costs some 40 and 90 us (hash,
+// neighbouring codes, comparison: 15 instructions a value).  Small tensors are the host's: 45 to 55 us for 20 of them.
 #include "fp8_common.cuh"
 #include "host_common.cuh"
 #include <math.h>
@@ -36,9 +37,10 @@ namespace {
 using namespace mbf8;
 
 constexpr int BLOCK = 256;    // values that share an exponent; one warp
-constexpr int WARP_BLOCKS = 4;                          // neighbouring blocks of a warp
 constexpr int THREADS = 128;                            // (256: bf16 parameters 3 % slower)
-constexpr int CHUNK = THREADS / 32 * WARP_BLOCKS * BLOCK;   // values of one thread block
+// neighbouring blocks of a warp (with 32-bit states 8 are 2 % slower; with 8-bit ones 4 are as much slower)
+constexpr int warp_blocks(bool eight) { return eight ? 8 : 4; }
+constexpr int chunk_of(bool eight) { return THREADS / 32 * warp_blocks(eight) * BLOCK; }   // values of one thread block
 constexpr int CAP_SMALL = 32, CAP_LARGE = 512;   // tensors of one launch: the table travels as a kernel argument of
 // 1.5 or 24 KiB (20 tensors: 10 us of the host's time with the small one, 14 with the large one)
 
@@ -140,7 +142,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // ---- noise: 32 random bits for each of the 8 values of a lane, a hash of their group's place and a linear congruence after it.
-// The upper 23 bits round the root, the lower 20 the first moment (what they share weighs 2^-13 and less in the root's).
+// The lower 23 bits round the root, the upper 20 the first moment (what they share weighs 2^-10 and less in the latter's).
 __device__ __forceinline__ uint32_t first_noise(uint32_t group, uint32_t key) {
   uint32_t x = group * 0x9E3779B9u + key;
   x = (x ^ (x >> 16)) * 0xB7E15163u;
@@ -148,8 +150,7 @@ __device__ __forceinline__ uint32_t first_noise(uint32_t group, uint32_t key) {
   return x ^ (x >> 16);
 }
 __device__ __forceinline__ uint32_t next_noise(uint32_t x) { return x * 0x6A09E667u + 0xBB67AE85u; }
-__device__ __forceinline__ uint32_t bits_of(uint32_t x) { return x ^ (x >> 16); }
-__device__ __forceinline__ float one_plus(uint32_t bits) { return __uint_as_float(0x3f800000u | (bits >> 9)); }
+__device__ __forceinline__ float one_plus(uint32_t bits) { return __uint_as_float(0x3f800000u | (bits & 0x7fffffu)); }
 
 constexpr float NORMAL = 0.015625f;   // 2^-6: below it codes keep the distance 2^-9
 // the largest code that is at most a in [0, 448], after `add` units of 2^-20 of a code's last place; its distance to the next
@@ -162,33 +163,31 @@ __device__ __forceinline__ float code_below(float a, uint32_t add, float& gap) {
 // m / 2^k and a root / 2^k as one of the two neighbouring codes; NaN stays
 __device__ __forceinline__ float round_noisy(float y, uint32_t bits) {
   float gap;
-  const float r = copysignf(code_below(fabsf(y), bits & 0xfffffu, gap), y);
+  const float r = copysignf(code_below(fabsf(y), bits >> 12, gap), y);
   return y == y ? r : y;
 }
-__device__ __forceinline__ float round_root_noisy(float y, uint32_t bits, float one) {
+__device__ __forceinline__ float round_root_noisy(float y, uint32_t bits) {
   float gap;
-  const float lo = code_below(y, 0u, gap), q = gap * (2.f * lo + gap);            // hi^2 - lo^2: exact, as all is here but u q
-  const float t = __fmaf_rn(__fmul_rn(one_plus(bits), q), one, fmaf(lo, lo, -q));   // lo^2 + u q
-  float r = __fmul_rn(y, y) > t ? lo + gap : lo;
+  const float lo = code_below(y, 0u, gap), q = gap * (2.f * lo + gap);      // hi^2 - lo^2: exact, as lo^2 - q is
+  float r = __fmul_rn(y, y) > fmaf(one_plus(bits), q, fmaf(lo, lo, -q)) ? lo + gap : lo;    // lo^2 + u q
   if (y > 0.f) r = fmaxf(r, 0.001953125f);
   return y == y ? r : y;
 }
 // the same for eight values that are no smaller than NORMAL
-__device__ __forceinline__ void round_all(float2 (&m)[4], float2 (&r)[4], uint32_t x, float one) {
-  const float2 one2 = make_float2(one, one), two = make_float2(2.f, 2.f);
+__device__ __forceinline__ void round_all(float2 (&m)[4], float2 (&r)[4], uint32_t x) {
+  const float2 two = make_float2(2.f, 2.f);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t a = bits_of(x), b = bits_of(x = next_noise(x));
-    x = next_noise(x);
-    m[j].x = __uint_as_float((__float_as_uint(m[j].x) + (a & 0xfffffu)) & 0xfff00000u);
-    m[j].y = __uint_as_float((__float_as_uint(m[j].y) + (b & 0xfffffu)) & 0xfff00000u);
+    const uint32_t a = x, b = next_noise(x);
+    x = next_noise(b);
+    m[j].x = __uint_as_float((__float_as_uint(m[j].x) + (a >> 12)) & 0xfff00000u);
+    m[j].y = __uint_as_float((__float_as_uint(m[j].y) + (b >> 12)) & 0xfff00000u);
     const uint32_t lx = __float_as_uint(r[j].x) & 0xfff00000u, ly = __float_as_uint(r[j].y) & 0xfff00000u;
     const float2 lo = make_float2(__uint_as_float(lx), __uint_as_float(ly));
     const float2 gap = mul2(make_float2(__uint_as_float(lx & 0x7f800000u), __uint_as_float(ly & 0x7f800000u)), 0.125f);
-    const float2 q = mul2(gap, fma2(lo, two, gap));
-    const float2 t = fma2(mul2(make_float2(one_plus(a), one_plus(b)), q), one2, fma2(lo, lo, make_float2(-q.x, -q.y)));
-    const float2 hi = fma2(lo, one2, gap), w = mul2(r[j], r[j]);
-    r[j] = make_float2(w.x > t.x ? hi.x : lo.x, w.y > t.y ? hi.y : lo.y);
+    const float2 q = mul2(gap, fma2(lo, two, gap)), w = mul2(r[j], r[j]);
+    const float2 t = fma2(make_float2(one_plus(a), one_plus(b)), q, fma2(lo, lo, make_float2(-q.x, -q.y)));
+    r[j] = make_float2(__uint_as_float(w.x > t.x ? lx + 0x100000u : lx), __uint_as_float(w.y > t.y ? ly + 0x100000u : ly));
   }
 }
 
@@ -348,19 +347,17 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
       float small = INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) small = fminf(fminf(small, fabsf(m[j].x)), fabsf(m[j].y));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) small = fminf(fminf(small, v[j].x), v[j].y);
       // (a whole warp goes one way; the margin over 2^-12 covers the roots' roundings)
-      if (!__any_sync(~0u, odd || !(small >= NORMAL))) {
-        round_all(m, v, x, h.one);
+      if (!__any_sync(~0u, odd || !(least * (ir * ir) >= 2.45e-4f && small >= NORMAL))) {
+        round_all(m, v, x);
       } else {
         uint32_t y = x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t a = bits_of(y), b = bits_of(y = next_noise(y));
-          y = next_noise(y);
+          const uint32_t a = y, b = next_noise(y);
+          y = next_noise(b);
           m[j] = make_float2(round_noisy(m[j].x, a), round_noisy(m[j].y, b));
-          v[j] = make_float2(round_root_noisy(v[j].x, a, h.one), round_root_noisy(v[j].y, b, h.one));
+          v[j] = make_float2(round_root_noisy(v[j].x, a), round_root_noisy(v[j].y, b));
         }
       }
     } else if (!(least * (ir * ir) >= 3.9e-6f)) {
@@ -378,6 +375,7 @@ __device__ __forceinline__ uint2 next_block(P* p, const P* g, __nv_bfloat16* cop
 template <typename P, bool EIGHT, int CAP>
 __global__ void __launch_bounds__(THREADS, 8)
 adamw_multi_kernel(const __grid_constant__ Table<CAP> tab, const Hyper h, const States st) {
+  constexpr int WARP_BLOCKS = warp_blocks(EIGHT), CHUNK = chunk_of(EIGHT);
   int lo = 0, hi = tab.count - 1;
   const int chunk = blockIdx.x;
   while (lo < hi) {
@@ -427,7 +425,7 @@ int launch(const Tensor* rows, int& at, int count, bool bf16, bool eight, const 
   while (at < count && tab.count < CAP) {
     Tensor t = rows[at];
     if (t.n < 0 || (t.off & (BLOCK - 1))) return -3;
-    const long long c = (t.n + CHUNK - 1) / CHUNK;
+    const long long c = (t.n + chunk_of(eight) - 1) / chunk_of(eight);
     if (chunks + c > 0x7fffffffll) {
       if (!tab.count) return -3;
       break;

@@ -302,7 +302,7 @@ def state_noise(step: int, first: int, n: int, device=None) -> torch.Tensor:
     for j in range(1, 8):
         x = x * 0x6A09E667 + 0xBB67AE85 & m32
         out = torch.where(i & 7 == j, x, out)
-    return out ^ (out >> 16)
+    return out
 
 
 def _code_below(a: torch.Tensor, add) -> tuple[torch.Tensor, torch.Tensor]:
@@ -316,7 +316,7 @@ def _code_below(a: torch.Tensor, add) -> tuple[torch.Tensor, torch.Tensor]:
 
 def state_round(y: torch.Tensor, noise: torch.Tensor) -> torch.Tensor:
     """Values in [-448, 448] rounded to one of their two neighbouring codes, so that the expectation is the value."""
-    a, _ = _code_below(y.abs(), (noise & 0xFFFFF).to(torch.int32))
+    a, _ = _code_below(y.abs(), (noise >> 12).to(torch.int32))
     return torch.where(y.isnan(), y, torch.copysign(a, y))
 
 
@@ -324,9 +324,10 @@ def state_round_root(y: torch.Tensor, noise: torch.Tensor) -> torch.Tensor:
     """Values in [0, 448] rounded to one of their two neighbouring codes, so that the expectation of the SQUARE is the value's;
     what is not zero does not become zero."""
     lo, gap = _code_below(y, 0)
-    u1 = ((noise >> 9).to(torch.int32) | 0x3F800000).view(torch.float32)        # 1 + u
+    u1 = ((noise & 0x7FFFFF).to(torch.int32) | 0x3F800000).view(torch.float32)  # 1 + u
     q = gap * (2 * lo + gap)                                                      # hi^2 - lo^2
-    out = torch.where(y * y > u1 * q + (lo * lo - q), lo + gap, lo)
+    at = (u1.double() * q.double() + (lo * lo - q).double()).float()              # lo^2 + u q, rounded once
+    out = torch.where(y * y > at, lo + gap, lo)
     out = torch.where(y > 0, out.clamp_min(E4M3_TINY), out)
     return torch.where(y.isnan(), y, out)
 
