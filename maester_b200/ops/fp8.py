@@ -48,6 +48,8 @@ class Fp8Blocks:
             raise ValueError(f"scales have to be contiguous uint8 {want}, got {scales.dtype} {tuple(scales.shape)}")
         if scales.device != data.device:
             raise ValueError(f"scales are on {scales.device}, codes on {data.device}")
+        if data.is_cuda and (data.data_ptr() | scales.data_ptr()) & 15:
+            raise ValueError("codes and scales have to start on a 16-byte boundary (parts of a larger buffer may not)")
         self.data, self.scales, self.cols = data, scales, cols
 
     @property

@@ -89,3 +89,20 @@ def test_sums_of_one_sign(kind, M, N):
     a, b, y = _product(kind, torch.rand(M, K, device="cuda") + 0.5, torch.rand(N, K, device="cuda") + 0.5)
     want = a.double() @ b.double().T
     assert ((y - want).abs() <= K / 32 * (2.0 ** -23 + 32 * 2.0 ** -25) / 2 * want).all()
+
+
+def test_codes_that_start_off_a_boundary_are_refused():
+    q = ops.quantize_fp8(torch.randn(40, 200, device="cuda"), square=True)
+    for at, ok in ((16, True), (8, False), (1, False)):
+        codes = torch.zeros(40 * 256 + at, device="cuda", dtype=torch.uint8)[at:].view(torch.float8_e4m3fn).view(40, 256)
+        scales = torch.zeros(q.scales.numel() + at, device="cuda", dtype=torch.uint8)[at:].view(q.scales.shape)
+        codes.copy_(q.data)
+        scales.copy_(q.scales)
+        for args in ((codes, q.scales), (q.data, scales)):
+            if ok:
+                w = ops.Fp8Blocks(*args, 200)
+                x = torch.randn(3, 200, device="cuda")
+                assert torch.equal(ops.linear_fp8(x, w), ops.linear_fp8(x, q))
+            else:
+                with pytest.raises(ValueError, match="16-byte"):
+                    ops.Fp8Blocks(*args, 200)
