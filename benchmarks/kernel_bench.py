@@ -237,6 +237,7 @@ def bench_ce(iters: int, small: bool) -> None:
 
 def bench_logprobs(iters: int, small: bool) -> None:
     """Token log-probabilities, entropies and alternatives, and the gradient: one read, or one read and one write, of the logits."""
+    from maester_b200 import ops
     _, bw_peak = _peaks()
     shapes = [(4096, 32000)] if small else [(16, 262144), (4096, 128256), (8192, 32000)]
     warm = 0 if small else 3
@@ -253,6 +254,29 @@ def bench_logprobs(iters: int, small: bool) -> None:
         t = timeit(lambda: C.logprobs_bwd(x, tokens, 1.0, st, g, g, None, None), iters, warm)
         print(f"logprobs [{R} x {V}] gradient with entropy: {t * 1e3:.1f} us {2 * nb / t / 1e6:.0f} GB/s "
               f"({2 * nb / t / 1e6 / bw_peak:.2f} of measured)")
+        ids = C.logprobs_fwd(x, tokens, 1.0, True, 20, True)[3]
+        g_top = torch.randn(R, 20, device="cuda")
+        t = timeit(lambda: C.logprobs_bwd(x, tokens, 1.0, st, g, g, ids, g_top), iters, warm)
+        print(f"logprobs [{R} x {V}] gradient with entropy and 20 alternatives: {t * 1e3:.1f} us {2 * nb / t / 1e6:.0f} GB/s "
+              f"({2 * nb / t / 1e6 / bw_peak:.2f} of measured)")
+    # from hidden states: beside the products alone (one forward; forward again and two behind the gradient)
+    for R, D, V in [(1024, 1024, 32000)] if small else [(4096, 2560, 262144), (4096, 2560, 50257)]:
+        h = torch.randn(R, D, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        w = (torch.randn(V, D, device="cuda") * 0.02).bfloat16().requires_grad_(True)
+        w.main_grad = torch.zeros(V, D, device="cuda")
+        tokens = torch.randint(0, V, (R,), device="cuda")
+        g = torch.randn(R, device="cuda")
+        one = timeit(lambda: ops.linear(h.detach(), w.detach()), iters, warm)
+
+        def both():
+            out = ops.linear_logprobs(h, w, tokens, entropy=True)
+            torch.autograd.grad([out.logprobs, out.entropy], [h], [g, g], retain_graph=False, allow_unused=True)
+
+        with torch.no_grad():
+            t = timeit(lambda: ops.linear_logprobs(h, w, tokens, entropy=True), iters, warm)
+        print(f"linear logprobs [{R} x {D}] -> {V}: {t:.3f} ms (the product alone, 16-bit logits: {one:.3f})")
+        t = timeit(both, iters, warm)
+        print(f"linear logprobs [{R} x {D}] -> {V}, with gradients: {t:.3f} ms (four products: {4 * one:.3f})")
     C.check_status()
 
 
@@ -268,6 +292,10 @@ def bench_fp8(iters: int, small: bool) -> None:
         t = timeit(lambda: C.fp8_quantize(x, *mode), iters, warm)
         nb = M * K * (2 + out)
         print(f"fp8 quantise {name:17s} [{M} x {K}]: {t * 1e3:.1f} us {nb / t / 1e6:.0f} GB/s ({nb / t / 1e6 / bw_peak:.2f} of measured)")
+    x32 = torch.randn(M, K, device="cuda")
+    t = timeit(lambda: C.fp8_quantize(x32, True, True, False), iters, warm)
+    nb = M * K * 6
+    print(f"fp8 quantise fp32, rows and columns [{M} x {K}]: {t * 1e3:.1f} us {nb / t / 1e6:.0f} GB/s ({nb / t / 1e6 / bw_peak:.2f} of measured)")
     for M, N, K in [(8192, 4096, 4096)] if small else [(16384, 4096, 4096), (16384, 20480, 2560), (16384, 2560, 10240)]:
         a = ops.quantize_fp8(torch.randn(M, K, device="cuda", dtype=torch.bfloat16))
         b = ops.quantize_fp8(torch.randn(N, K, device="cuda", dtype=torch.bfloat16) * 0.02, square=True)
@@ -275,6 +303,10 @@ def bench_fp8(iters: int, small: bool) -> None:
         t = timeit(lambda: C.fp8_gemm(a.data, a.scales, b.data, b.scales, out), iters, warm)
         fl = 2 * M * N * K
         print(f"fp8 product [{M} x {N} x {K}]: {t:.3f} ms {fl / t / 1e9:6.0f} TF ({fl / t / 1e9 / tf_peak:.2f} of measured bf16)")
+        # a weight's gradient, added to what earlier micro-batches left: the rows are the contraction
+        c, d, main = ops.quantize_fp8(torch.randn(N, M, device="cuda")), ops.quantize_fp8(torch.randn(K, M, device="cuda")), torch.zeros(N, K, device="cuda")
+        t = timeit(lambda: C.fp8_gemm(c.data, c.scales, d.data, d.scales, main, True), iters, warm)
+        print(f"fp8 product added to fp32 [{N} x {K} x {M}]: {t:.3f} ms {fl / t / 1e9:6.0f} TF ({fl / t / 1e9 / tf_peak:.2f} of measured bf16)")
     N, K = 14336, 4096
     weights = [ops.quantize_fp8(torch.randn(N, K, device="cuda", dtype=torch.bfloat16), square=True) for _ in range(1 if small else 8)]
     for M in (1, 4, 8, 16, 64):
