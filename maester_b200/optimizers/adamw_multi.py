@@ -37,8 +37,9 @@ def _missing(x: torch.Tensor) -> int:
 
 
 def _overlap(tensors) -> bool:
-    """Do two of these contiguous tensors share memory?"""
-    spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in tensors if x.numel())
+    """Do two of these contiguous tensors share memory?  (One whose storage has been freed has none.)"""
+    spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in tensors
+                   if x.numel() and x.untyped_storage().nbytes())
     return any(a[1] > b[0] > 0 for a, b in zip(spans, spans[1:]))
 
 

@@ -107,3 +107,16 @@ def test_copies_that_share_memory_are_refused():
     opt.attach_copies({q: torch.zeros(70, dtype=torch.bfloat16)})
     _stepped(opt, [p, q])
     assert torch.equal(low[:50], p.detach().bfloat16())
+
+
+def test_parameters_may_move_while_copies_have_no_memory():
+    params = [torch.nn.Parameter(torch.randn(300)) for _ in range(2)]
+    opt = AdamWMulti(params, lr=0.1)
+    low = [torch.zeros(500, dtype=torch.bfloat16) for _ in range(2)]
+    opt.attach_copies({params[0]: low[0][10:310], params[1]: low[1][100:400]})
+    for x in low:
+        x.untyped_storage().resize_(0)
+    params[0].data = params[0].data.clone()
+    before = params[0].detach().clone()
+    _stepped(opt, params)
+    assert not torch.equal(params[0], before)
