@@ -347,8 +347,8 @@ class AdamWMulti(Optimizer):
         """Moments and step numbers become those of ``state_dict``; a parameter, or a part of its state, that is not in it
         starts afresh."""
         every = [p for g in self.param_groups for p in g["params"]]
-        states = [state_dict["state"].get(i, {}) for i in range(len(every))]
-        for p, state in zip(every, states):
+        states = [state_dict["state"].get(i, {}) for g in state_dict["param_groups"] for i in g["params"]]
+        for p, state in zip(every, states):     # (as many as there are, or the next call says so)
             self._fits(p, state)
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for k, x in self._buffers.items():

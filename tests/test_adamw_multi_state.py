@@ -131,3 +131,22 @@ def test_settings_that_it_does_not_follow_are_refused(key):
         p.grad = torch.ones_like(p)
     with pytest.raises(RuntimeError, match=key):
         opt.step()
+
+
+def test_a_state_is_found_by_the_names_that_its_groups_give():
+    """As torch.optim's: the entries of ``state`` are named by the groups' ``params``, whatever they are."""
+    params = _params()
+    opt = AdamWMulti(params, lr=1e-2)
+    _run(opt, params, 2)
+    sd = copy.deepcopy(opt.state_dict())
+    names = ["c", "a", "b"]
+    sd["state"] = {names[i]: s for i, s in sd["state"].items()}
+    sd["param_groups"][0]["params"] = names
+    want = [opt._moments(p)[0].clone() for p in params]
+    _run(opt, params, 1)
+    opt.load_state_dict(sd)
+    assert all(torch.equal(opt._moments(p)[0], m) and opt._slots[p].step == 2 for p, m in zip(params, want))
+    del sd["param_groups"][0]["params"][0]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(sd)
+    assert all(opt._slots[p].step == 2 for p in params)
