@@ -116,8 +116,14 @@ class AdamWMulti(Optimizer):
             b.table = np.array([(0, 0, 0, s.numel, s.offset, 0) for s in b.slots], dtype=np.int64)
             self._take_memory(b)
         self._copy_storages, self._copy_memory = [], []       # of the 16-bit copies: theirs once each, and where they were
+        self._mark()
         self.writes_lowp = False    # the sharding runtime's 16-bit parameters are written by step()
         self._sealed = True
+
+    def _mark(self) -> None:
+        """Entries in ``state``: torch's checkpoint helpers let an optimizer without any step with zeros first."""
+        for p in self._slots:
+            self.state[p] = {}
 
     def add_param_group(self, group) -> None:
         if self._sealed:
@@ -351,6 +357,7 @@ class AdamWMulti(Optimizer):
         for p, state in zip(every, states):     # (as many as there are, or the next call says so)
             self._fits(p, state)
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        self._mark()
         for k, x in self._buffers.items():
             x.view(torch.uint8).fill_(0 if not k.endswith("_exp") else
                                       127 + (ref.ROOT_MIN_EXP if "root" in k else ref.STATE_MIN_EXP))

@@ -150,3 +150,27 @@ def test_a_state_is_found_by_the_names_that_its_groups_give():
     with pytest.raises(ValueError):
         opt.load_state_dict(sd)
     assert all(opt._slots[p].step == 2 for p in params)
+
+
+def test_torch_checkpoint_helpers_leave_the_states_alone():
+    """They take an optimizer whose ``state`` is empty for one that has never stepped, and let it step with zeros."""
+    from torch.distributed.checkpoint.state_dict import get_optimizer_state_dict, set_optimizer_state_dict
+    torch.manual_seed(0)
+    m = torch.nn.Sequential(torch.nn.Linear(20, 30), torch.nn.Linear(30, 5))
+    params = list(m.parameters())
+    opt = AdamWMulti(params, lr=1e-2)
+    _run(opt, params, 2)
+    opt.zero_grad()
+    want = [[x.clone() for x in opt._moments(p)] for p in params]
+    for again in range(2):
+        sd = get_optimizer_state_dict(m, opt)
+        assert [s.step for s in opt._slots.values()] == [2] * 4
+        for p, w in zip(params, want):
+            assert all(torch.equal(x, y) for x, y in zip(opt._moments(p), w))
+        assert torch.equal(sd["state"]["1.weight"]["exp_avg"], want[2][0].view(5, 30))
+        _run(opt, params, 1)
+        opt.zero_grad()
+        set_optimizer_state_dict(m, opt, sd)
+    assert [s.step for s in opt._slots.values()] == [2] * 4
+    for p, w in zip(params, want):
+        assert all(torch.equal(x, y) for x, y in zip(opt._moments(p), w))
